@@ -85,9 +85,14 @@ SIGNATURES = {
     "ab200_module_info": [_i, _vp, _vp, _vp, _i],
     "ab200_module_tensor": [_i, _i, _vp, _i, _vp, _i, _vp, _vp],
     "ab200_forward_host_ns": [_i, _vp, _i, _vp, _i, _vp],
+    "ab200_kv8_append": [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _vp, _vp, _l, _l, _vp, _l, _vp, _l, _i, _vp, _i, _vp],
+    "ab200_kv8_read": [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp],
+    "ab200_kv8_attention": [_vp, _l, _vp] + [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp],
+    "ab200_kv8_step": [_vp] * 3 + [_l] * 3 + [_vp] * 5 + [_i] * 3 + [_vp, _l, _i, _vp, _i, _i, _i, _i, _vp, _f, _i, _vp, _sz, _vp],
+    "ab200_kv_copy_pages": [_i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp],
     "ab200_greedy_next": [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp],
 }
-OTHER_SYMBOLS = ["ab200_last_error", "ab200_abi_version", "ab200_w4a16_gemv_workspace_bytes", "ab200_comm_buffer_bytes",
+OTHER_SYMBOLS = ["ab200_last_error", "ab200_abi_version", "ab200_w4a16_gemv_workspace_bytes", "ab200_comm_buffer_bytes", "ab200_kv8_attention_workspace_bytes",
                  "ab200_comm_emulation_scratch_bytes", "ab200_w4a16_gemv_emulation_scratch_bytes"]
 
 _lib = None
@@ -110,6 +115,8 @@ def load():
         L.ab200_abi_version.restype = ctypes.c_int
         L.ab200_w4a16_gemv_workspace_bytes.restype = ctypes.c_size_t
         L.ab200_w4a16_gemv_workspace_bytes.argtypes = [_i, _i, _i]
+        L.ab200_kv8_attention_workspace_bytes.restype = ctypes.c_size_t
+        L.ab200_kv8_attention_workspace_bytes.argtypes = [_i, _i, _i, _i, _i]
         L.ab200_comm_buffer_bytes.restype = ctypes.c_size_t
         L.ab200_comm_buffer_bytes.argtypes = [_i, _i]
         L.ab200_comm_emulation_scratch_bytes.restype = ctypes.c_size_t

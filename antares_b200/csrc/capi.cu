@@ -2,7 +2,7 @@
 #include <stdarg.h>
 #include <string.h>
 
-#include "common.cuh"
+#include "kv8.cuh"
 
 namespace ab200 {
 
@@ -103,6 +103,7 @@ extern "C" int ab200_kernel_status(int *status_host) {
   if (*status_host != 0) {
     const int zero = 0;
     AB200_CUDA(cudaMemcpyToSymbol(g_kernel_error, &zero, sizeof(int)));
+    if (*status_host == KV8_BAD_PAGE) return fail(AB200_EINVAL, "a page table entry outside the cache was used (site %d)", *status_host);
     return fail(AB200_ETIMEOUT, "a bounded wait ran out in a kernel (site %d)", *status_host);
   }
   return AB200_OK;

@@ -318,3 +318,212 @@ def row_program(rp, mats, cols, out=None, out_dtype=None):
          ctypes.cast(cst, P), len(consts), ctypes.cast(mp, P), ctypes.cast(md, P), len(mats), ctypes.cast(cp, P), ctypes.cast(cd, P), len(cols),
          _chk(out, "out"), _code(out.dtype), rows, ncols, _stream())
     return out
+
+
+# ---- a paged KV cache held in 8 bits ---------------------------------------------------------------------------
+# A layer's cache is four tensors (k, v, k_scale, v_scale): int8 [pages, kv heads, page rows, 128] twice, fp32 [pages, kv
+# heads, page rows / 16] twice; a value is code * scale.  kv_cache.PagedKV8Cache keeps the pages of many sequences.
+# `page_table` int32 [S, max_pages]: position p of sequence s is row p % page_rows of page table[s, p // page_rows].
+# `pos0` int32 [S]: the position of each sequence's first row of the call.  `cu_rows` int32 [S + 1]: which rows are whose
+# (None: as many for each).  The tensors' device is the one that works, whichever is current.
+
+def _kv8_args(cache, page_table, pos0, cu_rows, T, q=None):
+    """The cache and row arguments of a kv8 entry point; checks what only tensors can say."""
+    k, v, ks, vs = cache
+    if k.dim() != 4 or k.shape[3] != 128 or v.shape != k.shape:
+        raise ValueError("a kv8 cache holds k and v int8 [pages, kv heads, page rows, 128], got %s and %s" % (tuple(k.shape), tuple(v.shape)))
+    pages, heads, rows, _ = k.shape
+    if rows < 16 or rows & (rows - 1):
+        raise ValueError("a kv8 cache's pages hold a power of two of rows, 16 or more; got %d" % rows)
+    if ks.shape != (pages, heads, rows // 16) or vs.shape != ks.shape:
+        raise ValueError("a kv8 cache holds scales fp32 %s, got %s and %s" % ((pages, heads, rows // 16), tuple(ks.shape), tuple(vs.shape)))
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_cuda or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise ValueError("page_table must be a CUDA int32 tensor [sequences, pages] with consecutive columns")
+    S = page_table.shape[0]
+    if pos0.numel() != S or (cu_rows is not None and cu_rows.numel() != S + 1):
+        raise ValueError("%d sequences need %d positions in pos0 and %d offsets in cu_rows" % (S, S, S + 1))
+    for t in (v, ks, vs, page_table, pos0, cu_rows, q):
+        if t is not None and t.device != k.device:
+            raise ValueError("the tensors of a kv8 call lie on one device (%s and %s)" % (k.device, t.device))
+    return (_chk(k, "k cache", torch.int8), _chk(v, "v cache", torch.int8), _chk(ks, "k_scale", torch.float32), _chk(vs, "v_scale", torch.float32),
+            pages, rows, heads, page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), page_table.shape[1], _chk(pos0, "pos0", torch.int32),
+            0 if cu_rows is None else _chk(cu_rows, "cu_rows", torch.int32), S, T)
+
+
+def _rows3(t, name, dtype, T=None, heads=None):
+    """Pointer and row stride of [T, heads, 128] rows; the heads of a row lie together."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError("%s must be a CUDA tensor (antares_b200 has no CPU path)" % name)
+    if t.dim() != 3 or t.shape[2] != 128 or (T is not None and t.shape[0] != T) or (heads is not None and t.shape[1] != heads):
+        raise ValueError("%s must be [%s, %s, 128], got %s" % (name, "rows" if T is None else T, "heads" if heads is None else heads, tuple(t.shape)))
+    if t.dtype != dtype:
+        raise ValueError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128)):
+        raise ValueError("the heads of a row of %s must lie together" % name)
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * 128
+
+
+def _disjoint(out, name, *others):
+    """A result lies over no input (a cache's pages are read by other rows long after a row's result is stored)."""
+    a, b = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for t in others:
+        if t is not None and t.numel() and t.data_ptr() < b and a < t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size():
+            raise ValueError("%s may not lie over an input" % name)
+
+
+def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=None, q_out=None):
+    """Writes rows k, v [T, kv heads, 128] into the cache; with inv_freq, k rotated by halves at its positions, and q [T, query
+    heads, 128] too: returns the rotated queries (q_out, which may be q), else None."""
+    T = k.shape[0]
+    if q_out is not None and q is None:
+        raise ValueError("q_out without q")
+    if q is not None and inv_freq is None:
+        raise ValueError("q is only rotated: it needs inv_freq")
+    args = _kv8_args(cache, page_table, pos0, cu_rows, T, k)
+    kp, k_stride = _rows3(k, "k", k.dtype, heads=args[6])
+    vp, v_stride = _rows3(v, "v", k.dtype, T, args[6])
+    fp = 0
+    if inv_freq is not None:
+        fp = _chk(inv_freq, "inv_freq", torch.float32)
+        if inv_freq.numel() < 64:
+            raise ValueError("inv_freq must hold 64 values")
+    qp = q_stride = qo = qo_stride = hq = 0
+    if q is not None:
+        qp, q_stride = _rows3(q, "q", k.dtype, T)
+        hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if cu_rows is None else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        qo, qo_stride = _rows3(q_out, "q_out", k.dtype, T, hq)
+    for t in (v, q, q_out, inv_freq):
+        if t is not None and t.device != k.device:
+            raise ValueError("the tensors of a kv8 call lie on one device")
+    with torch.cuda.device(k.device):
+        call("ab200_kv8_append", *args, kp, vp, k_stride, v_stride, qp, q_stride, qo, qo_stride, hq, fp, _code(k.dtype), _stream())
+    return q_out
+
+
+def kv8_read(cache, page_table, pos0, rows, cu_rows=None, dtype=torch.float16, out=None):
+    """The values held at the rows' positions, (k, v) [rows, kv heads, 128] each; zeros outside the table.  out: a pair of
+    tensors to write to, whose rows behind the last sequence's stay as they are (new tensors: zeros)."""
+    args = _kv8_args(cache, page_table, pos0, cu_rows, rows)
+    if out is None:
+        make = torch.empty if cu_rows is None and rows else torch.zeros
+        out = tuple(make((rows, args[6], 128), dtype=dtype, device=cache[0].device) for _ in range(2))
+    dtype = out[0].dtype
+    for t in out:
+        _rows3(t, "out", dtype, rows, args[6])
+        if not t.is_contiguous() or t.device != cache[0].device:
+            raise ValueError("out must be contiguous and on the cache's device")
+    with torch.cuda.device(cache[0].device):
+        call("ab200_kv8_read", *args, out[0].data_ptr(), out[1].data_ptr(), _code(dtype), _stream())
+    return out[0], out[1]
+
+
+def kv8_attention_workspace_bytes(S, T, max_rows, Hq, Hkv):
+    return int(_lib.load().ab200_kv8_attention_workspace_bytes(int(S), int(T), int(max_rows), int(Hq), int(Hkv)))
+
+
+def _kv8_workspace(workspace, S, T, max_rows, Hq, Hkv, device):
+    """(pointer, bytes, the tensor that holds them).  Without one of the caller's: memory of this call alone, so that two
+    streams or two captured graphs never share it."""
+    if workspace is None:
+        n = kv8_attention_workspace_bytes(S, T, max_rows, Hq, Hkv)
+        if n == 0:
+            return 0, 0, None
+        workspace = torch.empty(n, dtype=torch.uint8, device=device)
+    elif workspace.device != device:
+        raise ValueError("workspace must lie on %s" % device)
+    return _chk(workspace, "workspace"), workspace.numel() * workspace.element_size(), workspace
+
+
+def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale=None, out=None, workspace=None):
+    """Row r of sequence s, q [T, query heads, 128], over the positions 0 .. pos0[s] + r of the cache, which holds them already
+    (kv8_append); kv head = query head // (query heads / kv heads).  Rows with no position to attend to are zeros, and so are
+    rows behind the last sequence's in a new result (in `out` they stay as they are).  max_rows: the most rows of a sequence,
+    a hint.  out may be q where q is contiguous."""
+    T, hq = q.shape[0], q.shape[1]
+    args = _kv8_args(cache, page_table, pos0, cu_rows, T, q)
+    qp, q_stride = _rows3(q, "q", q.dtype)
+    if hq == 0 or hq % args[6]:
+        raise ValueError("%d query heads are not a multiple of %d kv heads" % (hq, args[6]))
+    S = args[12]
+    if max_rows is None:
+        max_rows = T if cu_rows is not None else (T // S if S else 0)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if cu_rows is None and S else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.device != q.device:
+            raise ValueError("out must be %s on %s" % (tuple(q.shape), q.device))
+        _chk(out, "out", q.dtype)
+        if not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
+            _disjoint(out, "out", q)
+    scale = 128 ** -0.5 if scale is None else scale
+    with torch.cuda.device(q.device):
+        ws, ws_bytes, held = _kv8_workspace(workspace, S, T, max_rows, hq, args[6], q.device)
+        call("ab200_kv8_attention", qp, q_stride, out.data_ptr(), *args, int(max_rows), hq, 128, float(scale), _code(q.dtype), ws, ws_bytes, _stream())
+    return out
+
+
+def kv8_step(q, k, v, cache, page_table, pos0, inv_freq=None, scale=None, out=None, workspace=None):
+    """A decode step's kv8_append and kv8_attention in one call: q [T, query heads, 128], k, v [T, kv heads, 128], T / S rows of
+    each sequence, rotated if inv_freq is given."""
+    T, hq = q.shape[0], q.shape[1]
+    args = _kv8_args(cache, page_table, pos0, None, T, q)
+    qp, q_stride = _rows3(q, "q", q.dtype)
+    kp, k_stride = _rows3(k, "k", q.dtype, T, args[6])
+    vp, v_stride = _rows3(v, "v", q.dtype, T, args[6])
+    if hq == 0 or hq % args[6]:
+        raise ValueError("%d query heads are not a multiple of %d kv heads" % (hq, args[6]))
+    fp = 0
+    if inv_freq is not None:
+        fp = _chk(inv_freq, "inv_freq", torch.float32)
+        if inv_freq.numel() < 64:
+            raise ValueError("inv_freq must hold 64 values")
+    for t in (k, v, inv_freq, out):
+        if t is not None and t.device != q.device:
+            raise ValueError("the tensors of a kv8 call lie on one device")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if args[12] else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape:
+            raise ValueError("out must be %s" % (tuple(q.shape),))
+        _chk(out, "out", q.dtype)
+        _disjoint(out, "out", q, k, v)
+    S = args[12]
+    scale = 128 ** -0.5 if scale is None else scale
+    with torch.cuda.device(q.device):
+        ws, ws_bytes, held = _kv8_workspace(workspace, S, T, T // S if S else 0, hq, args[6], q.device)
+        call("ab200_kv8_step", qp, kp, vp, q_stride, k_stride, v_stride, out.data_ptr(), *args[:11], S, T, hq, 128, fp, float(scale), _code(q.dtype), ws, ws_bytes,
+             _stream())
+    return out
+
+
+def kv_copy_pages(buffers, src, dst):
+    """Copies the pages src[i] to dst[i] (host integers) inside every buffer [layers, pages, ...]: caches of any type, all in
+    one launch.  A page's elements lie together.  No destination may occur twice or be a source too."""
+    import ctypes
+    if len(src) != len(dst):
+        raise ValueError("%d sources and %d destinations" % (len(src), len(dst)))
+    buffers = list(buffers)
+    if not buffers:
+        raise ValueError("kv_copy_pages needs a buffer")
+    pages, device = buffers[0].shape[1] if buffers[0].dim() >= 3 else 0, buffers[0].device
+    base, layers, ls, ps, size = [], [], [], [], []
+    for t in buffers:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError("a buffer must be a CUDA tensor (antares_b200 has no CPU path)")
+        if t.dim() < 3 or t.shape[1] != pages or t.device != device or t.numel() == 0:
+            raise ValueError("buffers must be [layers, pages, ...] with as many pages each, on one device; got %s" % (tuple(t.shape),))
+        if not t[0, 0].is_contiguous():
+            raise ValueError("the elements of a page must lie together")
+        e = t.element_size()
+        base.append(t.data_ptr())
+        layers.append(t.shape[0])
+        size.append(t[0, 0].numel() * e)
+        ls.append(t.stride(0) * e if t.shape[0] > 1 else 0)
+        ps.append(t.stride(1) * e if pages > 1 else size[-1])
+    n, m, P = len(src), len(buffers), ctypes.c_void_p
+    arr = lambda ty, v: ctypes.cast((ty * max(1, len(v)))(*v), P)  # noqa: E731
+    with torch.cuda.device(device):
+        call("ab200_kv_copy_pages", m, arr(P, base), arr(ctypes.c_int, layers), arr(ctypes.c_long, ls), arr(ctypes.c_long, ps), arr(ctypes.c_long, size), pages,
+             arr(ctypes.c_int32, [int(i) for i in src]), arr(ctypes.c_int32, [int(i) for i in dst]), n, _stream())

@@ -43,7 +43,8 @@ int ab200_abi_version(void);
 /* Reads and clears the device-side status word.  Kernels that wait on barriers bound every
  * wait; a wait that ran out leaves a site code here instead of hanging (the reference has a
  * host watchdog that exits the process, graph_evaluator/run_graph.cpp:59-73).  Returns
- * AB200_ETIMEOUT if the word was set.  Synchronises the device; not legal during capture. */
+ * AB200_ETIMEOUT if the word was set, AB200_EINVAL if what it holds is that a page table entry outside
+ * an 8-bit cache was used.  Synchronises the device; not legal during capture. */
 int ab200_kernel_status(int *status_host);
 
 /* Tuning knobs, the counterpart of the `config=` hints of autort.export
@@ -423,6 +424,68 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
                                   const int32_t *prompt, int n_prompt, int32_t *const *token_host,
                                   int32_t *const *pos_host, int32_t *const *out_tokens_host, int out_cap,
                                   void *emu_scratch_dev, void *stream);
+
+/* ---- a paged KV cache held in 8 bits --------------------------------------------------------------
+ * For contexts and batches whose fp16 cache is what a decode step waits for (the reference keeps one sequence's cache
+ * in the activations' type, samples/05_llama2_7b_int4.py:119-120).  One layer's cache:
+ *   k_cache, v_cache  int8 [pages][Hkv][page_rows][128], 16-byte aligned; value = code * scale, codes -127 .. 127
+ *   k_scale, v_scale  fp32 [pages][Hkv][page_rows / 16], one for each block of 16 rows and head
+ * page_rows is a power of two from 16.  page_table int32 [S][table_stride], its first max_pages columns in use: position p
+ * of sequence s is row p % page_rows of page table[s][p / page_rows].  Entries of positions that a call does not touch are
+ * not read.  An entry outside 0 .. pages - 1 that it does touch writes nothing, reads as zeros or as page 0, and shows in
+ * ab200_kernel_status.
+ * The call's rows: T rows of S sequences, sequence s has rows cu_rows_dev[s] .. cu_rows_dev[s + 1] - 1 (int32 [S + 1];
+ * NULL: T / S each) at the positions pos0_dev[s], pos0_dev[s] + 1, ... (int32 [S]).  Rows behind the last sequence's are
+ * left as they were.  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the results; rows may be
+ * strided (in elements, a multiple of 16 bytes), the heads of a row lie together. */
+
+/* Writes the rows of k and v [T][Hkv][128] into the cache.  inv_freq (fp32, 64 values used; NULL: none) rotates k by halves
+ * at the rows' positions first, and q [T][Hq][128] into q_out (both NULL: no queries; q_out may be q).  For each block that
+ * new rows lie in and each head: scale = max(scale of the block if it holds rows before pos0, else 0; largest |value| of
+ * the new rows / 127), codes = value / scale rounded to the nearest, ties to even; rows before the new ones are rounded again
+ * if their scale grew; codes behind the new rows stay as they are.  8 bits hold no infinities or NaN: +-inf becomes the
+ * code +-127, NaN 0, and neither counts for the scale.  A scale below 2^-100 is held as 0.  Rows at negative positions or
+ * behind the table's max_pages are not stored.  fp32 rows are rotated in 64 bits, so that the codes are the definition's. */
+int ab200_kv8_append(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int pages, int page_rows, int Hkv,
+                     const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev,
+                     const int32_t *cu_rows_dev, int S, int T, const void *k, const void *v, long k_stride, long v_stride,
+                     const void *q, long q_stride, void *q_out, long q_out_stride, int Hq, const float *inv_freq, int dtype,
+                     void *stream);
+
+/* k_out, v_out [T][Hkv][128] = the values held at the rows' positions (zeros outside the table). */
+int ab200_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages,
+                   int page_rows, int Hkv, const int32_t *page_table, long table_stride, int max_pages,
+                   const int32_t *pos0_dev, const int32_t *cu_rows_dev, int S, int T, void *k_out, void *v_out, int dtype,
+                   void *stream);
+
+/* out [T][Hq][128]: row r of sequence s over the positions 0 .. pos0_dev[s] + r (those of the table), query head h over kv
+ * head h / (Hq / Hkv); zeros where there is none.  The cache holds the call's own rows already (ab200_kv8_append).
+ * max_rows: the most rows a sequence has (a hint for the choice of kernels, any value gives the same rows).  out may be q
+ * where q is contiguous.  workspace: device scratch of ab200_kv8_attention_workspace_bytes(...), 16-byte aligned, nothing
+ * kept in it between calls; two calls that may overlap on the GPU need one each. */
+int ab200_kv8_attention(const void *q, long q_stride, void *out, const void *k_cache, const void *v_cache,
+                        const float *k_scale, const float *v_scale, int pages, int page_rows, int Hkv,
+                        const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev,
+                        const int32_t *cu_rows_dev, int S, int T, int max_rows, int Hq, int D, float scale, int dtype,
+                        void *workspace, size_t workspace_bytes, void *stream);
+size_t ab200_kv8_attention_workspace_bytes(int S, int T, int max_rows, int Hq, int Hkv);
+
+/* A decode step's ab200_kv8_append and ab200_kv8_attention in one call: T / S rows of each sequence.  q, k and v may be
+ * slices of one projection's result; out is none of them.  Rotates q and k if inv_freq is given.  workspace as above, of
+ * ab200_kv8_attention_workspace_bytes(S, T, T / S, Hq, Hkv) bytes. */
+int ab200_kv8_step(const void *q, const void *k, const void *v, long q_stride, long k_stride, long v_stride, void *out,
+                   void *k_cache, void *v_cache, float *k_scale, float *v_scale, int pages, int page_rows, int Hkv,
+                   const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev, int S, int T, int Hq,
+                   int D, const float *inv_freq, float scale, int dtype, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
+/* Copies pages src_host[i] -> dst_host[i], i < n, inside each of `buffers` (1 to 8) buffers: buffer b has layers_host[b]
+ * layers layer_stride_host[b] bytes apart, each with `pages` pages of page_bytes_host[b] bytes, page_stride_host[b] bytes
+ * apart.  For caches of any type.  No destination may occur twice or be a source too (AB200_EINVAL): the copies have no
+ * order.  The lists are host arrays and part of the launch: free to change after the call, kept by a captured one. */
+int ab200_kv_copy_pages(int buffers, void *const *base_host, const int *layers_host, const long *layer_stride_host,
+                        const long *page_stride_host, const long *page_bytes_host, int pages, const int32_t *src_host,
+                        const int32_t *dst_host, int n, void *stream);
 
 /* ---- the reference's native plugin boundary ---------------------------------------------------
  * frameworks/pytorch/main_ops.cc:17-54 binds two calls over kernel-source text:

@@ -1,0 +1,427 @@
+"""The 8-bit paged cache's operators against their definitions in 64 bits (kv8_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_ref
+from antares_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+F16, F32 = torch.float16, torch.float32
+INV_FREQ = (10000.0 ** -(np.arange(0, 128, 2) / 128)).astype(np.float32)
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _setup(seed, past, rows, heads, page, spare=3, filled=True):
+    """A cache whose pages lie in any order, what lies outside the sequences poisoned: huge scales, codes, table entries."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-max(p + n, 1) // page) for p, n in zip(past, rows)]
+    pages = sum(need) + spare
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((len(past), max(need) + 2), 0x7FFFFFF0, dtype=torch.int32)
+    for s, n in enumerate(need):
+        table[s, :n] = torch.tensor(order[:n])
+        order = order[n:]
+    spread = 20 + 30 * torch.rand(pages, heads, 1, 1, generator=g)
+    cache = []
+    for _ in range(2):
+        cache.append((torch.randn(pages, heads, page, 128, generator=g) * spread).round().clamp(-127, 127).to(torch.int8))
+    for _ in range(2):
+        cache.append(0.01 + 0.04 * torch.rand(pages, heads, page // 16, generator=g))
+    for s, (p, n) in enumerate(zip(past, rows)):  # blocks that no position lies in yet
+        for b in range(need[s] * page // 16):
+            if 16 * b >= (p + n if filled else max(p, 0)):
+                pg, i = int(table[s, 16 * b // page]), 16 * b % page // 16
+                cache[2][pg, :, i] = float("nan")
+                cache[3][pg, :, i] = float("inf")
+    return [t.cuda() for t in cache], table.cuda()
+
+
+def _ref(cache, table):
+    return kv8_ref.Cache(cache, table)
+
+
+def _randn(seed, *shape, dtype=F16, mul=1.0):
+    return (mul * torch.randn(*shape, generator=torch.Generator().manual_seed(seed))).to(dtype).cuda()
+
+
+def _cu(rows):
+    return _ints(np.cumsum([0] + list(rows)).tolist())
+
+
+def _check_attention(got, ref_cache, q, pos0, cu, keys, dtype, scale=None, inv_freq=None):
+    want, spread, score = kv8_ref.attention(ref_cache, q.double().cpu().numpy(), pos0, cu, scale, inv_freq)
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    off = np.abs(got - want) / kv8_ref.bound(want, spread, score, keys, dtype)
+    assert off.max() <= 1, "off by %.2f of the bound at %s" % (off.max(), np.unravel_index(off.argmax(), off.shape))
+
+
+# past, rows: lengths of one, block and page borders, empty rows and sequences
+CASES = [
+    ([0], [1], 4, 4, 16), ([15], [1], 4, 4, 16), ([16], [1], 4, 2, 16), ([31, 0, 500, 63], [1] * 4, 8, 1, 64), ([383], [1], 32, 32, 16), ([1000, 7, 77], [1] * 3, 14, 2, 32),
+    ([5, 200, 31], [4] * 3, 16, 4, 32), ([100, 3], [2] * 2, 5, 1, 128), ([2500], [1], 16, 1, 256), ([300] * 40, [1] * 40, 8, 8, 32), ([129, 300], [8, 8], 32, 2, 64),
+    ([0], [17], 4, 4, 16), ([0], [130], 4, 2, 16), ([77], [64], 8, 2, 32), ([0, 40, 333, 0], [3, 200, 1, 129], 6, 2, 64), ([10, 20, 30], [0, 70, 0], 4, 4, 32),
+    ([1200, 5, 64], [90, 1, 300], 8, 1, 128), ([0, 0], [256, 256], 2, 2, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("past,rows,hq,hkv,page", CASES)
+def test_attention(cuda, past, rows, hq, hkv, page, dtype):
+    cache, table = _setup(len(past) + sum(rows), past, rows, hkv, page)
+    T, uniform = sum(rows), len(set(rows)) == 1
+    q = _randn(1, T, hq, 128, dtype=dtype, mul=2)
+    cu = None if uniform else np.cumsum([0] + rows)
+    got = ops.kv8_attention(q, cache, table, _ints(past), cu_rows=None if uniform else _cu(rows), max_rows=max(rows))
+    ref = _ref(cache, table)
+    _check_attention(got, ref, q, past, cu, max(p + n for p, n in zip(past, rows)), dtype)
+    # the same rows whatever the hint says and however the rows are named
+    for hint in (1, 7, T):
+        again = ops.kv8_attention(q, cache, table, _ints(past), cu_rows=_cu(rows), max_rows=hint)
+        _check_attention(again, ref, q, past, cu, max(p + n for p, n in zip(past, rows)), dtype)
+    assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("mul", [0.0, 24.0])
+@pytest.mark.parametrize("past,rows,hq,hkv", [([333, 64], [1, 1], 8, 2), ([50], [140], 4, 1)])
+def test_flat_and_sharp_scores(cuda, past, rows, hq, hkv, mul, dtype):
+    """All scores alike, and scores spread over hundreds: the running maximum moves often."""
+    cache, table = _setup(3, past, rows, hkv, 32)
+    q = _randn(2, sum(rows), hq, 128, dtype=dtype, mul=mul)
+    got = ops.kv8_attention(q, cache, table, _ints(past), max_rows=max(rows))
+    _check_attention(got, _ref(cache, table), q, past, None, max(p + n for p, n in zip(past, rows)), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rows", [1, 40, 150])
+def test_block_scales_far_apart(cuda, rows, dtype):
+    """Scales from 2^-40 to 2^12, and blocks of zeros, side by side."""
+    past, hq, hkv = 200, 8, 2
+    cache, table = _setup(5, [past], [rows], hkv, 64)
+    g = torch.Generator().manual_seed(8)
+    for t in cache[2:]:
+        e = torch.randint(-40, 13, t.shape, generator=g).float()
+        t.copy_(torch.where(torch.rand(t.shape, generator=g) < 0.2, 0.0, 2.0 ** e).cuda())
+    cache[2].clamp_(max=2.0 ** -4)
+    q = _randn(2, rows, hq, 128, dtype=dtype, mul=0.1)
+    if dtype == F16:
+        cache[3].clamp_(max=2.0 ** 5)
+    got = ops.kv8_attention(q, cache, table, _ints([past]))
+    _check_attention(got, _ref(cache, table), q, [past], None, past + rows, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rows", [1, 5, 150])
+def test_rows_with_nothing_to_attend_to(cuda, rows, dtype):
+    """Negative positions attend to nothing (zeros), positions behind the table to all of it."""
+    cache, table = _setup(6, [400 - rows, 400 - rows], [rows] * 2, 2, 64)
+    table = table[:, :6].contiguous()  # capacity 384
+    q = _randn(3, 2 * rows, 4, 128, dtype=dtype)
+    for pos0 in ([-3, 384 - rows // 2], [-rows, -1000], [0, 383], [2 ** 31 - 1, -2 ** 31]):
+        if max(pos0) > 10000 and rows > 1:
+            continue
+        got = ops.kv8_attention(q, cache, table, _ints(pos0), max_rows=rows)
+        _check_attention(got, _ref(cache, table), q, pos0, None, 400, dtype)
+        if max(pos0) < 0 and pos0[0] <= -rows:
+            assert not got.any()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_queries_that_are_not_finite_stay_in_their_row(cuda, value, dtype):
+    for past, rows in (([90], [3]), ([20], [150])):
+        cache, table = _setup(7, past, rows, 2, 32)
+        q = _randn(4, rows[0], 6, 128, dtype=dtype)
+        want = ops.kv8_attention(q, cache, table, _ints(past))
+        q[1, 4, 7] = value
+        got = ops.kv8_attention(q, cache, table, _ints(past))
+        assert not got[1, 4].isfinite().any()
+        keep = torch.ones(rows[0], 6, dtype=torch.bool, device="cuda")
+        keep[1, 4] = False
+        assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("past,rows,hkv,page", [([0], [1], 4, 16), ([5], [1], 1, 16), ([0], [33], 2, 32), ([30, 0, 47, 16], [1] * 4, 5, 64), ([7, 100, 0, 31], [40, 1, 0, 17], 3, 32),
+                                               ([250], [300], 2, 128)])
+def test_append(cuda, past, rows, hkv, page, rope, dtype):
+    """Scales and codes as the definition has them; everything else keeps its bytes."""
+    cache, table = _setup(sum(rows) + hkv, past, rows, hkv, page, filled=False)
+    T, hq = sum(rows), 2 * hkv
+    k, v, q = _randn(1, T, hkv, 128, dtype=dtype), _randn(2, T, hkv, 128, dtype=dtype, mul=3), _randn(3, T, hq, 128, dtype=dtype)
+    ref = _ref(cache, table)
+    uniform = len(set(rows)) == 1
+    cu = None if uniform else np.cumsum([0] + rows)
+    freq = torch.from_numpy(INV_FREQ).cuda() if rope else None
+    kv8_ref.append(ref, k.float().cpu().numpy(), v.float().cpu().numpy(), past, cu, INV_FREQ if rope else None)
+    got_q = ops.kv8_append(cache, k, v, table, _ints(past), cu_rows=None if uniform else _cu(rows), q=q if rope else None, inv_freq=freq)
+    assert ops.kernel_status() == 0
+    kc, vc, ks, vs = (t.cpu().numpy() for t in cache)
+    assert np.array_equal(vs, ref.vs) and np.array_equal(vc, ref.v)
+    if not rope or dtype == F32:
+        assert np.array_equal(ks, ref.ks, equal_nan=True) and np.array_equal(kc, ref.k)
+    else:
+        # sines, cosines and the rotation in 32 bits: 2^-21 of the largest value, so a scale may differ by that and a code by one
+        # where the quotient, at most 127, lies within 127 * 2^-20 of the middle of two
+        assert np.allclose(ks, ref.ks, rtol=2.0 ** -20, atol=0, equal_nan=True)
+        off = np.abs(kc.astype(int) - ref.k.astype(int))
+        assert off.max() <= 1 and off.sum() <= max(2, 2e-3 * T * hkv * 128)
+    if rope:
+        pos = np.concatenate([np.arange(p, p + n) for p, n in zip(past, rows)])
+        want = kv8_ref.rotate(q.double().cpu().numpy(), pos, INV_FREQ)
+        tol = np.abs(want) * torch.finfo(dtype).eps / 2 * 1.01 + (2.0 ** -20 if dtype == F16 else 2.0 ** -30)
+        assert (np.abs(got_q.double().cpu().numpy() - want) <= tol).all()
+    else:
+        assert got_q is None
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_append_token_by_token_and_growth(cuda, dtype):
+    """Rows that arrive one at a time, each larger than the last: the block is rounded again at every growth."""
+    cache, table = _setup(1, [0], [40], 2, 16, filled=False)
+    ref = _ref(cache, table)
+    for p in range(40):
+        k, v = _randn(10 + p, 1, 2, 128, dtype=dtype, mul=1 + 0.3 * p), _randn(100 + p, 1, 2, 128, dtype=dtype)
+        ops.kv8_append(cache, k, v, table, _ints([p]))
+        kv8_ref.append(ref, k.float().cpu().numpy(), v.float().cpu().numpy(), [p])
+    kc, vc, ks, vs = (t.cpu().numpy() for t in cache)
+    assert np.array_equal(kc, ref.k) and np.array_equal(vc, ref.v) and np.array_equal(ks, ref.ks, equal_nan=True) and np.array_equal(vs, ref.vs)
+
+
+def test_append_values_between_codes_and_extremes(cuda):
+    """Middles between two codes go to the even one; infinities, NaN, zeros, subnormals and the largest values."""
+    cache, table = _setup(2, [0], [16], 1, 16, filled=False)
+    x = torch.zeros(16, 1, 128)
+    x[0, 0] = torch.arange(-64, 64) + 0.5
+    x[0, 0, 0] = 127.0                      # scale 1: the others lie in the middle of two codes
+    x[1, 0, :4] = torch.tensor([float("inf"), float("-inf"), float("nan"), 1e-30])
+    ref = _ref(cache, table)
+    ops.kv8_append(cache, x.cuda(), x.cuda(), table, _ints([0]))
+    kv8_ref.append(ref, x.numpy(), x.numpy(), [0])
+    assert np.array_equal(cache[0].cpu().numpy(), ref.k) and ref.ks[int(table[0, 0])] == 1
+    assert cache[0][int(table[0, 0]), 0, 1, :4].tolist() == [127, -127, 0, 0]
+    for mul in (1e-42, 1e-33, 2.5e38, 0.0):
+        y = (mul * torch.randn(16, 1, 128, generator=torch.Generator().manual_seed(1)).clamp(-1.3, 1.3)).float()
+        ops.kv8_append(cache, y.cuda(), y.cuda(), table, _ints([0]))
+        kv8_ref.append(ref, y.numpy(), y.numpy(), [0])
+        assert np.array_equal(cache[0].cpu().numpy(), ref.k) and np.array_equal(cache[2].cpu().numpy(), ref.ks, equal_nan=True)
+
+
+def test_append_outside_the_table(cuda):
+    """Rows at negative positions and behind the table are not stored."""
+    cache, table = _setup(4, [60, 60], [8, 8], 2, 32, filled=False)
+    table = table[:, :2].contiguous()
+    before = [t.clone() for t in cache]
+    x = _randn(1, 16, 2, 128)
+    ops.kv8_append(cache, x, x, table, _ints([-8, 64]))
+    ops.kv8_append(cache, x, x, table, _ints([-2 ** 31, 2 ** 31 - 1]))
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, before))
+    ref = _ref(cache, table)
+    ops.kv8_append(cache, x, x, table, _ints([-3, 61]))
+    kv8_ref.append(ref, x.float().cpu().numpy(), x.float().cpu().numpy(), [-3, 61])
+    assert np.array_equal(cache[0].cpu().numpy(), ref.k) and np.array_equal(cache[3].cpu().numpy(), ref.vs, equal_nan=True)
+    assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_read(cuda, dtype):
+    past, rows = [0, 20, 9, 33], [50, 0, 1, 31]
+    cache, table = _setup(9, past, rows, 3, 32)
+    ref = _ref(cache, table)
+    k, v = ops.kv8_read(cache, table, _ints(past), sum(rows), cu_rows=_cu(rows), dtype=dtype)
+    at = 0
+    for s, (p, n) in enumerate(zip(past, rows)):
+        rk, rv = ref.values(s, p + n)
+        for got, want in ((k, rk), (v, rv)):
+            want = torch.from_numpy(want[p:]).float().to(dtype)
+            assert torch.equal(got[at:at + n].cpu(), want)
+        at += n
+    # outside the table: zeros; rows behind the last sequence's: as they were
+    out = tuple(torch.full((6, 3, 128), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+    small = table[:2, :1].contiguous()
+    ops.kv8_read(cache, small, _ints([-1, 31]), 6, cu_rows=_ints([0, 2, 4]), out=out)
+    assert not out[0][0].any() and not out[1][3].any() and out[0][1].any() and out[1][2].any() and (out[0][4:] == 7).all() and (out[1][4:] == 7).all()
+
+
+@pytest.mark.parametrize("rows", [1, 30, 200])
+def test_rows_behind_the_last_sequence(cuda, rows):
+    """A padded batch: rows that are nobody's keep what `out` held, and are zeros in a new result."""
+    cache, table = _setup(11, [40, 3], [rows, 2], 2, 32)
+    T = rows + 2 + 9
+    q = _randn(1, T, 4, 128)
+    cu = _ints([0, rows, rows + 2])
+    out = torch.full_like(q, 5.0)
+    ops.kv8_attention(q, cache, table, _ints([40, 3]), cu_rows=cu, out=out)
+    assert (out[rows + 2:] == 5).all()
+    new = ops.kv8_attention(q, cache, table, _ints([40, 3]), cu_rows=cu)
+    assert torch.equal(new[:rows + 2], out[:rows + 2]) and not new[rows + 2:].any()
+    _check_attention(new[:rows + 2], _ref(cache, table), q[:rows + 2], [40, 3], np.array([0, rows, rows + 2]), 300, F16)
+    qo = torch.full_like(q, 5.0)
+    k = _randn(2, T, 2, 128)
+    ops.kv8_append(cache, k, k, table, _ints([40, 3]), cu_rows=cu, q=q, inv_freq=torch.from_numpy(INV_FREQ).cuda(), q_out=qo)
+    assert (qo[rows + 2:] == 5).all() and (qo[:rows + 2] != 5).any()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("past,n,hq,hkv,page", [([383], 1, 32, 32, 16), ([0, 15, 16, 600, 31], 1, 8, 2, 32), ([20, 0], 3, 6, 1, 64), ([0], 20, 4, 4, 16), ([-1, 50], 1, 16, 2, 32),
+                                               ([300, 17], 1, 40, 2, 128)])
+def test_step(cuda, past, n, hq, hkv, page, rope, dtype):
+    """One call = append, then attention, with q, k and v slices of one projection's result."""
+    S = len(past)
+    cache, table = _setup(13, past, [n] * S, hkv, page, filled=False)
+    both = _randn(5, S * n, hq + 2 * hkv, 128, dtype=dtype)
+    q, k, v = both[:, :hq], both[:, hq:hq + hkv], both[:, hq + hkv:]
+    freq = torch.from_numpy(INV_FREQ).cuda() if rope else None
+    apart = [t.clone() for t in cache]
+    out = ops.kv8_step(q, k, v, cache, table, _ints(past), inv_freq=freq)
+    ops.kv8_append(apart, k, v, table, _ints(past), inv_freq=freq)
+    for a, b in zip(cache, apart):
+        assert torch.equal(a.view(torch.int8), b.view(torch.int8))
+    # against the cache as it now is; a rotated query may be kept in its type: half a step of it moves every score
+    ref = _ref(cache, table)
+    want, spread, score = kv8_ref.attention(ref, q.double().cpu().numpy(), past, None, None, INV_FREQ if rope else None)
+    if rope:
+        _, _, mag = kv8_ref.attention(ref, q.double().cpu().numpy(), past, None)
+        score = score + 1.5 * mag * 2.0 ** 19 * (torch.finfo(dtype).eps / 2 + 2.0 ** -21)
+    off = np.abs(out.double().cpu().numpy() - want) / kv8_ref.bound(want, spread, score, max(past) + n, dtype)
+    assert off.max() <= 1, off.max()
+    assert ops.kernel_status() == 0
+
+
+def test_a_bad_page_is_reported(cuda):
+    """Entries that name no page: nothing is written there, the status says so, and the next call is well."""
+    for rows in (1, 150):
+        cache, table = _setup(15, [70], [rows], 2, 32, filled=False)
+        table[0, 2] = cache[0].shape[0]
+        before = [t.clone() for t in cache]
+        x, q = _randn(1, rows, 2, 128), _randn(2, rows, 4, 128)
+        ops.kv8_append(cache, x, x, table, _ints([70]))
+        with pytest.raises(_lib.Ab200Error, match="page table"):
+            ops.kernel_status()
+        if rows == 1:
+            assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, before))
+        ops.kv8_attention(q, cache, table, _ints([70]))
+        with pytest.raises(_lib.Ab200Error, match="page table"):
+            ops.kernel_status()
+        k, _ = ops.kv8_read(cache, table, _ints([64]), 1)
+        assert not k.any()
+        with pytest.raises(_lib.Ab200Error, match="page table"):
+            ops.kernel_status()
+        assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("make", [
+    lambda: torch.arange(2 * 7 * 3 * 16, device="cuda").half().view(2, 7, 3, 16), lambda: torch.arange(7 * 5, device="cuda", dtype=torch.int32).view(1, 7, 5).float(),
+    lambda: torch.randint(-128, 128, (3, 7, 11), device="cuda", dtype=torch.int8), lambda: torch.randn(4, 7, 40000, device="cuda").half(),
+    lambda: torch.randn(7, 4, 64, device="cuda").transpose(0, 1), lambda: torch.randn(2, 9, 10, 64, device="cuda")[:, 1:8]])
+def test_copy_pages(cuda, make):
+    a, b = make(), make()
+    want = [a.clone(), b.clone()]
+    src, dst = [5, 0, 5, 2], [1, 3, 4, 6]
+    for t in want:
+        t[:, dst] = t[:, src].clone()
+    ops.kv_copy_pages([a, b], src, dst)
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
+def test_copy_many_pages_of_several_types(cuda):
+    """More pairs than one launch carries, a whole 8-bit cache at once."""
+    g = torch.Generator().manual_seed(0)
+    P, n = 2000, 900
+    cache = [torch.randint(-127, 128, (2, P, 2, 16, 128), generator=g).to(torch.int8).cuda() for _ in range(2)] + [torch.rand(2, P, 2, 1, generator=g).cuda() for _ in range(2)]
+    order = torch.randperm(P, generator=g).tolist()
+    src, dst = order[:n], order[n:2 * n]
+    want = [t.clone() for t in cache]
+    for t in want:
+        t[:, dst] = t[:, src].clone()
+    ops.kv_copy_pages(cache, src, dst)
+    assert all(torch.equal(a, b) for a, b in zip(cache, want))
+
+
+def test_refusals_of_tensors(cuda):
+    cache, table = _setup(1, [10], [1], 2, 32)
+    x, q, pos0 = _randn(1, 1, 2, 128), _randn(2, 1, 4, 128), _ints([10])
+    bad = [lambda: ops.kv8_attention(q[..., :64], cache, table, pos0), lambda: ops.kv8_attention(q.bfloat16(), cache, table, pos0), lambda: ops.kv8_attention(q[:, :3], cache, table, pos0),
+           lambda: ops.kv8_attention(q, cache, table.long(), pos0), lambda: ops.kv8_attention(q, cache, table, pos0.long()), lambda: ops.kv8_attention(q, cache, table, _ints([1, 2])),
+           lambda: ops.kv8_attention(q, cache, table, pos0, cu_rows=_ints([0])), lambda: ops.kv8_attention(q, [cache[0], cache[1], cache[2][..., :0], cache[3]], table, pos0),
+           lambda: ops.kv8_attention(q, [cache[0][:, :, :24], cache[1][:, :, :24], cache[2], cache[3]], table, pos0), lambda: ops.kv8_attention(q, cache, table, pos0, out=x),
+           lambda: ops.kv8_append(cache, x, x.float(), table, pos0), lambda: ops.kv8_append(cache, x, x[:, :1], table, pos0), lambda: ops.kv8_append(cache, x, x, table, pos0, q=q),
+           lambda: ops.kv8_append(cache, x, x, table, pos0, inv_freq=torch.ones(10, device="cuda")), lambda: ops.kv8_append(cache, x, x, table, pos0, q_out=q),
+           lambda: ops.kv8_step(q, x, x, cache, table, pos0, out=q), lambda: ops.kv8_step(q, x, x, cache, table.t(), pos0), lambda: ops.kv8_read(cache, table, pos0, 1, dtype=torch.int8),
+           lambda: ops.kv_copy_pages([cache[0][None]], [0], [0, 1]), lambda: ops.kv_copy_pages([], [], []), lambda: ops.kv_copy_pages([x[0]], [0], [1]),
+           lambda: ops.kv8_attention(q.expand(4, 4, 128).transpose(0, 1), cache, table, pos0)]
+    for i, f in enumerate(bad):
+        with pytest.raises((ValueError, _lib.Ab200Error)):
+            f()
+            pytest.fail("call %d was taken" % i)
+    assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (32, 32)])
+def test_captured_with_other_streams_alive(cuda, hq, hkv):
+    """Two captured decode steps replayed on two streams at once, and an eager call between: each has its own scratch."""
+    states = []
+    for i in range(2):
+        cache, table = _setup(20 + i, [700, 33], [1, 1], hkv, 32, filled=False)
+        q, k = _randn(i, 2, hq, 128), _randn(9 + i, 2, hkv, 128)
+        pos0 = _ints([700, 33])
+        want = ops.kv8_step(q, k, k, [t.clone() for t in cache], table, pos0)
+        states.append((cache, table, q, k, pos0, want))
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for cache, table, q, k, pos0, _ in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.kv8_step(q, k, k, cache, table, pos0))
+        graphs.append(g)
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = ops.kv8_attention(states[0][2], states[1][0], states[1][1], _ints([600, 20]))
+    torch.cuda.synchronize()
+    for out, st in zip(outs, states):
+        assert torch.equal(out, st[5])
+    assert torch.equal(eager, ops.kv8_attention(states[0][2], states[1][0], states[1][1], _ints([600, 20])))
+
+
+def test_same_bits_every_time(cuda):
+    for past, rows, hq, hkv in (([3000, 1, 900], [1] * 3, 32, 8), ([500], [200], 8, 2)):
+        cache, table = _setup(30, past, rows, hkv, 64)
+        q = _randn(1, sum(rows), hq, 128)
+        first = ops.kv8_attention(q, cache, table, _ints(past))
+        assert all(torch.equal(first, ops.kv8_attention(q, cache, table, _ints(past))) for _ in range(5))
+
+
+def test_a_long_cache(cuda):
+    """Positions beyond 2^17, cache offsets beyond 2^31 bytes (pages far up in a large cache)."""
+    P, page, hkv, hq = 9000, 256, 8, 16   # 2.4 GB each of K and V
+    past = 140001
+    need = -(-(past + 1) // page)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k = torch.randint(-127, 128, (P, hkv, page, 128), generator=g, device="cuda", dtype=torch.int8)
+    v = torch.randint(-127, 128, (P, hkv, page, 128), generator=g, device="cuda", dtype=torch.int8)
+    ks, vs = (0.001 + 0.02 * torch.rand(P, hkv, page // 16, generator=g, device="cuda") for _ in range(2))
+    table = torch.arange(P - 1, P - 1 - need, -1, dtype=torch.int32, device="cuda")[None].contiguous()
+    q, x = _randn(1, 1, hq, 128), _randn(2, 1, hkv, 128)
+    ops.kv8_append((k, v, ks, vs), x, x, table, _ints([past]))
+    got = ops.kv8_attention(q, (k, v, ks, vs), table, _ints([past])).double()
+    pos = torch.arange(past + 1, device="cuda")
+    pg, at = table[0].long()[pos // page], pos % page
+    kk, vv = ((c[pg, :, at].double() * s[pg, :, at // 16].double()[..., None]) for c, s in ((k, ks), (v, vs)))
+    sc = torch.einsum("hgd,lhd->hgl", q[0].double().view(hkv, hq // hkv, 128), kk) * 128 ** -0.5
+    p = torch.softmax(sc, -1)
+    want, spread = torch.einsum("hgl,lhd->hgd", p, vv).view(1, hq, 128), torch.einsum("hgl,lhd->hgd", p, vv.abs()).view(1, hq, 128)
+    mag = torch.einsum("hgd,lhd->hgl", q[0].double().abs().view(hkv, hq // hkv, 128), kk.abs()).amax(-1).view(1, hq, 1) * 128 ** -0.5
+    b = kv8_ref.bound(want.cpu().numpy(), spread.cpu().numpy(), (mag * 2.0 ** -18).cpu().numpy(), past, F16)
+    assert (np.abs((got - want).cpu().numpy()) <= b).all()
+    back, _ = ops.kv8_read((k, v, ks, vs), table, _ints([past]), 1)
+    assert torch.equal(back, (kk[-1:].float()).half())
+    assert (back.float() - x.float()).abs().max() <= 0.5 * max(float(ks.max()), float(x.float().abs().max()) / 127) + 0.002

@@ -1,0 +1,103 @@
+"""The 8-bit paged cache on the CPU: what its calls refuse before any kernel runs."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_ref
+from antares_b200 import _lib, ops
+
+
+def _entry(name, *args):
+    L = _lib.load()
+    return getattr(L, name)(*args), L.ab200_last_error().decode()
+
+
+CACHE = dict(k=4096, v=4096, ks=4096, vs=4096, pages=8, page_rows=32, H=2)
+ROWS = dict(table=4096, stride=4, max_pages=4, pos0=4096, cu=None, S=2, T=2)
+
+
+def _attention(q=4096, q_stride=512, out=4096, max_rows=1, Hq=4, D=128, dtype=0, **kw):
+    a = {**CACHE, **ROWS, **kw}
+    return _entry("ab200_kv8_attention", q, q_stride, out, a["k"], a["v"], a["ks"], a["vs"], a["pages"], a["page_rows"], a["H"], a["table"], a["stride"], a["max_pages"],
+                  a["pos0"], a["cu"], a["S"], a["T"], max_rows, Hq, D, 0.1, dtype, None, 0, None)
+
+
+def _append(k=4096, v=4096, k_stride=256, v_stride=256, q=None, q_stride=0, q_out=None, qo_stride=0, Hq=0, freq=None, dtype=0, **kw):
+    a = {**CACHE, **ROWS, **kw}
+    return _entry("ab200_kv8_append", CACHE["k"], CACHE["v"], a["ks"], a["vs"], a["pages"], a["page_rows"], a["H"], a["table"], a["stride"], a["max_pages"], a["pos0"], a["cu"],
+                  a["S"], a["T"], k, v, k_stride, v_stride, q, q_stride, q_out, qo_stride, Hq, freq, dtype, None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(page_rows=24), _lib.EINVAL, "page_rows=24"), (dict(page_rows=8), _lib.EINVAL, "page_rows=8"), (dict(page_rows=0), _lib.EINVAL, "page_rows"),
+    (dict(pages=0), _lib.EINVAL, "pages=0"), (dict(H=0), _lib.EINVAL, "heads=0"), (dict(stride=3), _lib.EINVAL, "table_stride=3"), (dict(max_pages=0), _lib.EINVAL, "max_pages=0"),
+    (dict(max_pages=1 << 27, stride=1 << 27), _lib.EINVAL, "2^30"), (dict(S=-1), _lib.EINVAL, "S=-1"), (dict(T=3), _lib.EINVAL, "do not divide"), (dict(table=None), _lib.EINVAL, "null"),
+    (dict(pos0=None), _lib.EINVAL, "null"), (dict(ks=None), _lib.EINVAL, "null"), (dict(k=4104), _lib.EINVAL, "aligned"), (dict(Hq=3), _lib.EINVAL, "multiple of 2"),
+    (dict(Hq=0), _lib.EINVAL, "query heads"), (dict(D=64), _lib.EUNSUPPORTED, "head size 64"), (dict(dtype=2), _lib.EINVAL, "dtype 2"), (dict(q=4104), _lib.EINVAL, "aligned"),
+    (dict(q_stride=500), _lib.EINVAL, "at least 512"), (dict(q_stride=516), _lib.EINVAL, "16 bytes"), (dict(out=None), _lib.EINVAL, "out"), (dict(T=1 << 29, S=1), _lib.EINVAL, "limits")])
+def test_attention_refuses(change, code, word):
+    rc, text = _attention(**change)
+    assert rc == code and word in text and "kv8_attention" in text
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(k_stride=128), "at least 256"), (dict(v_stride=260), "16 bytes"), (dict(k=None), "16-byte"), (dict(q=4096), "come together"), (dict(q=4096, q_out=4096), "only rotated"),
+    (dict(q=4096, q_out=4096, freq=4096, Hq=4, q_stride=512, qo_stride=500), "at least 512"), (dict(dtype=7), "dtype 7"), (dict(page_rows=48), "page_rows=48")])
+def test_append_refuses(change, word):
+    rc, text = _append(**change)
+    assert rc == _lib.EINVAL and word in text
+
+
+def test_nothing_to_do_is_no_error():
+    assert _attention(S=0, T=0, q=None, out=None)[0] == 0 and _attention(T=0, q=None, out=None)[0] == 0
+    assert _append(S=0, T=0, k=None, v=None)[0] == 0
+
+
+def _copy(src, dst, pages=8, base=4096, layers=1, ls=0, ps=64, size=64, buffers=1):
+    arr = lambda ty, v: ctypes.cast((ty * max(1, len(v)))(*v), ctypes.c_void_p)  # noqa: E731
+    return _entry("ab200_kv_copy_pages", buffers, arr(ctypes.c_void_p, [base]), arr(ctypes.c_int, [layers]), arr(ctypes.c_long, [ls]), arr(ctypes.c_long, [ps]),
+                  arr(ctypes.c_long, [size]), pages, arr(ctypes.c_int32, src), arr(ctypes.c_int32, dst), len(src), None)
+
+
+@pytest.mark.parametrize("src,dst,word", [([0], [8], "outside"), ([-1], [2], "outside"), ([0, 1], [3, 3], "twice"), ([0, 3], [3, 4], "source and a destination"), ([2], [2], "source and")])
+def test_page_lists_that_are_refused(src, dst, word):
+    rc, text = _copy(src, dst)
+    assert rc == _lib.EINVAL and word in text
+
+
+@pytest.mark.parametrize("kw", [dict(base=0), dict(layers=0), dict(size=0), dict(ps=32), dict(ls=-64), dict(buffers=0), dict(buffers=9), dict(pages=0)])
+def test_page_buffers_that_are_refused(kw):
+    assert _copy([0], [1], **kw)[0] == _lib.EINVAL
+
+
+def test_no_pairs_is_no_copy():
+    assert _copy([], [])[0] == 0
+
+
+def test_tensors_on_the_cpu_are_refused():
+    cache = (torch.zeros(2, 1, 16, 128, dtype=torch.int8), torch.zeros(2, 1, 16, 128, dtype=torch.int8), torch.zeros(2, 1, 1), torch.zeros(2, 1, 1))
+    table, pos0 = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    x = torch.zeros(1, 1, 128).half()
+    for f in (lambda: ops.kv8_append(cache, x, x, table, pos0), lambda: ops.kv8_attention(x, cache, table, pos0), lambda: ops.kv8_step(x, x, x, cache, table, pos0),
+              lambda: ops.kv8_read(cache, table, pos0, 1), lambda: ops.kv_copy_pages([x[None]], [0], [0])):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_the_reference_keeps_half_a_step():
+    """The oracle itself: what it holds is within half a step of what it was given, after growth within a step and a half."""
+    rng = np.random.default_rng(0)
+    c = kv8_ref.Cache([torch.zeros(3, 2, 32, 128, dtype=torch.int8), torch.zeros(3, 2, 32, 128, dtype=torch.int8), torch.zeros(3, 2, 2), torch.zeros(3, 2, 2)],
+                      torch.tensor([[2, 0]], dtype=torch.int32))
+    x = rng.standard_normal((40, 2, 128)).astype(np.float32)
+    kv8_ref.append(c, x, -x, [0])
+    k, v = c.values(0, 40)
+    step = np.repeat(np.concatenate([c.ks[2], c.ks[0]], 1), 16, 1).T[:40, :, None]
+    assert (np.abs(k - x) <= step * 0.5000001).all() and (np.abs(v + x) <= step * 0.5000001).all()
+    y = 3 * rng.standard_normal((1, 2, 128)).astype(np.float32)
+    kv8_ref.append(c, y, y, [40])
+    k, _ = c.values(0, 41)
+    step = np.repeat(np.concatenate([c.ks[2], c.ks[0]], 1), 16, 1).T[:41, :, None]
+    assert (np.abs(k[:40] - x) <= step[:40] * 1.0001).all() and (np.abs(k[40:] - y) <= step[40:] * 0.5000001).all()
