@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(AppendParams<T> 
     }
     most = warp_max(most);
     const float was = older ? *scale : 0.f;
-    float now = __fdiv_rn(most, 127.f);
+    float now = most * (1.f / 127.f);
     now = now < KA_LEAST_SCALE ? 0.f : now;
     now = fmaxf(was, now);
     const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f;

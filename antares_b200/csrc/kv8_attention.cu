@@ -1,87 +1,521 @@
 // Attention over the 8-bit paged KV cache (layout: kv8.cuh): row r of sequence s, at position pos0[s] + r, over the cache's
 // positions 0 .. pos0[s] + r; query head h reads kv head h / (Hq / Hkv).  A row with no position to attend to gives zeros.
+//
+// Mathematics.  K and V codes are integers that fp16 holds exactly, so both products run on the tensor cores' fp16 form
+// with fp32 sums and nothing of the cache is rounded.  A block of 16 keys has one scale for K and one for V:
+//   x  = (q . k_code) * scale log2(e) ks + log2(vs)          the exponent of p vs
+//   P  = 2^(x - m)                                           at most 2^8, whatever the scales
+//   O += P v_code,  l += sum P / vs,  result O / l
+// so the V scale costs one addition where the maximum is subtracted anyway, and no product can leave fp16's range.  The
+// maximum m is only raised when a score exceeds it by more than 2^8 (then O and l are rescaled).  P goes in as a pair of
+// fp16 numbers, 22 bits; queries in fp32 too.
 #include <math_constants.h>
 
 #include "kv8.cuh"
 
 namespace ab200 {
 
+constexpr int KD_WARPS = 4, KD_THREADS = KD_WARPS * 32, KD_STAGES = 4;
+constexpr int KD_STAGE_BYTES = 2 * KV8_BLOCK * KV8_D;  // a block of K, a block of V
+constexpr int KD_LEAST = 8;                            // blocks a CTA takes at least, two a warp
+constexpr float KD_RAISE = 8.f, KD_P_EXP = 6.f;        // P is scaled by 2^6: its second half stays out of fp16's subnormals
+constexpr float KD_LEAST_SCALE = 0x1p-100f;            // a V scale below it is a block of zeros
 
-constexpr int KD_THREADS = 128, KD_WARPS = KD_THREADS / 32;
-
-template <typename T>
-struct AttendParams {
+struct DecodeParams {
   Kv8Cache c;
   Kv8Rows r;
-  const T *q;
+  const void *q;
   long q_stride;
-  T *out;
-  int Hq;
-  float scale;
+  void *out;
+  int Hq, group;
+  float scale;               // times log2(e)
+  const float *inv_freq;     // rotate the queries, or nullptr
+  int few;                   // sequences with more rows than this (rows x group) are another kernel's
+  float *partial;            // [CTAs][2][rows][128], then [CTAs][2][rows][2]: maximum, sum
+  int4 *split;               // [CTAs]: what is begun in CTA c and ended in a later one: CTAs, first row, kv head | rows - 1 << 16 |
+                             // rows with nothing to attend to << 20, first packed row
   int *status;
 };
 
-// A CTA per row and query head; a warp takes every fourth key, a lane four dims; running maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(KD_THREADS) kv8_attention_kernel(AttendParams<T> p) {
-  __shared__ int seq_s;
-  __shared__ float m_s[KD_WARPS], l_s[KD_WARPS], o_s[KD_WARPS][KV8_D];
-  const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __forceinline__ uint32_t kd_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void kd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void kd_ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void kd_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float kd_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two of a word's four codes (flipped to 0 .. 255) as fp16: 1024 + u is the half 0x6400 | u, and 1152 less is exact.
+template <int SEL>
+__device__ __forceinline__ uint32_t kd_half2(uint32_t flipped) {
+  return h22u(__hsub2(u2h2(__byte_perm(flipped, 0x64646464u, SEL)), u2h2(0x64806480u)));
+}
+
+// One tile of packed query rows (row j = token j / group, head j % group of the kv head's) over blocks of keys.
+struct Tile {
+  int s, hk, row0, rows, first, last;  // first row of the sequence in q, rows x group of the sequence, packed rows first .. last
+  long pos0;
+};
+
+// The blocks that tile t of sequence s attends to (one at least: a row with no key is written by the CTA that has it).
+template <int ROWS>
+__device__ __forceinline__ int kd_blocks(const DecodeParams &p, long pos0, int packed, int t) {
+  const int last = min((t + 1) * ROWS, packed) - 1;
+  const long limit = min(pos0 + last / p.group + 1, (long)p.r.max_pages << p.c.shift);
+  return max(1, (int)((max(limit, 0l) + 15) >> 4));
+}
+template <int ROWS>
+__device__ __forceinline__ long kd_weight(const DecodeParams &p, int s) {  // blocks of all tiles of sequence s, one kv head
+  const int packed = max(0, p.r.end(s) - p.r.begin(s)) * p.group;
+  if (packed == 0 || packed > p.few) return 0;
+  const long pos0 = p.r.pos0[s];
+  long w = 0;
+  for (int t = 0; t * ROWS < packed; ++t) w += kd_blocks<ROWS>(p, pos0, packed, t);
+  return w;
+}
+
+// ROWS: packed query rows of a tile.  With 8, rows 8-15 of the tensor cores' tile carry the second halves: of P always,
+// of q where LO (fp32 or rotated queries); with 16, each half is a product of its own.
+template <typename T, int ROWS, bool LO>
+__global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kernel(const __grid_constant__ DecodeParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float scales_s[KD_WARPS][KD_STAGES][2];
+  __shared__ long scan_s[KD_WARPS];
+  __shared__ long found_start;
+  __shared__ int found_s;
+  __shared__ float m_s[KD_WARPS][ROWS], l_s[KD_WARPS][ROWS];
+  constexpr int NR = ROWS / 8;  // query rows a thread holds: lane / 4, and 8 more
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j4 = lane & 3;
   const Kv8Rows &r = p.r;
   pdl_launch_dependents();
   pdl_wait();
-  if (tid == 0) seq_s = r.cu ? -1 : row / r.n;
+
+  // ---- this CTA's share: blocks w0 .. w1 - 1 of all, ordered by sequence, kv head, tile, block
+  long mine = 0;
+  for (int s = tid; s < r.S; s += KD_THREADS) mine += kd_weight<ROWS>(p, s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) scan_s[warp] = mine;
   __syncthreads();
-  if (r.cu) {
-    for (int s = tid; s < r.S; s += KD_THREADS)
-      if (row >= r.begin(s) && row < r.end(s)) seq_s = s;
+  long total = 0;
+#pragma unroll
+  for (int w = 0; w < KD_WARPS; ++w) total += scan_s[w];
+  total *= p.c.H;
+  const long per = max((total + gridDim.x - 1) / gridDim.x, (long)KD_LEAST);
+  const long w0 = blockIdx.x * per, w1 = min(w0 + per, total);
+  if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (w0 >= w1) return;
+  long before = 0;
+  for (int base = 0; base < r.S; base += KD_THREADS) {
+    const int s = base + tid;
+    const long w = s < r.S ? kd_weight<ROWS>(p, s) * p.c.H : 0;
+    long incl = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
     __syncthreads();
+    if (lane == 31) scan_s[warp] = incl;
+    __syncthreads();
+    long chunk = 0;
+#pragma unroll
+    for (int i = 0; i < KD_WARPS; ++i) {
+      if (i < warp) incl += scan_s[i];
+      chunk += scan_s[i];
+    }
+    const long start = before + incl - w;
+    if (w0 >= start && w0 < start + w) found_s = s, found_start = start;
+    before += chunk;
+    if (before > w0) break;
   }
-  const int s = seq_s;
-  if (s < 0) return;
-  const int hk = h / (p.Hq / p.c.H);
-  const int limit = (int)max(0l, min((long)r.pos0[s] + row - r.begin(s) + 1, (long)r.max_pages << p.c.shift));
-  float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -CUDART_INF_F, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = (float)p.q[(size_t)row * p.q_stride + (size_t)h * KV8_D + 4 * lane + i];
-  for (int pos = warp; pos < limit; pos += KD_WARPS) {
-    const long page = max(kv8_page(p.c, r, s, pos, p.status), 0l);
-    const size_t at = (size_t)page * p.c.H + hk;
-    const int in = pos & ((1 << p.c.shift) - 1);
-    const size_t elt = ((at << p.c.shift) + in) * KV8_D + 4 * lane, blk = (at << (p.c.shift - 4)) + (in >> 4);
-    const uint32_t kw = *reinterpret_cast<const uint32_t *>(p.c.k + elt), vw = *reinterpret_cast<const uint32_t *>(p.c.v + elt);
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dot = fmaf(q[i], (float)(int8_t)(kw >> (8 * i)), dot);
-    dot = warp_sum(dot) * p.c.ks[blk] * p.scale;
-    const float m_new = fmaxf(m, dot);
-    const float f = expf(m - m_new), w = expf(dot - m_new), wv = w * p.c.vs[blk];
-    l = fmaf(l, f, w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(acc[i], f, wv * (float)(int8_t)(vw >> (8 * i)));
-    m = m_new;
-  }
-  if (lane == 0) m_s[warp] = m, l_s[warp] = l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o_s[warp][4 * lane + i] = acc[i];
   __syncthreads();
-  float mx = -CUDART_INF_F, sum = 0.f, o = 0.f;
+  int s = found_s;
+  long start = found_start;
+
+  const uint32_t ring = kd_smem(smem) + warp * (KD_STAGES * KD_STAGE_BYTES);
+  // 16-byte piece i * 32 + lane of a block: row i * 4 + lane / 8, and its place under the XOR of row and piece that ldmatrix wants
+  const uint32_t put0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), put1 = put0 ^ 64;
+  const uint32_t k_row = (lane & 7) * 128, k_sw = lane & 7, k_chunk = lane >> 3;
+  const uint32_t v_row = (lane & 15) * 128, v_chunk = lane >> 4;
+
+  for (long w = w0; w < w1;) {
+    // ---- the item that w lies in
+    Tile tl;
+    tl.s = s, tl.row0 = r.begin(s), tl.pos0 = r.pos0[s];
+    tl.rows = max(0, r.end(s) - tl.row0) * p.group;
+    const long per_head = kd_weight<ROWS>(p, s);
+    tl.hk = (int)((w - start) / per_head);
+    long at = (w - start) - tl.hk * per_head;
+    int t = 0, blocks = kd_blocks<ROWS>(p, tl.pos0, tl.rows, 0);
+    while (at >= blocks) at -= blocks, blocks = kd_blocks<ROWS>(p, tl.pos0, tl.rows, ++t);
+    tl.first = t * ROWS, tl.last = min(tl.first + ROWS, tl.rows) - 1;
+    const int b0 = (int)at, b1 = (int)min((long)blocks, at + (w1 - w));
+    const long cap = (long)r.max_pages << p.c.shift;
+    auto limit_of = [&](int packed) { return (int)max(0l, min(tl.pos0 + packed / p.group + 1, cap)); };
+    const int full = limit_of(tl.first);  // keys that every row attends to
+    const int any = limit_of(tl.last);
+
+    // ---- queries: thread's rows, dims 16 c + 4 j4 .. + 3 as the A operand of step c
+    uint32_t qh[NR][8][2], ql[LO ? NR : 1][8][2];
+    float back[NR];  // what undoes the power of two that fp32 queries are scaled by
+    int limit[NR];
 #pragma unroll
-  for (int w = 0; w < KD_WARPS; ++w) mx = fmaxf(mx, m_s[w]);
+    for (int n = 0; n < NR; ++n) {
+      const int packed = tl.first + 8 * n + g;
+      const bool in = packed <= tl.last;
+      limit[n] = in ? limit_of(packed) : 0x7fffffff;
+      const int token = in ? packed / p.group : 0, head = tl.hk * p.group + (in ? packed - token * p.group : 0);
+      const T *q = (const T *)p.q + (size_t)(tl.row0 + token) * p.q_stride + (size_t)head * KV8_D + 4 * j4;
+      float f[8][4];
 #pragma unroll
-  for (int w = 0; w < KD_WARPS; ++w) {
-    const float f = m_s[w] == -CUDART_INF_F ? 0.f : expf(m_s[w] - mx);
-    sum = fmaf(l_s[w], f, sum);
-    o = fmaf(o_s[w][tid], f, o);
+      for (int c = 0; c < 8; ++c) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 v = in ? *reinterpret_cast<const uint2 *>(q + 16 * c) : make_uint2(0, 0);
+          if constexpr (!LO) qh[n][c][0] = v.x, qh[n][c][1] = v.y;
+          const float2 a = __half22float2(u2h2(v.x)), b = __half22float2(u2h2(v.y));
+          f[c][0] = a.x, f[c][1] = a.y, f[c][2] = b.x, f[c][3] = b.y;
+        } else {
+          const float4 v = in ? *reinterpret_cast<const float4 *>(q + 16 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+          f[c][0] = v.x, f[c][1] = v.y, f[c][2] = v.z, f[c][3] = v.w;
+        }
+      }
+      back[n] = 1.f;
+      if constexpr (LO) {
+        if (p.inv_freq) {
+          const float pos = (float)(int)(tl.pos0 + token);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float sn, cs;
+              sincosf(pos * p.inv_freq[16 * c + 4 * j4 + e], &sn, &cs);
+              const float a = f[c][e], b = f[c + 4][e];
+              f[c][e] = a * cs - b * sn;
+              f[c + 4][e] = b * cs + a * sn;
+            }
+        }
+        float most = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(f[c][e]));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // the largest to 2^13 .. 2^14: its second half is then far above the subnormals
+        int e = 0;
+        if (most > 0.f && most < CUDART_INF_F) frexpf(most, &e);
+        e = max(-100, min(100, 14 - e));
+        const float up = __int_as_float((127 + e) << 23);
+        back[n] = __int_as_float((127 - e) << 23);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float a = f[c][2 * i] * up, b = f[c][2 * i + 1] * up;
+            const __half2 hi = __floats2half2_rn(a, b);
+            const float2 hf = __half22float2(hi);
+            qh[n][c][i] = h22u(hi);
+            ql[n][c][i] = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
+          }
+      }
+    }
+    float o[16][4], m[NR], l[NR];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) m[n] = -CUDART_INF_F, l[n] = 0.f;
+
+    // ---- this warp's blocks: b0 + warp, + 4, ...
+    const int live = min(b1, (any + 15) >> 4);  // blocks that hold a key
+    const int count = max(0, (live - b0 - warp + KD_WARPS - 1) / KD_WARPS);
+    const int32_t *row_table = r.table + (size_t)tl.s * r.table_stride;
+    int pages = 0;
+    auto issue = [&](int i) {
+      if (i < count) {
+        if ((i & 31) == 0) {  // the pages of the next 32 blocks, one a lane
+          const int b = b0 + warp + (i + lane) * KD_WARPS;
+          pages = i + lane < count ? row_table[(b << 4) >> p.c.shift] : 0;
+          if ((unsigned)pages >= (unsigned)p.c.pages) {
+            atomicExch(p.status, KV8_BAD_PAGE);
+            pages = 0;
+          }
+        }
+        const int b = b0 + warp + i * KD_WARPS, page = __shfl_sync(0xffffffffu, pages, i & 31);
+        const size_t head = (size_t)page * p.c.H + tl.hk;
+        const int in_page = (b << 4) & ((1 << p.c.shift) - 1);
+        const size_t from = ((head << p.c.shift) + in_page) * KV8_D + lane * 16;
+        const uint32_t to = ring + (i % KD_STAGES) * KD_STAGE_BYTES;
+        const int8_t *kp = p.c.k + from, *vp = p.c.v + from;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + n * 512 + (n & 1 ? put1 : put0)), "l"(kp + n * 512) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 2048 + n * 512 + (n & 1 ? put1 : put0)), "l"(vp + n * 512) : "memory");
+        }
+        if (lane < 2) {
+          const float *sc = (lane ? p.c.vs : p.c.ks) + (head << (p.c.shift - 4)) + (in_page >> 4);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(kd_smem(&scales_s[warp][i % KD_STAGES][lane])), "l"(sc) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < KD_STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < count; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(KD_STAGES - 2) : "memory");
+      __syncwarp();  // every lane's pieces have landed, and everyone is done with the stage that is filled next
+      issue(i + KD_STAGES - 1);
+      const uint32_t st = ring + (i % KD_STAGES) * KD_STAGE_BYTES;
+      const float ks = scales_s[warp][i % KD_STAGES][0] * p.scale, vs = scales_s[warp][i % KD_STAGES][1];
+      const bool zero = !(vs >= KD_LEAST_SCALE);
+      const float lvs = zero ? 0.f : __log2f(vs), inv_vs = zero ? 1.f : __fdividef(1.f, vs);
+      float sc[2][4];
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[hb][e] = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t x[4];
+          kd_ldsm(x, st + hb * 1024 + k_row + (((4 * cc + k_chunk) ^ k_sw) << 4));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t u = x[c] ^ 0x80808080u, lo2 = kd_half2<0x4140>(u), hi2 = kd_half2<0x4342>(u);
+            const int ch = 4 * cc + c;
+            if constexpr (ROWS == 8) {
+              kd_mma(sc[hb], qh[0][ch][0], LO ? ql[0][ch][0] : 0u, qh[0][ch][1], LO ? ql[0][ch][1] : 0u, lo2, hi2);
+            } else {
+              kd_mma(sc[hb], qh[0][ch][0], qh[NR - 1][ch][0], qh[0][ch][1], qh[NR - 1][ch][1], lo2, hi2);
+              if constexpr (LO) kd_mma(sc[hb], ql[0][ch][0], ql[NR - 1][ch][0], ql[0][ch][1], ql[NR - 1][ch][1], lo2, hi2);
+            }
+          }
+        }
+        if constexpr (ROWS == 8 && LO) sc[hb][0] += sc[hb][2], sc[hb][1] += sc[hb][3];
+      }
+      // exponents of p vs: thread's rows, keys 8 hb + 2 j4, + 1
+      const int key0 = (b0 + warp + i * KD_WARPS) * 16 + 2 * j4;
+      const bool masked = key0 - 2 * j4 + 16 > full;  // the same for the whole warp
+      bool raise = false;
+      float top[NR];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const float f = LO ? ks * back[n] : ks;
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float &x = sc[hb][2 * n + e];
+            x = fmaf(x, f, lvs);
+            if (masked && key0 + 8 * hb + e >= limit[n]) x = -CUDART_INF_F;
+          }
+        top[n] = fmaxf(fmaxf(sc[0][2 * n], sc[0][2 * n + 1]), fmaxf(sc[1][2 * n], sc[1][2 * n + 1]));
+        raise = raise || top[n] > m[n] + KD_RAISE;
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], 1));
+          top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], 2));
+          const float up = fmaxf(m[n], top[n]), f = m[n] == -CUDART_INF_F ? 0.f : kd_ex2(m[n] - up);
+          m[n] = up;
+          l[n] *= f;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            o[d][2 * n] *= f, o[d][2 * n + 1] *= f;
+            if constexpr (ROWS == 8) o[d][2] *= f, o[d][3] *= f;
+          }
+        }
+      }
+      uint32_t ph[NR][2], pl[NR][2];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const float shift = m[n] == -CUDART_INF_F ? 0.f : m[n] - KD_P_EXP;
+        float sum = 0.f;
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb) {
+          const float a = kd_ex2(sc[hb][2 * n] - shift), b = kd_ex2(sc[hb][2 * n + 1] - shift);
+          sum += a + b;
+          const __half2 hi = __floats2half2_rn(a, b);
+          const float2 hf = __half22float2(hi);
+          ph[n][hb] = h22u(hi);
+          pl[n][hb] = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
+        }
+        l[n] = fmaf(sum, inv_vs, l[n]);
+      }
+      if (!zero) {
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+          uint32_t x[4];
+          // keys 0-7 and 8-15 of piece c, then of piece c + 1; transposed: two keys, two dims a word
+          kd_ldsm_t(x, st + 2048 + v_row + (((c + v_chunk) ^ k_sw) << 4));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t u = x[2 * h] ^ 0x80808080u, v = x[2 * h + 1] ^ 0x80808080u;
+            const uint32_t e0 = kd_half2<0x4240>(u), e1 = kd_half2<0x4240>(v), d0 = kd_half2<0x4341>(u), d1 = kd_half2<0x4341>(v);
+            float(&even)[4] = o[2 * (c + h)];
+            float(&odd)[4] = o[2 * (c + h) + 1];
+            if constexpr (ROWS == 8) {
+              kd_mma(even, ph[0][0], pl[0][0], ph[0][1], pl[0][1], e0, e1);
+              kd_mma(odd, ph[0][0], pl[0][0], ph[0][1], pl[0][1], d0, d1);
+            } else {
+              kd_mma(even, ph[0][0], ph[NR - 1][0], ph[0][1], ph[NR - 1][1], e0, e1);
+              kd_mma(odd, ph[0][0], ph[NR - 1][0], ph[0][1], ph[NR - 1][1], d0, d1);
+              kd_mma(even, pl[0][0], pl[NR - 1][0], pl[0][1], pl[NR - 1][1], e0, e1);
+              kd_mma(odd, pl[0][0], pl[NR - 1][0], pl[0][1], pl[NR - 1][1], d0, d1);
+            }
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+
+    // ---- the four warps' parts to shared memory (the ring is idle), then joined
+    __syncthreads();
+    float *part = reinterpret_cast<float *>(smem);  // [warp][ROWS][128]
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+      if (j4 == 0) m_s[warp][8 * n + g] = m[n], l_s[warp][8 * n + g] = l[n];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {  // thread's dims of piece c: 16 c + 4 j4 + 0 .. 3
+        float4 v;
+        if constexpr (ROWS == 8)
+          v = make_float4(o[2 * c][0] + o[2 * c][2], o[2 * c + 1][0] + o[2 * c + 1][2], o[2 * c][1] + o[2 * c][3], o[2 * c + 1][1] + o[2 * c + 1][3]);
+        else
+          v = make_float4(o[2 * c][2 * n], o[2 * c + 1][2 * n], o[2 * c][2 * n + 1], o[2 * c + 1][2 * n + 1]);
+        *reinterpret_cast<float4 *>(part + ((warp * ROWS + 8 * n + g) * KV8_D + 16 * c + 4 * j4)) = v;
+      }
+    }
+    __syncthreads();
+    const bool whole = b0 == 0 && b1 == blocks;
+    const int empty = (int)max(0l, min((long)ROWS, -tl.pos0 * p.group - tl.first));  // leading rows with nothing to attend to
+    const int slot = b0 == 0 ? 1 : 0;
+    float *mine_o = p.partial + ((size_t)blockIdx.x * 2 + slot) * ROWS * KV8_D;
+    float *mine_ml = p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D + ((size_t)blockIdx.x * 2 + slot) * ROWS * 2;
+    for (int row = 0; row <= tl.last - tl.first; ++row) {
+      float mx = -CUDART_INF_F, sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int i = 0; i < KD_WARPS; ++i) mx = fmaxf(mx, m_s[i][row]);
+#pragma unroll
+      for (int i = 0; i < KD_WARPS; ++i) {
+        const float f = m_s[i][row] == -CUDART_INF_F ? 0.f : kd_ex2(m_s[i][row] - mx);
+        sum = fmaf(l_s[i][row], f, sum);
+        acc = fmaf(part[(i * ROWS + row) * KV8_D + tid], f, acc);
+      }
+      if (whole) {
+        const int packed = tl.first + row, token = packed / p.group, head = tl.hk * p.group + packed - token * p.group;
+        ((T *)p.out)[((size_t)(tl.row0 + token) * p.Hq + head) * KV8_D + tid] = (T)(row < empty ? 0.f : acc / sum);
+      } else {
+        mine_o[row * KV8_D + tid] = acc;
+        if (tid == 0) mine_ml[2 * row] = mx, mine_ml[2 * row + 1] = sum;
+      }
+    }
+    if (!whole && slot == 1 && tid == 0)  // begun here: the CTAs up to the one with the item's last block have the rest
+      p.split[blockIdx.x] = make_int4((int)((w - b0 + blocks - 1) / per) - (int)blockIdx.x + 1, tl.row0, tl.hk | (tl.last - tl.first) << 16 | empty << 20, tl.first);
+    __syncthreads();
+    w += b1 - b0;
+    while (w < w1) {  // the next sequence that has rows here
+      const long weight = kd_weight<ROWS>(p, s) * p.c.H;
+      if (w < start + weight) break;
+      start += weight;
+      ++s;
+    }
   }
-  p.out[((size_t)row * p.Hq + h) * KV8_D + tid] = (T)(limit > 0 ? o / sum : 0.f);
 }
 
-template <typename T>
-static int attend_launch(const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int Hq, float scale, cudaStream_t stream) {
-  AttendParams<T> p{c, r, (const T *)q, q_stride, (T *)out, Hq, scale, kernel_error_ptr()};
-  AB200_CUDA(launch_pdl(kv8_attention_kernel<T>, dim3(r.T, Hq), dim3(KD_THREADS), 0, stream, p));
+// Joins the parts of the items that several CTAs share.  A CTA per CTA of the first kernel and four rows; two warps a row,
+// each every second part.
+constexpr int KJ_ROWS = 4, KJ_THREADS = KJ_ROWS * 64;
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_constant__ DecodeParams p) {
+  __shared__ float4 acc_s[KJ_ROWS][32];
+  __shared__ float m_s[KJ_ROWS], l_s[KJ_ROWS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int4 split = p.split[blockIdx.x];
+  const int lane = threadIdx.x & 31, sub = (threadIdx.x >> 5) & 1, i = threadIdx.x >> 6, row = blockIdx.y * KJ_ROWS + i;
+  const int n = split.x, first = split.w, more = split.z >> 16 & 15, empty = split.z >> 20, hk = split.z & 0xFFFF;
+  if (n == 0) return;
+  const bool in = row <= more;
+  float m = -CUDART_INF_F, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (in) {
+    const float *ml = p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D;
+#pragma unroll 4
+    for (int c = sub; c < n; c += 2) {
+      const size_t at = ((size_t)(blockIdx.x + c) * 2 + (c == 0 ? 1 : 0)) * ROWS + row;
+      const float mc = ml[2 * at], lc = ml[2 * at + 1];
+      const float4 v = *reinterpret_cast<const float4 *>(p.partial + at * KV8_D + 4 * lane);
+      const float up = fmaxf(m, mc), f = m == -CUDART_INF_F ? 0.f : kd_ex2(m - up), fc = mc == -CUDART_INF_F ? 0.f : kd_ex2(mc - up);
+      l = l * f + lc * fc;
+      acc.x = acc.x * f + v.x * fc, acc.y = acc.y * f + v.y * fc, acc.z = acc.z * f + v.z * fc, acc.w = acc.w * f + v.w * fc;
+      m = up;
+    }
+    if (sub == 1) {
+      acc_s[i][lane] = acc;
+      if (lane == 0) m_s[i] = m, l_s[i] = l;
+    }
+  }
+  __syncthreads();
+  if (!in || sub == 1) return;
+  const float mc = m_s[i], lc = l_s[i], up = fmaxf(m, mc), f = m == -CUDART_INF_F ? 0.f : kd_ex2(m - up), fc = mc == -CUDART_INF_F ? 0.f : kd_ex2(mc - up);
+  const float4 v = acc_s[i][lane];
+  const float sum = l * f + lc * fc;
+  const int packed = first + row, token = packed / p.group, head = hk * p.group + packed - token * p.group;
+  T *out = (T *)p.out + ((size_t)(split.y + token) * p.Hq + head) * KV8_D + 4 * lane;
+  const float x[4] = {(acc.x * f + v.x * fc) / sum, (acc.y * f + v.y * fc) / sum, (acc.z * f + v.z * fc) / sum, (acc.w * f + v.w * fc) / sum};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(row < empty ? 0.f : x[e]);
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+struct DecodePlan {
+  int rows, ctas;
+  size_t partial_bytes, bytes;
+};
+static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv) {
+  DecodePlan d;
+  const long group = Hq / Hkv;
+  d.rows = (long)max_rows * group <= 8 ? 8 : 16;
+  d.ctas = sm_count() * (d.rows == 8 ? 3 : 2);
+  d.partial_bytes = (size_t)d.ctas * 2 * d.rows * (KV8_D + 2) * sizeof(float);
+  d.bytes = d.partial_bytes + (size_t)d.ctas * sizeof(int4);
+  return d;
+}
+
+template <typename T, int ROWS, bool LO>
+static int decode_launch(const DecodeParams &p, const DecodePlan &d, cudaStream_t stream) {
+  constexpr int smem = KD_WARPS * KD_STAGES * KD_STAGE_BYTES;
+  static_assert(smem >= KD_WARPS * ROWS * KV8_D * (int)sizeof(float), "the warps' parts fit into the ring");
+  AB200_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<T, ROWS, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  AB200_CUDA(launch_pdl(kv8_decode_kernel<T, ROWS, LO>, dim3(d.ctas), dim3(KD_THREADS), smem, stream, p));
+  AB200_CUDA(launch_pdl(kv8_join_kernel<T, ROWS>, dim3(d.ctas, ROWS / KJ_ROWS), dim3(KJ_THREADS), 0, stream, p));
   return AB200_OK;
+}
+
+static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, int D, float scale, int dtype,
+                  const float *inv_freq, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (r.T == 0 || r.S == 0) return AB200_OK;
+  const DecodePlan d = decode_plan(r.S, r.T, max_rows, Hq, c.H);
+  AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= d.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, d.bytes, workspace_bytes);
+  DecodeParams p{c, r, q, q_stride, out, Hq, Hq / c.H, scale * 1.4426950408889634f, inv_freq, 0x7fffffff, (float *)workspace,
+                 (int4 *)((char *)workspace + d.partial_bytes), kernel_error_ptr()};
+  AB200_REQUIRE(p.status != nullptr, "%s: cannot resolve the status word", who);
+  if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8, true>(p, d, stream) : decode_launch<float, 16, true>(p, d, stream);
+  if (inv_freq) return d.rows == 8 ? decode_launch<__half, 8, true>(p, d, stream) : decode_launch<__half, 16, true>(p, d, stream);
+  return d.rows == 8 ? decode_launch<__half, 8, false>(p, d, stream) : decode_launch<__half, 16, false>(p, d, stream);
 }
 
 static int attention_check(const char *who, const Kv8Cache &c, int T, const void *q, long q_stride, const void *out, int Hq, int D, int dtype) {
@@ -89,6 +523,7 @@ static int attention_check(const char *who, const Kv8Cache &c, int T, const void
   if (D != KV8_D) return fail(AB200_EUNSUPPORTED, "%s: head size %d is not the built size %d", who, D, KV8_D);
   AB200_REQUIRE(Hq > 0 && Hq <= 65535 && Hq % c.H == 0, "%s: %d query heads are not a multiple of %d kv heads", who, Hq, c.H);
   if (T == 0) return AB200_OK;
+  AB200_REQUIRE((long)T * Hq <= 1 << 30, "%s: %d rows of %d heads are beyond the built limits", who, T, Hq);
   const long vec = dtype == AB200_F16 ? 8 : 4;
   AB200_REQUIRE(q && out && aligned16(q) && aligned16(out) && q_stride % vec == 0 && q_stride >= (long)Hq * D,
                 "%s: q must be 16-byte aligned rows of at least %d values, a multiple of 16 bytes apart, and out 16-byte aligned", who, Hq * D);
@@ -100,8 +535,8 @@ static int attention_check(const char *who, const Kv8Cache &c, int T, const void
 using namespace ab200;
 
 extern "C" size_t ab200_kv8_attention_workspace_bytes(int S, int T, int max_rows, int Hq, int Hkv) {
-  (void)S, (void)T, (void)max_rows, (void)Hq, (void)Hkv;
-  return 0;
+  if (S <= 0 || T <= 0 || Hkv <= 0 || Hq < Hkv) return 0;
+  return decode_plan(S, T, max_rows, Hq, Hkv).bytes;
 }
 
 extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages,
@@ -112,9 +547,8 @@ extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, cons
   Kv8Rows r;
   int rc = kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_attention", c, T, q, q_stride, out, Hq, D, dtype);
-  if (rc || S == 0 || T == 0) return rc;
-  return dtype == AB200_F16 ? attend_launch<__half>(c, r, q, q_stride, out, Hq, scale, (cudaStream_t)stream)
-                            : attend_launch<float>(c, r, q, q_stride, out, Hq, scale, (cudaStream_t)stream);
+  if (rc) return rc;
+  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, D, scale, dtype, nullptr, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long q_stride, long k_stride, long v_stride, void *out, void *k_cache, void *v_cache,
@@ -127,10 +561,8 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   int rc = kv8_check("kv8_step", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_step", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc || S == 0 || T == 0) return rc;
-  // the rotated queries wait in `out`: a row's are read before its result is stored
   rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
-                        inv_freq ? q : nullptr, q_stride, inv_freq ? out : nullptr, (long)Hq * D, Hq, inv_freq, dtype, stream);
+                        nullptr, 0, nullptr, 0, 0, inv_freq, dtype, stream);
   if (rc) return rc;
-  return ab200_kv8_attention(inv_freq ? out : q, inv_freq ? (long)Hq * D : q_stride, out, k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride,
-                             max_pages, pos0_dev, nullptr, S, T, T / S, Hq, D, scale, dtype, workspace, workspace_bytes, stream);
+  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, D, scale, dtype, inv_freq, workspace, workspace_bytes, (cudaStream_t)stream);
 }

@@ -442,7 +442,7 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
 /* Writes the rows of k and v [T][Hkv][128] into the cache.  inv_freq (fp32, 64 values used; NULL: none) rotates k by halves
  * at the rows' positions first, and q [T][Hq][128] into q_out (both NULL: no queries; q_out may be q).  For each block that
  * new rows lie in and each head: scale = max(scale of the block if it holds rows before pos0, else 0; largest |value| of
- * the new rows / 127), codes = value / scale rounded to the nearest, ties to even; rows before the new ones are rounded again
+ * the new rows times 1/127, all fp32), codes = value / scale rounded to the nearest, ties to even; rows before the new ones are rounded again
  * if their scale grew; codes behind the new rows stay as they are.  8 bits hold no infinities or NaN: +-inf becomes the
  * code +-127, NaN 0, and neither counts for the scale.  A scale below 2^-100 is held as 0.  Rows at negative positions or
  * behind the table's max_pages are not stored.  fp32 rows are rotated in 64 bits, so that the codes are the definition's. */

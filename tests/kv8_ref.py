@@ -64,7 +64,7 @@ def append(c, k, v, pos0, cu=None, inv_freq=None):
                 rows = rows.astype(np.float32).astype(np.float64)
                 for h in range(codes.shape[1]):
                     finite = np.abs(rows[:, h][np.isfinite(rows[:, h])])
-                    most = np.float32(finite.max() if finite.size else 0) / np.float32(127)
+                    most = np.float32(finite.max() if finite.size else 0) * (np.float32(1) / np.float32(127))
                     most = np.float32(0) if most < 2.0 ** -100 else most
                     was = scales[page, h, i0 // BLOCK] if p0 > at else np.float32(0)
                     now = max(was, most)
@@ -78,11 +78,11 @@ def append(c, k, v, pos0, cu=None, inv_freq=None):
 
 
 def attention(c, q, pos0, cu=None, scale=None, inv_freq=None):
-    """(result, sum of p |v|, largest error weight of a score) float64 for q [T, Hq, 128] (numpy)."""
+    """(result, sum of p |v|, largest error of a score, what a p too small for its pair moves) float64 for q [T, Hq, 128] (numpy)."""
     T, Hq, _ = q.shape
     H = c.k.shape[1]
     scale = D ** -0.5 if scale is None else scale
-    out, spread, score = np.zeros(q.shape), np.zeros(q.shape), np.zeros((T, Hq, 1))
+    out, spread, score, tiny = np.zeros(q.shape), np.zeros(q.shape), np.zeros((T, Hq, 1)), np.zeros((T, Hq, 1))
     for s, (row0, n) in enumerate(rows_of(len(c.table), T, cu)):
         limits = [int(min(max(int(pos0[s]) + r + 1, 0), c.capacity)) for r in range(n)]
         if not n or not max(limits):
@@ -100,16 +100,20 @@ def attention(c, q, pos0, cu=None, scale=None, inv_freq=None):
             p = torch.softmax(sc[r, ..., :L], -1)
             out[row0 + r] = torch.einsum("hgl,lhd->hgd", p, v[:L]).reshape(Hq, D).numpy()
             spread[row0 + r] = torch.einsum("hgl,lhd->hgd", p, v[:L].abs()).reshape(Hq, D).numpy()
+            # p vs is held as a pair of fp16 numbers, scaled so that the largest is 2^6 or more: the pair's last step is 2^-24, half
+            # of it 2^-31 of the largest p vs, for every key, times a code of at most 127
+            steps = torch.tensor(np.array([c.vs[c.place(s, i)[0], :, c.place(s, i)[1] // BLOCK] for i in range(L)]), dtype=torch.float64)
+            tiny[row0 + r] = (L * 2.0 ** -31 * 127 * torch.einsum("hgl,lh->hgl", p, steps).amax(-1)).reshape(Hq, 1).numpy()
             mag = torch.einsum("hgd,lhd->hgl", x[r].abs(), k[:L].abs()).amax(-1)
             tall = torch.einsum("hg,lh->hgl", x[r].abs().amax(-1), k[:L].abs().sum(-1)).amax(-1)
             score[row0 + r] = (scale * (2.0 ** -19 * mag + 2.0 ** -21 * tall)).reshape(Hq, 1).numpy()
-    return out, spread, score
+    return out, spread, score, tiny
 
 
-def bound(want, spread, score, keys, dtype, q_half_steps=0.0, q_mag=0.0):
+def bound(want, spread, score, tiny, keys, dtype):
     """How far a result may be off `want`.  Half a step of its type.  A score is a sum of 128 exact products in eight steps
     of sixteen, each cut to 24 bits: 2^-19 of its magnitude holds twice that, and 2^-21 of the largest |q| times sum |k| a
     query kept as two 11-bit halves; e^error moves every p by twice the largest one's error.  p as two halves and its
-    exponential: 2^-20.  The sums over the keys, sixteen at a time: 2^-23 a step of sum p |v|."""
+    exponential: 2^-20, and `tiny` where the pair runs out of exponents.  The sums over the keys, sixteen at a time: 2^-23 a step of sum p |v|."""
     half = torch.finfo(dtype).eps / 2
-    return np.abs(want) * half * 1.01 + spread * (2 * score + 2.0 ** -20 + (keys / 16 + 8) * 2.0 ** -23) + (2.0 ** -25 if dtype == torch.float16 else 1e-30)
+    return np.abs(want) * half * 1.01 + spread * (2 * score + 2.0 ** -20 + (keys / 16 + 8) * 2.0 ** -23) + tiny + (2.0 ** -25 if dtype == torch.float16 else 1e-30)

@@ -53,10 +53,10 @@ def _cu(rows):
 
 
 def _check_attention(got, ref_cache, q, pos0, cu, keys, dtype, scale=None, inv_freq=None):
-    want, spread, score = kv8_ref.attention(ref_cache, q.double().cpu().numpy(), pos0, cu, scale, inv_freq)
+    want, spread, score, tiny = kv8_ref.attention(ref_cache, q.double().cpu().numpy(), pos0, cu, scale, inv_freq)
     got = got.double().cpu().numpy()
     assert np.isfinite(got).all()
-    off = np.abs(got - want) / kv8_ref.bound(want, spread, score, keys, dtype)
+    off = np.abs(got - want) / kv8_ref.bound(want, spread, score, tiny, keys, dtype)
     assert off.max() <= 1, "off by %.2f of the bound at %s" % (off.max(), np.unravel_index(off.argmax(), off.shape))
 
 
@@ -286,11 +286,11 @@ def test_step(cuda, past, n, hq, hkv, page, rope, dtype):
         assert torch.equal(a.view(torch.int8), b.view(torch.int8))
     # against the cache as it now is; a rotated query may be kept in its type: half a step of it moves every score
     ref = _ref(cache, table)
-    want, spread, score = kv8_ref.attention(ref, q.double().cpu().numpy(), past, None, None, INV_FREQ if rope else None)
+    want, spread, score, tiny = kv8_ref.attention(ref, q.double().cpu().numpy(), past, None, None, INV_FREQ if rope else None)
     if rope:
-        _, _, mag = kv8_ref.attention(ref, q.double().cpu().numpy(), past, None)
+        _, _, mag, _ = kv8_ref.attention(ref, q.double().cpu().numpy(), past, None)
         score = score + 1.5 * mag * 2.0 ** 19 * (torch.finfo(dtype).eps / 2 + 2.0 ** -21)
-    off = np.abs(out.double().cpu().numpy() - want) / kv8_ref.bound(want, spread, score, max(past) + n, dtype)
+    off = np.abs(out.double().cpu().numpy() - want) / kv8_ref.bound(want, spread, score, tiny, max(past) + n, dtype)
     assert off.max() <= 1, off.max()
     assert ops.kernel_status() == 0
 
@@ -420,7 +420,7 @@ def test_a_long_cache(cuda):
     p = torch.softmax(sc, -1)
     want, spread = torch.einsum("hgl,lhd->hgd", p, vv).view(1, hq, 128), torch.einsum("hgl,lhd->hgd", p, vv.abs()).view(1, hq, 128)
     mag = torch.einsum("hgd,lhd->hgl", q[0].double().abs().view(hkv, hq // hkv, 128), kk.abs()).amax(-1).view(1, hq, 1) * 128 ** -0.5
-    b = kv8_ref.bound(want.cpu().numpy(), spread.cpu().numpy(), (mag * 2.0 ** -18).cpu().numpy(), past, F16)
+    b = kv8_ref.bound(want.cpu().numpy(), spread.cpu().numpy(), (mag * 2.0 ** -18).cpu().numpy(), 0.0, past, F16)
     assert (np.abs((got - want).cpu().numpy()) <= b).all()
     back, _ = ops.kv8_read((k, v, ks, vs), table, _ints([past]), 1)
     assert torch.equal(back, (kk[-1:].float()).half())
