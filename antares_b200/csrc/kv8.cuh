@@ -50,6 +50,7 @@ inline int kv8_check(const char *who, const void *k, const void *v, const void *
   while (shift < 30 && (1 << shift) < page_rows) ++shift;
   AB200_REQUIRE(page_rows >= KV8_BLOCK && (1 << shift) == page_rows, "%s: page_rows=%d must be a power of two from %d", who, page_rows, KV8_BLOCK);
   AB200_REQUIRE(pages > 0 && Hkv > 0 && Hkv <= 65535, "%s: bad cache, pages=%d heads=%d", who, pages, Hkv);
+  AB200_REQUIRE((long)pages * Hkv << (shift - 4) < 1l << 31, "%s: %d pages of %d heads and %d rows are more blocks than the built 2^31", who, pages, Hkv, page_rows);
   AB200_REQUIRE(S >= 0 && T >= 0 && max_pages > 0 && table_stride >= max_pages, "%s: bad shape S=%d T=%d max_pages=%d table_stride=%ld", who, S, T, max_pages, table_stride);
   AB200_REQUIRE((long)max_pages << shift <= 1l << 30, "%s: %d pages of %d rows are more positions than the built 2^30", who, max_pages, page_rows);
   AB200_REQUIRE(T <= 1 << 28 && S <= 1 << 20, "%s: T=%d rows of S=%d sequences are beyond the built limits", who, T, S);
