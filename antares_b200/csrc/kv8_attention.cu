@@ -19,9 +19,9 @@ namespace ab200 {
 constexpr int KD_WARPS = 4, KD_THREADS = KD_WARPS * 32, KD_STAGES = 4;
 constexpr int KD_STAGE_BYTES = 2 * KV8_BLOCK * KV8_D;  // a block of K, a block of V
 constexpr int KD_LEAST = 8;                            // blocks a CTA takes at least, two a warp
-constexpr int KD_ITEM = 8;                             // what an item costs besides its blocks, in blocks
+constexpr int KD_ITEM = 16;                            // what an item costs besides its blocks, in blocks: 7800 cycles against 470 a block
 constexpr float KD_RAISE = 8.f, KD_P_EXP = 6.f;        // P is scaled by 2^6: its second half stays out of fp16's subnormals
-constexpr float KD_LEAST_SCALE = 0x1p-100f;            // a V scale below it is a block of zeros
+constexpr float KD_LEAST_SCALE = 0x1p-100f;            // a V scale below it (a block of zeros) counts as this
 
 struct DecodeParams {
   Kv8Cache c;
@@ -45,16 +45,30 @@ __device__ __forceinline__ void kd_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void kd_imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// The first product of a chain starts from KD_ZERO: an integer below 2^22 added to these bits is that integer plus 1.5 * 2^23
+// as a float, so a subtraction reads the sum and nothing is converted.
+constexpr int KD_ZERO = 0x4B400000;
+__device__ __forceinline__ float kd_sum(int bits) { return __int_as_float(bits) - 12582912.f; }
+__device__ __forceinline__ void kd_imma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 __device__ __forceinline__ void kd_ldsm(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void kd_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float kd_lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float kd_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ float kd_ex2(float x) {
   float y;
@@ -85,162 +99,200 @@ __device__ __forceinline__ long kd_weight(const DecodeParams &p, int s) {  // wo
   return w;
 }
 
+__device__ __forceinline__ long kd_div(long a, long b) {  // a, b >= 0; most fit into 32 bits, where a division is a fifth of the work
+  return ((a | b) >> 32) == 0 ? (long)((unsigned)a / (unsigned)b) : a / b;
+}
+// What the threads before this one hold together; *total grows by what all hold.
+__device__ __forceinline__ long kd_scan(long v, long (&s)[KD_WARPS], long *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  __syncthreads();
+  if (lane == 31) s[warp] = incl;
+  __syncthreads();
+  long all = 0;
+#pragma unroll
+  for (int i = 0; i < KD_WARPS; ++i) {
+    if (i == warp) incl += all;
+    all += s[i];
+  }
+  *total += all;
+  return incl - v;
+}
+__device__ __forceinline__ void kd_store4(float *out, float4 v, float f) { *reinterpret_cast<float4 *>(out) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
+__device__ __forceinline__ void kd_store4(__half *out, float4 v, float f) {
+  *reinterpret_cast<uint2 *>(out) = make_uint2(h22u(__floats2half2_rn(v.x * f, v.y * f)), h22u(__floats2half2_rn(v.z * f, v.w * f)));
+}
+
 // ROWS: packed query rows of a tile.  With 8, rows 8-15 of the tensor cores' tile carry second parts: the second byte of
 // q, the second half of P; with 16, each part is a product of its own.
+// A warp takes two blocks at a time: two independent chains of products and exponentials.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int NR = ROWS / 8;  // query rows a thread holds: lane / 4, and 8 more
-  __shared__ float scales_s[KD_WARPS][KD_STAGES][2];
+  __shared__ __align__(16) float scales_s[KD_WARPS][KD_STAGES][2];
   __shared__ long scan_s[KD_WARPS];
   __shared__ long found_start;
   __shared__ int found_s;
-  __shared__ float m_s[KD_WARPS][ROWS], l_s[KD_WARPS][ROWS];
-  __shared__ uint32_t q_s[NR][3][8][32];  // bytes of the queries, as the lanes hold them
+  __shared__ float m_s[KD_WARPS][ROWS], l_s[KD_WARPS][ROWS], q_max_s[KD_WARPS][ROWS];
+  constexpr int BYTES = 3;                    // of a query value
+  __shared__ uint32_t q_s[NR][BYTES][8][32];  // as the lanes hold them
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j4 = lane & 3;
   const Kv8Rows &r = p.r;
   pdl_launch_dependents();
   pdl_wait();
 
   // ---- this CTA's share: w0 .. w1 - 1 of all work, ordered by sequence, kv head, tile, block
-  long mine = 0;
-  for (int s = tid; s < r.S; s += KD_THREADS) mine += kd_weight<ROWS>(p, s);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) scan_s[warp] = mine;
-  __syncthreads();
-  long total = 0;
-#pragma unroll
-  for (int w = 0; w < KD_WARPS; ++w) total += scan_s[w];
-  total *= p.c.H;
-  const long per = max((total + gridDim.x - 1) / gridDim.x, (long)KD_LEAST);
+  long total = 0, start = 0, weight = 0;
+  for (int base = 0; base < r.S; base += KD_THREADS) {
+    weight = base + tid < r.S ? kd_weight<ROWS>(p, base + tid) * p.c.H : 0;
+    const long before = total;
+    start = before + kd_scan(weight, scan_s, &total);
+  }
+  const long per = max((long)kd_div(total + gridDim.x - 1, gridDim.x), (long)KD_LEAST);
   const long w0 = blockIdx.x * per, w1 = min(w0 + per, total);
   if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
   if (w0 >= w1) return;
-  long before = 0;
-  for (int base = 0; base < r.S; base += KD_THREADS) {
-    const int s = base + tid;
-    const long w = s < r.S ? kd_weight<ROWS>(p, s) * p.c.H : 0;
-    long incl = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
+  if (r.S > KD_THREADS) total = 0;
+  for (int base = 0;;) {
+    if (r.S > KD_THREADS) {
+      weight = base + tid < r.S ? kd_weight<ROWS>(p, base + tid) * p.c.H : 0;
+      const long before = total;
+      start = before + kd_scan(weight, scan_s, &total);
     }
-    __syncthreads();
-    if (lane == 31) scan_s[warp] = incl;
-    __syncthreads();
-    long chunk = 0;
-#pragma unroll
-    for (int i = 0; i < KD_WARPS; ++i) {
-      if (i < warp) incl += scan_s[i];
-      chunk += scan_s[i];
-    }
-    const long start = before + incl - w;
-    if (w0 >= start && w0 < start + w) found_s = s, found_start = start;
-    before += chunk;
-    if (before > w0) break;
+    if (w0 >= start && w0 < start + weight) found_s = base + tid, found_start = start;
+    base += KD_THREADS;
+    if (total > w0 || base >= r.S) break;
   }
   __syncthreads();
   int s = found_s;
-  long start = found_start;
+  start = found_start;
+  long w = w0;
+  const long cap = (long)r.max_pages << p.c.shift;
+  // the next item, or part of one, in the share
+  struct Part {
+    long pos0, item;  // where the item begins in the order of all work
+    int seq, row0, rows, hk, first, last, blocks, b0, b1;  // packed rows first .. last, blocks b0 .. b1 - 1 of `blocks`
+  };
+  auto next = [&](Part &it) {
+    while (w < w1) {
+      const int row0 = r.begin(s), rows = max(0, r.end(s) - row0) * p.group;
+      const long per_head = kd_weight<ROWS>(p, s);
+      if (w >= start + per_head * p.c.H) {
+        start += per_head * p.c.H, ++s;
+        continue;
+      }
+      it.pos0 = r.pos0[s], it.seq = s, it.row0 = row0, it.rows = rows;
+      it.hk = (int)kd_div(w - start, per_head);
+      long at = (w - start) - it.hk * per_head;
+      int t = 0;
+      it.blocks = kd_blocks<ROWS>(p, it.pos0, rows, 0);
+      while (at >= it.blocks + KD_ITEM) at -= it.blocks + KD_ITEM, it.blocks = kd_blocks<ROWS>(p, it.pos0, rows, ++t);
+      it.first = t * ROWS, it.last = min(it.first + ROWS, rows) - 1;
+      const long take = min(it.blocks + KD_ITEM - at, w1 - w);
+      it.b0 = (int)max(0l, at - KD_ITEM), it.b1 = (int)max(0l, at + take - KD_ITEM);
+      it.item = w - at;
+      w += take;
+      if (it.b1 > 0) return true;  // else the share ends before the item's first block
+    }
+    return false;
+  };
 
-  const uint32_t ring = kd_smem(smem) + warp * (KD_STAGES * KD_STAGE_BYTES);
+  unsigned char *const ring_mine = smem + warp * (KD_STAGES * KD_STAGE_BYTES);
+  const uint32_t ring = kd_smem(ring_mine);
   // 16-byte piece i * 32 + lane of a block: row i * 4 + lane / 8, and its place under the XOR of row and piece that ldmatrix wants
   const uint32_t put0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), put1 = put0 ^ 64;
   const uint32_t k_at = (lane & 7) * 128 + (((lane >> 3) ^ (lane & 7)) << 4);                         // pieces 0-3; pieces 4-7: ^ 64
   const uint32_t v_row = 2048 + (lane & 15) * 128, v_sw = lane & 7, v_chunk = lane >> 4;
   const int8_t *const k_lane = p.c.k + lane * 16, *const v_lane = p.c.v + lane * 16;
   const float *const sc_lane = lane ? p.c.vs : p.c.ks;
+  const uint32_t sc_put = kd_smem(&scales_s[warp][0][0]) + 4 * lane;
+  static_assert(KD_STAGES == 4 && KD_STAGE_BYTES == 4096, "two pairs of blocks; a pair's scales lie 16 bytes after the other's");
+  const int nothing[4] = {KD_ZERO, KD_ZERO, KD_ZERO, KD_ZERO};
 
-  for (long w = w0; w < w1;) {
-    // ---- the item that w lies in
-    const int row0 = r.begin(s), rows = max(0, r.end(s) - row0) * p.group;
-    const long pos0 = r.pos0[s], cap = (long)r.max_pages << p.c.shift, per_head = kd_weight<ROWS>(p, s);
-    const int hk = (int)((w - start) / per_head);
-    long at = (w - start) - hk * per_head;
-    int t = 0, blocks = kd_blocks<ROWS>(p, pos0, rows, 0);
-    while (at >= blocks + KD_ITEM) at -= blocks + KD_ITEM, blocks = kd_blocks<ROWS>(p, pos0, rows, ++t);
-    const int first = t * ROWS, last = min(first + ROWS, rows) - 1;  // packed rows of the tile
-    const long take = min(blocks + KD_ITEM - at, w1 - w);
-    const int b0 = (int)max(0l, at - KD_ITEM), b1 = (int)max(0l, at + take - KD_ITEM);
-    const long item = w - at;
-    w += take;
-    const int seq = s;
-    if (w < w1) {  // the next sequence that has rows here
-      long weight = per_head * p.c.H;
-      while (w >= start + weight) start += weight, weight = kd_weight<ROWS>(p, ++s) * p.c.H;
-    }
-    if (b1 == 0) continue;  // ended before the item's first block
-    auto limit_of = [&](int packed) { return (int)max(0l, min(pos0 + packed / p.group + 1, cap)); };
-    const int full = limit_of(first), any = limit_of(last);  // keys that every row, that some row attends to
-
-    // ---- this warp's blocks: b0 + warp, + 4, ...
-    const int live = min(b1, (any + 15) >> 4);  // blocks that hold a key
-    const int count = max(0, (live - b0 - warp + KD_WARPS - 1) / KD_WARPS);
-    const int32_t *row_table = r.table + (size_t)seq * r.table_stride;
-    int where = 0, put = 0, asked = 0;
-    auto issue = [&]() {
-      if (asked < count) {
-        if ((asked & 31) == 0 && asked + lane < count) {  // where the next 32 blocks lie, one a lane
-          const int b = b0 + warp + (asked + lane) * KD_WARPS;
-          int page = row_table[b >> (p.c.shift - 4)];
-          if ((unsigned)page >= (unsigned)p.c.pages) {
-            atomicExch(p.status, KV8_BAD_PAGE);
-            page = 0;
-          }
-          where = ((page * p.c.H + hk) << (p.c.shift - 4)) + (b & ((1 << (p.c.shift - 4)) - 1));
+  // ---- this warp's blocks of a part: the pairs b0 + 2 (warp, warp + 4, ...).  The second of an odd last pair is the first
+  // again, its keys masked like all behind `end`.
+  Part it = {};
+  int live = 0, pairs = 0, asked = 0, where = 0;
+  uint32_t put = 0;
+  auto limit_of = [&](int packed) { return (int)max(0l, min(it.pos0 + packed / p.group + 1, cap)); };
+  auto issue = [&]() {
+    if (asked < pairs) {
+      if ((asked & 15) == 0) {  // where the next 16 pairs' blocks lie, one a lane
+        const int b = min(it.b0 + 2 * (warp + (asked + (lane >> 1)) * KD_WARPS) + (lane & 1), live - 1);
+        int page = r.table[(size_t)it.seq * r.table_stride + (b >> (p.c.shift - 4))];
+        if ((unsigned)page >= (unsigned)p.c.pages) {
+          atomicExch(p.status, KV8_BAD_PAGE);
+          page = 0;
         }
-        const int blk = __shfl_sync(0xffffffffu, where, asked & 31);
-        const int8_t *kp = k_lane + (size_t)blk * (KV8_BLOCK * KV8_D), *vp = v_lane + (size_t)blk * (KV8_BLOCK * KV8_D);
-        const uint32_t to = ring + put * KD_STAGE_BYTES;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + n * 512 + (n & 1 ? put1 : put0)), "l"(kp + n * 512) : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 2048 + n * 512 + (n & 1 ? put1 : put0)), "l"(vp + n * 512) : "memory");
-        }
-        if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(kd_smem(&scales_s[warp][put][lane])), "l"(sc_lane + blk) : "memory");
-        ++asked;
-        put = put == KD_STAGES - 1 ? 0 : put + 1;
+        where = ((page * p.c.H + it.hk) << (p.c.shift - 4)) + (b & ((1 << (p.c.shift - 4)) - 1));
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
 #pragma unroll
-    for (int i = 0; i < KD_STAGES - 1; ++i) issue();
+      for (int u = 0; u < 2; ++u) {
+        const int blk = __shfl_sync(0xffffffffu, where, 2 * (asked & 15) + u);
+        const int8_t *kp = k_lane + (size_t)blk * (KV8_BLOCK * KV8_D), *vp = v_lane + (size_t)blk * (KV8_BLOCK * KV8_D);
+        const uint32_t to0 = ring + put + put0, to1 = ring + put + put1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((i & 1 ? to1 : to0) + u * KD_STAGE_BYTES + i * 512), "l"(kp + i * 512) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((i & 1 ? to1 : to0) + u * KD_STAGE_BYTES + 2048 + i * 512), "l"(vp + i * 512) : "memory");
+        }
+        if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_put + (put >> 9) + 8 * u), "l"(sc_lane + blk) : "memory");
+      }
+      ++asked;
+      put ^= 2 * KD_STAGE_BYTES;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto begin = [&]() {
+    live = min(it.b1, (limit_of(it.last) + 15) >> 4);  // blocks that hold a key some row attends to
+    pairs = max(0, ((live - it.b0 + 1) / 2 - warp + KD_WARPS - 1) / KD_WARPS);
+    asked = 0, put = 0;
+    issue();
+  };
 
+  bool more = next(it);
+  if (more) begin();
+  while (more) {
     // ---- queries, meanwhile.  A warp takes the pieces warp and warp + 4 (a rotated pair is one thread's): thread's row(s),
-    // dims 16 c + 4 j4 .. + 3.  Each row is scaled by a power of two, its largest to 2^21 .. 2^22, rounded to an integer
-    // and cut into three signed bytes (the first is 64 at most): half a step is 2^-22 of the largest, and fp16 rows are
-    // exact unless they span more than 11 octaves.
+    // dims 16 c + 4 j4 .. + 3.  Each row is scaled by a power of two, its largest to 2^21 .. 2^22, rounded to an
+    // integer and cut into signed bytes (the first is 64 at most): half a step is 2^-22 of the largest, and fp16 rows are exact
+    // unless they span more than 11 octaves.
     float f[NR][2][4], back[NR];
     int limit[NR];
+    const int end = 16 * live;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const int packed = first + 8 * n + g;
-      const bool in = packed <= last;
-      limit[n] = in ? limit_of(packed) : 0x7fffffff;
-      const int token = in ? packed / p.group : 0, head = hk * p.group + (in ? packed - token * p.group : 0);
-      const T *q = (const T *)p.q + (size_t)(row0 + token) * p.q_stride + (size_t)head * KV8_D + 16 * warp + 4 * j4;
+    for (int i = 0; i < NR; ++i) {
+      const int packed = it.first + 8 * i + g;
+      const bool in = packed <= it.last;
+      limit[i] = in ? min(limit_of(packed), end) : end;
+      const int token = in ? packed / p.group : 0, head = it.hk * p.group + (in ? packed - token * p.group : 0);
+      const T *q = (const T *)p.q + (size_t)(it.row0 + token) * p.q_stride + (size_t)head * KV8_D + 16 * warp + 4 * j4;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if constexpr (sizeof(T) == 2) {
           const uint2 v = in ? *reinterpret_cast<const uint2 *>(q + 64 * c) : make_uint2(0, 0);
           const float2 a = __half22float2(u2h2(v.x)), b = __half22float2(u2h2(v.y));
-          f[n][c][0] = a.x, f[n][c][1] = a.y, f[n][c][2] = b.x, f[n][c][3] = b.y;
+          f[i][c][0] = a.x, f[i][c][1] = a.y, f[i][c][2] = b.x, f[i][c][3] = b.y;
         } else {
           const float4 v = in ? *reinterpret_cast<const float4 *>(q + 64 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-          f[n][c][0] = v.x, f[n][c][1] = v.y, f[n][c][2] = v.z, f[n][c][3] = v.w;
+          f[i][c][0] = v.x, f[i][c][1] = v.y, f[i][c][2] = v.z, f[i][c][3] = v.w;
         }
       }
       if (p.inv_freq) {
-        const float pos = (float)(int)(pos0 + token);
+        const float pos = (float)(int)(it.pos0 + token);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float sn, cs;
           sincosf(pos * p.inv_freq[16 * warp + 4 * j4 + e], &sn, &cs);
-          const float a = f[n][0][e], b = f[n][1][e];
-          f[n][0][e] = a * cs - b * sn;
-          f[n][1][e] = b * cs + a * sn;
+          const float a = f[i][0][e], b = f[i][1][e];
+          f[i][0][e] = a * cs - b * sn;
+          f[i][1][e] = b * cs + a * sn;
         }
       }
       // a row that is not finite is made of NaN: its largest, as a bit pattern, is above that of every number
@@ -248,28 +300,28 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(f[n][c][e]) & 0x7fffffffu);
+        for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(f[i][c][e]) & 0x7fffffffu);
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      if (j4 == 0) m_s[warp][8 * n + g] = __uint_as_float(most);
+      if (j4 == 0) q_max_s[warp][8 * i + g] = __uint_as_float(most);
     }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       uint32_t most = 0;
 #pragma unroll
-      for (int i = 0; i < KD_WARPS; ++i) most = max(most, __float_as_uint(m_s[i][8 * n + g]));
+      for (int i = 0; i < KD_WARPS; ++i) most = max(most, __float_as_uint(q_max_s[i][8 * n + g]));
       const int e = max(-100, min(100, 21 - (int)(most >> 23) + 127));
       const float up = __int_as_float((127 + e) << 23);
       back[n] = most >= 0x7f800000u ? CUDART_NAN_F : __int_as_float((127 - e) << 23);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t part[3] = {0, 0, 0};
+        uint32_t part[BYTES] = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           int v = __float2int_rn(f[n][c][i] * up);
 #pragma unroll
-          for (int k = 2; k > 0; --k) {
+          for (int k = BYTES - 1; k > 0; --k) {
             const int low = (int)(int8_t)v;
             part[k] |= (uint32_t)(low & 255) << (8 * i);
             v = (v - low) >> 8;
@@ -277,17 +329,20 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
           part[0] |= (uint32_t)(v & 255) << (8 * i);
         }
 #pragma unroll
-        for (int k = 0; k < 3; ++k) q_s[n][k][warp + 4 * c][lane] = part[k];
+        for (int k = 0; k < BYTES; ++k) q_s[n][k][warp + 4 * c][lane] = part[k];
       }
     }
     __syncthreads();
-    uint32_t qa[NR][3][8];
+    // A operands: step c (dims 32 c .. + 31), product i
+    constexpr int PRODUCTS = ROWS == 8 ? 2 : 3;
+    uint32_t qa[4][PRODUCTS][4];
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int k = 0; k < 3; ++k)
+      for (int i = 0; i < PRODUCTS; ++i)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) qa[n][k][c] = q_s[n][k][c][lane];
+        for (int e = 0; e < 4; ++e)
+          qa[c][i][e] = ROWS == 8 ? q_s[0][i == 0 ? e & 1 : 2][2 * c + (e >> 1)][lane] : q_s[NR == 2 ? e & 1 : 0][i][2 * c + (e >> 1)][lane];
     float o[16][4], m[NR], l[NR];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -296,67 +351,69 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
 #pragma unroll
     for (int n = 0; n < NR; ++n) m[n] = -CUDART_INF_F, l[n] = 0.f;
 
-    int get = 0, key0 = (b0 + warp) * 16;
-    for (int i = 0; i < count; ++i, key0 += 16 * KD_WARPS) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(KD_STAGES - 2) : "memory");
-      __syncwarp();  // every lane's pieces have landed, and everyone is done with the stage that is filled next
+    const int full = min(limit_of(it.first), end);  // keys that every row attends to
+    uint32_t get = 0;
+    int key0 = (it.b0 + 2 * warp) * 16;
+    for (int i = 0; i < pairs; ++i, key0 += 32 * KD_WARPS, get ^= 2 * KD_STAGE_BYTES) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();  // every lane's pieces have landed, and everyone is done with the pair that is filled next
       issue();
-      const uint32_t st = ring + get * KD_STAGE_BYTES;
-      const float ks = scales_s[warp][get][0] * p.scale, vs = scales_s[warp][get][1];
-      get = get == KD_STAGES - 1 ? 0 : get + 1;
-      const bool zero = !(vs >= KD_LEAST_SCALE);
-      const float lvs = zero ? 0.f : __log2f(vs), inv_vs = zero ? 1.f : __fdividef(1.f, vs);
-      // q . k: bytes times bytes, exact; thread's rows, keys 8 hb + 2 j4, + 1
-      float x[NR][4];
+      const uint32_t st = ring + get;
+      const float4 scales = *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(&scales_s[warp][0][0]) + (get >> 9));
+      float x[2][NR][4], inv_vs[2];  // exponents of p vs: thread's rows, keys 8 hb + 2 j4, + 1 of each block
+      bool raise = false;
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        int a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0}, c[4] = {0, 0, 0, 0};
+      for (int u = 0; u < 2; ++u) {
+        const float ks = (u ? scales.z : scales.x) * p.scale, vs = fmaxf(u ? scales.w : scales.y, KD_LEAST_SCALE);
+        const float lvs = kd_lg2(vs);
+        inv_vs[u] = kd_rcp(vs);
+        // q . k: bytes times bytes, exact
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          uint32_t k[4];
-          kd_ldsm(k, st + hb * 1024 + (cc ? k_at ^ 64 : k_at));
+        for (int hb = 0; hb < 2; ++hb) {
+          int d[PRODUCTS][4];
 #pragma unroll
-          for (int d = 0; d < 4; d += 2) {
-            const int ch = 4 * cc + d;
+          for (int cc = 0; cc < 2; ++cc) {
+            uint32_t k[4];
+            kd_ldsm(k, st + u * KD_STAGE_BYTES + hb * 1024 + (cc ? k_at ^ 64 : k_at));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < PRODUCTS; ++e) {
+                if (cc == 0 && h == 0) kd_imma(d[e], qa[0][e], k[0], k[1], nothing);
+                else kd_imma(d[e], qa[2 * cc + h][e], k[2 * h], k[2 * h + 1], d[e]);
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
             if constexpr (ROWS == 8) {
-              kd_imma(a, qa[0][0][ch], qa[0][1][ch], qa[0][0][ch + 1], qa[0][1][ch + 1], k[d], k[d + 1]);
-              kd_imma(b, qa[0][2][ch], 0u, qa[0][2][ch + 1], 0u, k[d], k[d + 1]);
+              x[u][0][2 * hb + e] = fmaf(kd_sum(d[0][e]), 65536.f, fmaf(kd_sum(d[0][2 + e]), 256.f, kd_sum(d[1][e])));
             } else {
-              kd_imma(a, qa[0][0][ch], qa[NR - 1][0][ch], qa[0][0][ch + 1], qa[NR - 1][0][ch + 1], k[d], k[d + 1]);
-              kd_imma(b, qa[0][1][ch], qa[NR - 1][1][ch], qa[0][1][ch + 1], qa[NR - 1][1][ch + 1], k[d], k[d + 1]);
-              kd_imma(c, qa[0][2][ch], qa[NR - 1][2][ch], qa[0][2][ch + 1], qa[NR - 1][2][ch + 1], k[d], k[d + 1]);
+#pragma unroll
+              for (int n = 0; n < NR; ++n)
+                x[u][n][2 * hb + e] = fmaf(kd_sum(d[0][2 * n + e]), 65536.f, fmaf(kd_sum(d[1][2 * n + e]), 256.f, kd_sum(d[PRODUCTS - 1][2 * n + e])));
             }
           }
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if constexpr (ROWS == 8) {
-            x[0][2 * hb + e] = fmaf((float)a[e], 65536.f, fmaf((float)a[2 + e], 256.f, (float)b[e]));
-          } else {
+        for (int n = 0; n < NR; ++n) {
+          const float f = ks * back[n];
 #pragma unroll
-            for (int n = 0; n < NR; ++n) x[n][2 * hb + e] = fmaf((float)a[2 * n + e], 65536.f, fmaf((float)b[2 * n + e], 256.f, (float)c[2 * n + e]));
-          }
+          for (int e = 0; e < 4; ++e) x[u][n][e] = fmaf(x[u][n][e], f, lvs);
         }
       }
-      // exponents of p vs
-      bool raise = false;
+      if (key0 + 32 > full) {  // the same for the whole warp
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + 16 * u + 8 * (e >> 1) + 2 * j4 + (e & 1) >= limit[n]) x[u][n][e] = -CUDART_INF_F;
+      }
       float top[NR];
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const float f = ks * back[n];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] = fmaf(x[n][e], f, lvs);
-      }
-      if (key0 + 16 > full) {  // the same for the whole warp
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key0 + 8 * (e >> 1) + 2 * j4 + (e & 1) >= limit[n]) x[n][e] = -CUDART_INF_F;
-      }
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        top[n] = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
+        top[n] = fmaxf(fmaxf(fmaxf(x[0][n][0], x[0][n][1]), fmaxf(x[0][n][2], x[0][n][3])), fmaxf(fmaxf(x[1][n][0], x[1][n][1]), fmaxf(x[1][n][2], x[1][n][3])));
         raise = raise || top[n] > m[n] + KD_RAISE;
       }
       if (__any_sync(0xffffffffu, raise)) {
@@ -375,52 +432,54 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
           }
         }
       }
-      uint32_t ph[NR][2], pl[NR][2];
+      // A operands of P: [half][..] for 16 rows; both halves in one for 8
+      uint32_t pa[2][NR][4];
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         const float shift = m[n] == -CUDART_INF_F ? 0.f : m[n] - KD_P_EXP;
-        float sum = 0.f;
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {
-          const float a = kd_ex2(x[n][2 * hb] - shift), b = kd_ex2(x[n][2 * hb + 1] - shift);
-          sum += a + b;
-          const __half2 hi = __floats2half2_rn(a, b);
-          const float2 hf = __half22float2(hi);
-          ph[n][hb] = h22u(hi);
-          pl[n][hb] = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
+        for (int u = 0; u < 2; ++u) {
+          float sum = 0.f;
+#pragma unroll
+          for (int hb = 0; hb < 2; ++hb) {
+            const float a = kd_ex2(x[u][n][2 * hb] - shift), b = kd_ex2(x[u][n][2 * hb + 1] - shift);
+            sum += a + b;
+            const __half2 hi = __floats2half2_rn(a, b);
+            const float2 hf = __half22float2(hi);
+            const uint32_t lo = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
+            if constexpr (ROWS == 8) pa[u][0][2 * hb] = h22u(hi), pa[u][0][2 * hb + 1] = lo;
+            else pa[u][0][2 * hb + n] = h22u(hi), pa[u][NR - 1][2 * hb + n] = lo;
+          }
+          l[n] = fmaf(sum, inv_vs[u], l[n]);
         }
-        l[n] = fmaf(sum, inv_vs, l[n]);
       }
-      if (!zero) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
           uint32_t v[4];
           // keys 0-7 and 8-15 of piece c, then of piece c + 1; transposed: two keys, two dims a word
-          kd_ldsm_t(v, st + v_row + (((c + v_chunk) ^ v_sw) << 4));
+          kd_ldsm_t(v, st + u * KD_STAGE_BYTES + v_row + (((c + v_chunk) ^ v_sw) << 4));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t u0 = v[2 * h] ^ 0x80808080u, u1 = v[2 * h + 1] ^ 0x80808080u;
             const uint32_t e0 = kd_half2<0x4240>(u0), e1 = kd_half2<0x4240>(u1), d0 = kd_half2<0x4341>(u0), d1 = kd_half2<0x4341>(u1);
-            float(&even)[4] = o[2 * (c + h)];
-            float(&odd)[4] = o[2 * (c + h) + 1];
-            if constexpr (ROWS == 8) {
-              kd_mma(even, ph[0][0], pl[0][0], ph[0][1], pl[0][1], e0, e1);
-              kd_mma(odd, ph[0][0], pl[0][0], ph[0][1], pl[0][1], d0, d1);
-            } else {
-              kd_mma(even, ph[0][0], ph[NR - 1][0], ph[0][1], ph[NR - 1][1], e0, e1);
-              kd_mma(odd, ph[0][0], ph[NR - 1][0], ph[0][1], ph[NR - 1][1], d0, d1);
-              kd_mma(even, pl[0][0], pl[NR - 1][0], pl[0][1], pl[NR - 1][1], e0, e1);
-              kd_mma(odd, pl[0][0], pl[NR - 1][0], pl[0][1], pl[NR - 1][1], d0, d1);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              kd_mma(o[2 * (c + h)], pa[u][n][0], pa[u][n][1], pa[u][n][2], pa[u][n][3], e0, e1);
+              kd_mma(o[2 * (c + h) + 1], pa[u][n][0], pa[u][n][1], pa[u][n][2], pa[u][n][3], d0, d1);
             }
           }
         }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-
-    // ---- the four warps' parts to shared memory (the ring is idle), then joined
-    __syncthreads();
-    float *part = reinterpret_cast<float *>(smem);  // [warp][ROWS][128]
+    // ---- the next part's first blocks are on their way while the four warps' parts of this one are joined in the ring's
+    // other half
+    const Part done = it;
+    const int empty = (int)max(0l, min((long)ROWS, -it.pos0 * p.group - it.first));  // leading rows with nothing to attend to
+    more = next(it);
+    __syncwarp();
+    if (more) begin();
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
@@ -433,82 +492,107 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
           v = make_float4(o[2 * c][0] + o[2 * c][2], o[2 * c + 1][0] + o[2 * c + 1][2], o[2 * c][1] + o[2 * c][3], o[2 * c + 1][1] + o[2 * c + 1][3]);
         else
           v = make_float4(o[2 * c][2 * n], o[2 * c + 1][2 * n], o[2 * c][2 * n + 1], o[2 * c + 1][2 * n + 1]);
-        *reinterpret_cast<float4 *>(part + ((warp * ROWS + 8 * n + g) * KV8_D + 16 * c + 4 * j4)) = v;
+        *reinterpret_cast<float4 *>(ring_mine + 2 * KD_STAGE_BYTES + ((8 * n + g) * KV8_D + 16 * c + 4 * j4) * 4) = v;
       }
     }
     __syncthreads();
-    const bool whole = b0 == 0 && b1 == blocks;
-    const int empty = (int)max(0l, min((long)ROWS, -pos0 * p.group - first));  // leading rows with nothing to attend to
-    const int slot = b0 == 0 ? 1 : 0;
-    float *mine_o = p.partial + ((size_t)blockIdx.x * 2 + slot) * ROWS * KV8_D;
-    float *mine_ml = p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D + ((size_t)blockIdx.x * 2 + slot) * ROWS * 2;
-    for (int row = 0; row <= last - first; ++row) {
-      float mx = -CUDART_INF_F, sum = 0.f, acc = 0.f;
+    const bool whole = done.b0 == 0 && done.b1 == done.blocks;
+    const int slot = done.b0 == 0 ? 1 : 0;
+    constexpr int PER_ROW = KD_THREADS / ROWS, PIECES = KV8_D / 4 / PER_ROW;  // threads of a row, four dims at a time
+    const int row = tid / PER_ROW, col = tid % PER_ROW * 4;
+    if (row <= done.last - done.first) {
+      float mx = -CUDART_INF_F, sum = 0.f, f[KD_WARPS];
 #pragma unroll
       for (int i = 0; i < KD_WARPS; ++i) mx = fmaxf(mx, m_s[i][row]);
 #pragma unroll
       for (int i = 0; i < KD_WARPS; ++i) {
-        const float f = m_s[i][row] == -CUDART_INF_F ? 0.f : kd_ex2(m_s[i][row] - mx);
-        sum = fmaf(l_s[i][row], f, sum);
-        acc = fmaf(part[(i * ROWS + row) * KV8_D + tid], f, acc);
+        f[i] = m_s[i][row] == -CUDART_INF_F ? 0.f : kd_ex2(m_s[i][row] - mx);
+        sum = fmaf(l_s[i][row], f[i], sum);
       }
-      if (whole) {
-        const int packed = first + row, token = packed / p.group, head = hk * p.group + packed - token * p.group;
-        ((T *)p.out)[((size_t)(row0 + token) * p.Hq + head) * KV8_D + tid] = (T)(row < empty ? 0.f : acc / sum);
-      } else {
-        mine_o[row * KV8_D + tid] = acc;
-        if (tid == 0) mine_ml[2 * row] = mx, mine_ml[2 * row + 1] = sum;
+      const int packed = done.first + row, token = packed / p.group, head = done.hk * p.group + packed - token * p.group;
+      T *out = (T *)p.out + ((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + col;
+      float *part = p.partial + (((size_t)blockIdx.x * 2 + slot) * ROWS + row) * KV8_D + col;
+      const float over = row < empty ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < KD_WARPS; ++i) {
+          const float4 v = *reinterpret_cast<const float4 *>(smem + i * (KD_STAGES * KD_STAGE_BYTES) + 2 * KD_STAGE_BYTES + (row * KV8_D + col + c * PER_ROW * 4) * 4);
+          acc.x = fmaf(v.x, f[i], acc.x), acc.y = fmaf(v.y, f[i], acc.y), acc.z = fmaf(v.z, f[i], acc.z), acc.w = fmaf(v.w, f[i], acc.w);
+        }
+        if (whole) kd_store4(out + c * PER_ROW * 4, acc, over);
+        else *reinterpret_cast<float4 *>(part + c * PER_ROW * 4) = acc;
       }
+      if (!whole && col == 0)
+        reinterpret_cast<float2 *>(p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D)[((size_t)blockIdx.x * 2 + slot) * ROWS + row] = make_float2(mx, sum);
     }
     if (!whole && slot == 1 && tid == 0)  // begun here: the CTAs up to the one with the item's last block have the rest
-      p.split[blockIdx.x] = make_int4((int)((item + KD_ITEM + blocks - 1) / per) - (int)blockIdx.x + 1, row0, hk | (last - first) << 16 | empty << 20, first);
-    __syncthreads();
+      p.split[blockIdx.x] = make_int4((int)kd_div(done.item + KD_ITEM + done.blocks - 1, per) - (int)blockIdx.x + 1, done.row0,
+                                      done.hk | (done.last - done.first) << 16 | empty << 20, done.first);
   }
 }
 
-// Joins the parts of the items that several CTAs share.  A CTA per CTA of the first kernel and four rows; two warps a row,
-// each every second part.
-constexpr int KJ_ROWS = 4, KJ_THREADS = KJ_ROWS * 64;
+// Joins the parts of the items that several CTAs share.  A CTA has one row of the items begun in eight CTAs of the first
+// kernel, a warp each; an item in more than eight parts is all warps' work, part by part.
+constexpr int KJ_WARPS = 8, KJ_THREADS = KJ_WARPS * 32;
+struct Joined {
+  float m, l;
+  float4 acc;
+  __device__ __forceinline__ Joined() { m = -CUDART_INF_F, l = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void add(float2 ml, float4 v) {
+    const float up = fmaxf(m, ml.x), f = m == -CUDART_INF_F ? 0.f : kd_ex2(m - up), fc = ml.x == -CUDART_INF_F ? 0.f : kd_ex2(ml.x - up);
+    l = l * f + ml.y * fc;
+    acc.x = acc.x * f + v.x * fc, acc.y = acc.y * f + v.y * fc, acc.z = acc.z * f + v.z * fc, acc.w = acc.w * f + v.w * fc;
+    m = up;
+  }
+};
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_constant__ DecodeParams p) {
-  __shared__ float4 acc_s[KJ_ROWS][32];
-  __shared__ float m_s[KJ_ROWS], l_s[KJ_ROWS];
+__global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_constant__ DecodeParams p, int ctas) {
+  __shared__ float4 acc_s[KJ_WARPS][32];
+  __shared__ float2 ml_s[KJ_WARPS];
   pdl_launch_dependents();
   pdl_wait();
-  const int4 split = p.split[blockIdx.x];
-  const int lane = threadIdx.x & 31, sub = (threadIdx.x >> 5) & 1, i = threadIdx.x >> 6, row = blockIdx.y * KJ_ROWS + i;
-  const int n = split.x, first = split.w, more = split.z >> 16 & 15, empty = split.z >> 20, hk = split.z & 0xFFFF;
-  if (n == 0) return;
-  const bool in = row <= more;
-  float m = -CUDART_INF_F, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (in) {
-    const float *ml = p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D;
-#pragma unroll 4
-    for (int c = sub; c < n; c += 2) {
-      const size_t at = ((size_t)(blockIdx.x + c) * 2 + (c == 0 ? 1 : 0)) * ROWS + row;
-      const float mc = ml[2 * at], lc = ml[2 * at + 1];
-      const float4 v = *reinterpret_cast<const float4 *>(p.partial + at * KV8_D + 4 * lane);
-      const float up = fmaxf(m, mc), f = m == -CUDART_INF_F ? 0.f : kd_ex2(m - up), fc = mc == -CUDART_INF_F ? 0.f : kd_ex2(mc - up);
-      l = l * f + lc * fc;
-      acc.x = acc.x * f + v.x * fc, acc.y = acc.y * f + v.y * fc, acc.z = acc.z * f + v.z * fc, acc.w = acc.w * f + v.w * fc;
-      m = up;
-    }
-    if (sub == 1) {
-      acc_s[i][lane] = acc;
-      if (lane == 0) m_s[i] = m, l_s[i] = l;
-    }
-  }
-  __syncthreads();
-  if (!in || sub == 1) return;
-  const float mc = m_s[i], lc = l_s[i], up = fmaxf(m, mc), f = m == -CUDART_INF_F ? 0.f : kd_ex2(m - up), fc = mc == -CUDART_INF_F ? 0.f : kd_ex2(mc - up);
-  const float4 v = acc_s[i][lane];
-  const float sum = l * f + lc * fc;
-  const int packed = first + row, token = packed / p.group, head = hk * p.group + packed - token * p.group;
-  T *out = (T *)p.out + ((size_t)(split.y + token) * p.Hq + head) * KV8_D + 4 * lane;
-  const float x[4] = {(acc.x * f + v.x * fc) / sum, (acc.y * f + v.y * fc) / sum, (acc.z * f + v.z * fc) / sum, (acc.w * f + v.w * fc) / sum};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y, c0 = blockIdx.x * KJ_WARPS;
+  const int4 my = lane < KJ_WARPS && c0 + lane < ctas ? p.split[c0 + lane] : make_int4(0, 0, 0, 0);
+  const float2 *const ml = reinterpret_cast<const float2 *>(p.partial + (size_t)ctas * 2 * ROWS * KV8_D) + row;
+  const float4 *const acc = reinterpret_cast<const float4 *>(p.partial + row * KV8_D) + lane;
+  auto part = [&](int c, int i) { return ((size_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * ROWS; };
+  auto store = [&](int4 sp, const Joined &a) {
+    const int packed = sp.w + row, token = packed / p.group, head = (sp.z & 0xFFFF) * p.group + packed - token * p.group;
+    T *out = (T *)p.out + ((size_t)(sp.y + token) * p.Hq + head) * KV8_D + 4 * lane;
+    const bool none = row < sp.z >> 20;
+    kd_store4(out, a.acc, none ? 0.f : 1.f / a.l);
+  };
+  for (int k = 0; k < KJ_WARPS; ++k) {
+    const int4 sp = make_int4(__shfl_sync(0xffffffffu, my.x, k), __shfl_sync(0xffffffffu, my.y, k), __shfl_sync(0xffffffffu, my.z, k), __shfl_sync(0xffffffffu, my.w, k));
+    if (sp.x == 0 || row > (sp.z >> 16 & 15) || (sp.x <= KJ_WARPS && k != warp)) continue;
+    const int step = sp.x <= KJ_WARPS ? 1 : KJ_WARPS;
+    Joined a;
+    for (int i0 = step == 1 ? 0 : warp; i0 < sp.x; i0 += 8 * step) {
+      float2 s[8];
+      float4 v[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(row < empty ? 0.f : x[e]);
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j * step;
+        s[j] = i < sp.x ? ml[part(c0 + k, i)] : make_float2(-CUDART_INF_F, 0.f);
+        v[j] = i < sp.x ? acc[part(c0 + k, i) * (KV8_D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a.add(s[j], v[j]);
+    }
+    if (step > 1) {  // every warp is here
+      __syncthreads();
+      acc_s[warp][lane] = a.acc;
+      if (lane == 0) ml_s[warp] = make_float2(a.m, a.l);
+      __syncthreads();
+      if (k != warp) continue;
+      a = Joined();
+#pragma unroll
+      for (int j = 0; j < KJ_WARPS; ++j) a.add(ml_s[j], acc_s[j][lane]);
+    }
+    store(sp, a);
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
@@ -532,7 +616,7 @@ static int decode_launch(const DecodeParams &p, const DecodePlan &d, cudaStream_
   static_assert(smem >= KD_WARPS * ROWS * KV8_D * (int)sizeof(float), "the warps' parts fit into the ring");
   AB200_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<T, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   AB200_CUDA(launch_pdl(kv8_decode_kernel<T, ROWS>, dim3(d.ctas), dim3(KD_THREADS), smem, stream, p));
-  AB200_CUDA(launch_pdl(kv8_join_kernel<T, ROWS>, dim3(d.ctas, ROWS / KJ_ROWS), dim3(KJ_THREADS), 0, stream, p));
+  AB200_CUDA(launch_pdl(kv8_join_kernel<T, ROWS>, dim3((d.ctas + KJ_WARPS - 1) / KJ_WARPS, ROWS), dim3(KJ_THREADS), 0, stream, p, d.ctas));
   return AB200_OK;
 }
 
