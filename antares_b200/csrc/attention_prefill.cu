@@ -9,7 +9,7 @@
 // P is stored as an fp16 pair hi + lo, 22 bits of an fp32 probability's 24, and both halves are multiplied with V into
 // the same fp32 accumulator, so only q, K, V and the result are 16 bits wide.  P is scaled by 2^6 (the row sum with it),
 // which keeps lo out of the subnormals where it matters.  The running maximum is only raised when a tile exceeds it by
-// more than 2^8, as FlashAttention-4 does it (then O is rescaled in tensor memory): what the row is finally divided by
+// more than 2^8 (then O is rescaled in tensor memory): what the row is finally divided by
 // contains the same factor.  Error of the fp16 result against 64 bits, 2000 rows: 1.95138e-4, the fp32 single-query
 // kernel 1.95134e-4, the exact result rounded to fp16 1.95134e-4; the difference, 1e-6 of the result, is the tensor
 // cores' accumulation (it grows with the number of MMAs a row has gone through).  The pair's own share is 5e-8 of the
@@ -33,7 +33,7 @@
 
 #include <type_traits>
 
-#include "common.cuh"
+#include "attention_mma.cuh"
 
 namespace ab200 {
 
@@ -47,7 +47,6 @@ constexpr int AP_STAGES = 4;                      // two of K, two of V
 constexpr int AP_SMEM = AP_Q_BYTES + AP_STAGES * AP_STAGE_BYTES + 1024;
 constexpr int AP_TMEM_COLS = 256;                 // S0 | S1 (64 each, P overlays S), O (128)
 constexpr int AP_ROWB = AP_D * 2 + 16;            // bytes per parked output row
-constexpr unsigned AP_WAIT_POLLS = 1u << 22;
 constexpr float AP_P_EXP = 6.f;                   // P is scaled by 2^6
 constexpr float AP_RAISE = 8.f;                   // raise the running maximum when a tile exceeds it by 2^8
 
@@ -62,68 +61,6 @@ struct AttnPrefillParams {
   KvPages pages;
   int *status;
 };
-
-__device__ __forceinline__ uint32_t ap_smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// 128-byte-swizzled operand (rows of 128 B, atoms of 8 rows = 1024 B, stride between atoms 1024 B).  lead: bytes
-// between blocks of 64 elements along MN for an MN-major operand (unused, 1 unit, for a K-major one).
-__device__ __forceinline__ uint64_t ap_desc(uint32_t addr, uint32_t lead_bytes) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((lead_bytes >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
-__device__ __forceinline__ bool ap_wait(uint32_t bar, unsigned parity) {
-  for (unsigned i = 0; i < AP_WAIT_POLLS; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
-}
-__device__ __forceinline__ void ap_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// The whole warp runs the issuing loop and only these instructions are one thread's: in a divergent branch every
-// descriptor would have to be moved into uniform registers on its own.
-__device__ __forceinline__ void ap_commit(uint32_t bar) {
-  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar) : "memory");
-}
-// D (+)= A.B, A in shared memory (ss) or tensor memory (ts)
-__device__ __forceinline__ void ap_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
-      "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void ap_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
-      "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-#define AP_R16(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), \
-    "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), "=r"(r[o + 15])
-#define AP_I16(r) "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), \
-    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-// 32 columns of this warp's 32 lanes; the caller waits
-__device__ __forceinline__ void ap_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : AP_R16(r, 0), AP_R16(r, 16)
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void ap_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::AP_I16(r), "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void ap_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void ap_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ap_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Four consecutive query rows by one warp in fp32, two passes over exactly the keys each attends to (lane = 4 dims).
 // Four keys at a time: their rows are loaded once for the four queries, and the 16 dot products are summed over the warp
@@ -428,10 +365,7 @@ __global__ void __launch_bounds__(AP_THREADS, 2) attention_prefill_kernel(AttnPr
 #pragma unroll 1
         for (int d = 0; d < AP_D; d += 16) {
           uint32_t o[16];
-          asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                       : AP_R16(o, 0)
-                       : "r"(tmem_o + lanes + d)
-                       : "memory");
+          ap_ld16(tmem_o + lanes + d, o);
           ap_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);

@@ -13,6 +13,7 @@
 #include <math_constants.h>
 
 #include "kv8.cuh"
+#include "kv8_prefill.cuh"
 
 namespace ab200 {
 
@@ -620,14 +621,24 @@ static int decode_launch(const DecodeParams &p, const DecodePlan &d, cudaStream_
   return AB200_OK;
 }
 
+// Sequences of up to KD_FEW packed rows go through the kernel above, longer ones through the prompt kernel.
+constexpr int KD_FEW = 64;
 static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, int D, float scale, int dtype,
                   const float *inv_freq, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (r.T == 0 || r.S == 0) return AB200_OK;
   const DecodePlan d = decode_plan(r.S, r.T, max_rows, Hq, c.H);
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= d.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, d.bytes, workspace_bytes);
-  DecodeParams p{c, r, q, q_stride, out, Hq, Hq / c.H, scale * 1.4426950408889634f, inv_freq, 0x7fffffff, (float *)workspace,
-                 (int4 *)((char *)workspace + d.partial_bytes), kernel_error_ptr()};
-  AB200_REQUIRE(p.status != nullptr, "%s: cannot resolve the status word", who);
+  const int group = Hq / c.H;
+  int *status = kernel_error_ptr();
+  AB200_REQUIRE(status != nullptr, "%s: cannot resolve the status word", who);
+  const float scale2 = scale * 1.4426950408889634f;
+  const long most = r.cu ? max_rows : r.n;
+  const bool prompts = most * group > KD_FEW && inv_freq == nullptr;
+  if (prompts) {
+    const int rc = kv8_prefill(Kv8PrefillParams{c, r, q, q_stride, out, Hq, group, scale2, KD_FEW, nullptr, nullptr, status, 0, 0, 1}, dtype, stream);
+    if (rc || !r.cu) return rc;
+  }
+  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, prompts ? KD_FEW : 0x7fffffff, (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
   if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8>(p, d, stream) : decode_launch<float, 16>(p, d, stream);
   return d.rows == 8 ? decode_launch<__half, 8>(p, d, stream) : decode_launch<__half, 16>(p, d, stream);
 }

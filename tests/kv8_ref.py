@@ -106,14 +106,15 @@ def attention(c, q, pos0, cu=None, scale=None, inv_freq=None):
             tiny[row0 + r] = (L * 2.0 ** -31 * 127 * torch.einsum("hgl,lh->hgl", p, steps).amax(-1)).reshape(Hq, 1).numpy()
             mag = torch.einsum("hgd,lhd->hgl", x[r].abs(), k[:L].abs()).amax(-1)
             tall = torch.einsum("hg,lh->hgl", x[r].abs().amax(-1), k[:L].abs().sum(-1)).amax(-1)
-            score[row0 + r] = (scale * (2.0 ** -19 * mag + 2.0 ** -21 * tall)).reshape(Hq, 1).numpy()
+            score[row0 + r] = (abs(scale) * (2.0 ** -19 * mag + 2.0 ** -21 * tall)).reshape(Hq, 1).numpy()
     return out, spread, score, tiny
 
 
-def bound(want, spread, score, tiny, keys, dtype):
+def bound(want, spread, score, tiny, keys, dtype, p_single=False):
     """How far a result may be off `want`.  Half a step of its type.  A score is a sum of 128 exact products in eight steps
     of sixteen, each cut to 24 bits: 2^-19 of its magnitude holds twice that, and 2^-21 of the largest |q| times sum |k| a
     query kept as two 11-bit halves; e^error moves every p by twice the largest one's error.  p as two halves and its
-    exponential: 2^-20, and `tiny` where the pair runs out of exponents.  The sums over the keys, sixteen at a time: 2^-23 a step of sum p |v|."""
+    exponential: 2^-20, and `tiny` where the pair runs out of exponents.  p_single: p as one fp16 number, half a step of which is
+    2^-11 of it (prompts with fp16 queries).  The sums over the keys, sixteen at a time: 2^-23 a step of sum p |v|."""
     half = torch.finfo(dtype).eps / 2
-    return np.abs(want) * half * 1.01 + spread * (2 * score + 2.0 ** -20 + (keys / 16 + 8) * 2.0 ** -23) + tiny + (2.0 ** -25 if dtype == torch.float16 else 1e-30)
+    return np.abs(want) * half * 1.01 + spread * (2 * score + 2.0 ** -20 + (2.0 ** -11 if p_single else 0) + (keys / 16 + 8) * 2.0 ** -23) + tiny + (2.0 ** -25 if dtype == torch.float16 else 1e-30)
