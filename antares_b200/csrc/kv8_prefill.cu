@@ -8,17 +8,18 @@
 
 namespace ab200 {
 
-constexpr int KP_BM = 128, KP_BN = 128, KP_LOAD_WARPS = 4, KP_RING = 4;
+constexpr int KP_BM = 128, KP_BN = 128, KP_LOAD_WARPS = 4, KP_RING = 3, KP_RAW = 4;
 constexpr int KP_HALF_BYTES = KP_BN * 128;          // 64 dims of 128 rows, fp16, 128-byte swizzle
 constexpr int KP_STAGE_BYTES = 2 * KP_HALF_BYTES;   // a tile of K or of V
+constexpr int KP_RAW_BYTES = KP_BN * KV8_D;         // its codes
 constexpr int KP_BLOCKS = KP_BN / KV8_BLOCK;
 constexpr float KP_RAISE = 8.f, KP_P_EXP = 6.f, KP_LEAST_SCALE = 0x1p-100f;
 
 template <int TILES, int PARTS>
 struct KpShape {
   static constexpr int Q_BYTES = PARTS * KP_STAGE_BYTES;                                    // of one tile of rows
-  static constexpr int SMEM = TILES * Q_BYTES + KP_RING * KP_STAGE_BYTES + 1024;
-  static constexpr int SOFT_WARPS = 4 * TILES, LOAD_WARP = SOFT_WARPS, MMA_WARP = SOFT_WARPS + KP_LOAD_WARPS, THREADS = (MMA_WARP + 1) * 32;
+  static constexpr int SMEM = TILES * Q_BYTES + KP_RING * KP_STAGE_BYTES + KP_RAW * KP_RAW_BYTES + 1024;
+  static constexpr int SOFT_WARPS = 4 * TILES, LOAD_WARP = SOFT_WARPS, MMA_WARP = SOFT_WARPS + KP_LOAD_WARPS, THREADS = (MMA_WARP + TILES) * 32;
   static constexpr int TMEM_COLS = 256 * TILES;                                             // a tile: S (P over it), O
 };
 
@@ -53,6 +54,13 @@ __device__ __forceinline__ bool kp_wait(uint32_t bar, unsigned parity, const vol
   }
   return false;
 }
+// Nothing uses the loaded registers before this.
+__device__ __forceinline__ void kp_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
 template <int SEL>
 __device__ __forceinline__ uint32_t kp_half2(uint32_t flipped) {  // two codes (flipped to 0 .. 255) as fp16
   return h22u(__hsub2(u2h2(__byte_perm(flipped, 0x64646464u, SEL)), u2h2(0x64806480u)));
@@ -64,11 +72,11 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   using Z = KpShape<TILES, PARTS>;
   extern __shared__ unsigned char kp_smem_raw[];
   unsigned char *smem = kp_smem_raw + ((1024u - (ap_smem_u32(kp_smem_raw) & 1023u)) & 1023u);  // swizzle atoms need 1024-byte alignment
-  // barriers: full[4], empty[4], then for each tile: scores ready, P ready, O done; the end of all products
-  __shared__ __align__(8) uint64_t bars[2 * KP_RING + 3 * TILES + 1];
+  // barriers: full[], empty[], then for each tile: scores ready, P ready, O done, the end of all its products
+  __shared__ __align__(8) uint64_t bars[2 * KP_RING + 4 * TILES];
   __shared__ uint32_t tmem_s;
   __shared__ int fail_s, seq_s;
-  __shared__ float scales_s[4 * TILES][3][KP_BLOCKS];  // a softmax warp's own: factor of the scores, log2(vs), 1 / vs
+  __shared__ float4 scales_s[4 * TILES][KP_BLOCKS];  // a softmax warp's own: factor of the scores, log2(vs), 1 / vs
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Kv8Rows &r = p.r;
   pdl_wait();
@@ -106,18 +114,18 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   for (int t = 0; t < TILES; ++t) n_of[t] = max(0, min(n_of[t], j1) - j0);
   const int n = j1 - j0;
 
-  const uint32_t b_full = ap_smem_u32(bars), b_empty = b_full + 8 * KP_RING, b_tile = b_empty + 8 * KP_RING, b_end = b_tile + 24 * TILES;
+  const uint32_t b_full = ap_smem_u32(bars), b_empty = b_full + 8 * KP_RING, b_tile = b_empty + 8 * KP_RING;
   if (tid == 0) {
     for (int i = 0; i < KP_RING; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b_full + 8 * i), "n"(KP_LOAD_WARPS * 32));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_empty + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b_empty + 8 * i), "n"(TILES));
     }
     for (int t = 0; t < TILES; ++t) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 24 * t));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(b_tile + 24 * t + 8));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 24 * t + 16));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 32 * t));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(b_tile + 32 * t + 8));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 32 * t + 16));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 32 * t + 24));
     }
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_end));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == Z::MMA_WARP) {
@@ -134,8 +142,8 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   const int32_t *const table = r.table + (size_t)seq * r.table_stride;
 
   if (warp >= Z::LOAD_WARP && warp < Z::MMA_WARP) {
-    // ---- K and V tiles in turn through one ring: unit 2 j is K of tile j, 2 j + 1 its V.  The codes of the next unit are on
-    // their way while this one's become fp16.  A quarter of a warp stores four even pieces of two neighbouring rows: no
+    // ---- K and V tiles in turn through one ring: unit 2 j is K of tile j, 2 j + 1 its V.  The codes of the next three units
+    // are on their way while this one's become fp16.  A quarter of a warp stores four even pieces of two neighbouring rows: no
     // two in one bank.
     const int lw = warp - Z::LOAD_WARP, row = ((lane >> 2) & 1) + ((lane >> 4) << 1) + 4 * lw, piece = (lane & 3) | (lane >> 3 & 1) << 2;
     const uint32_t sw = row & 7;
@@ -157,28 +165,32 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       }
       ask(j + 1);
     };
-    uint4 now[KP_BLOCKS], next[KP_BLOCKS];
-    auto load = [&](int u, uint4(&v)[KP_BLOCKS]) {
-      const int8_t *src = (u & 1 ? p.c.v : p.c.k) + row * KV8_D + piece * 16;
+    // a thread's own 16 bytes of each block of a unit: it reads back what it asked for itself
+    const uint32_t raw = ap_smem_u32(smem) + TILES * Z::Q_BYTES + KP_RING * KP_STAGE_BYTES + (tid - Z::LOAD_WARP * 32) * 16;
+    auto load = [&](int u) {
+      if (u < 2 * n) {
+        if ((u & 1) == 0) lookup(u >> 1);
+        const int8_t *src = (u & 1 ? p.c.v : p.c.k) + row * KV8_D + piece * 16;
 #pragma unroll
-      for (int i = 0; i < KP_BLOCKS; ++i) {
-        const int blk = __shfl_sync(0xffffffffu, where, i);
-        v[i] = blk < 0 ? make_uint4(0, 0, 0, 0) : ldg_stream_v4(src + (size_t)blk * (KV8_BLOCK * KV8_D));
+        for (int i = 0; i < KP_BLOCKS; ++i) {
+          const int blk = __shfl_sync(0xffffffffu, where, i);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + u % KP_RAW * KP_RAW_BYTES + i * 2048), "l"(src + (size_t)max(blk, 0) * (KV8_BLOCK * KV8_D)), "r"(blk < 0 ? 0 : 16)
+                       : "memory");
+        }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
     bool good = true;
-    if (n > 0) {
-      ask(0);
-      lookup(0);
-      load(0, next);
-    }
-    for (int u = 0; u < 2 * n; ++u) {
+    if (n > 0) ask(0);
 #pragma unroll
-      for (int i = 0; i < KP_BLOCKS; ++i) now[i] = next[i];
-      if (u + 1 < 2 * n) {
-        if (u & 1) lookup((u + 1) >> 1);
-        load(u + 1, next);
-      }
+    for (int u = 0; u < KP_RAW - 1; ++u) load(u);
+    for (int u = 0; u < 2 * n; ++u) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(KP_RAW - 2) : "memory");
+      uint4 now[KP_BLOCKS];
+#pragma unroll
+      for (int i = 0; i < KP_BLOCKS; ++i)
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(now[i].x), "=r"(now[i].y), "=r"(now[i].z), "=r"(now[i].w) : "r"(raw + u % KP_RAW * KP_RAW_BYTES + i * 2048) : "memory");
+      load(u + KP_RAW - 1);
       const int st = u % KP_RING;
       if (u >= KP_RING && !__all_sync(0xffffffffu, kp_wait(b_empty + 8 * st, (u / KP_RING - 1) & 1, &fail_s))) {
         good = false;
@@ -194,15 +206,18 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       ap_arrive(b_full + 8 * st);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!good) fail_s = 1;
-  } else if (warp == Z::MMA_WARP) {
-    // ---- MMA issue.  Scores of a tile of rows go where its P lay, so they wait for that P's product; meanwhile the other
-    // tile's are under way.
+  } else if (warp >= Z::MMA_WARP) {
+    // ---- MMA issue, a warp for each tile of rows.  Its scores go where its P lay, so they wait for that P's product;
+    // meanwhile the other tile's are under way.
+    const int t = warp - Z::MMA_WARP, my_n = n_of[t];
+    const uint32_t bar = b_tile + 32 * t;
     constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_BN >> 3) << 17) | ((uint32_t)(KP_BM >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(KV8_D >> 3) << 17) | ((uint32_t)(KP_BM >> 4) << 24);  // bit 16: B is MN-major
     bool good = true;
-    auto wait = [&](uint32_t bar, unsigned parity) { return __all_sync(0xffffffffu, kp_wait(bar, parity, &fail_s)); };
-    auto scores = [&](int t, int j) {
+    auto wait = [&](uint32_t b, unsigned parity) { good = good && __all_sync(0xffffffffu, kp_wait(b, parity, &fail_s)); };
+    auto scores = [&](int j) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint64_t b0 = ap_desc(ring + (2 * j % KP_RING) * KP_STAGE_BYTES, 16);
 #pragma unroll
@@ -214,9 +229,9 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
           ap_mma_ss(tmem + 256 * t, a0 + step, b0 + step, ID_S, k > 0 || part > 0);
         }
       }
-      ap_commit(b_tile + 24 * t);
+      ap_commit(bar);
     };
-    auto values = [&](int t, int j) {
+    auto values = [&](int j) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint64_t b0 = ap_desc(ring + ((2 * j + 1) % KP_RING) * KP_STAGE_BYTES, KP_HALF_BYTES);
       const uint32_t a0 = tmem + 256 * t, d = a0 + 128;
@@ -225,44 +240,41 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
           ap_mma_ts(d, a0 + (PARTS == 1 ? 8 * k : 32 * (k >> 1) + 16 * part + 8 * (k & 1)), b0 + (uint64_t)(k * (2048 / 16)), ID_O, j > 0 || k > 0 || part > 0);
-      ap_commit(b_tile + 24 * t + 16);
+      ap_commit(bar + 16);
     };
-    // queries are in shared memory: the softmax warps' first arrival at "P ready"
-    for (int t = 0; t < TILES && good; ++t)
-      if (n_of[t] > 0) good = wait(b_tile + 24 * t + 8, 0);
-    if (n > 0 && good) good = wait(b_full, 0);
-    if (n > 0 && good) {
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        if (n_of[t] > 0) scores(t, 0);
-      ap_commit(b_empty);
+    // A warp says of every unit that it is done with it, also of one that its tile has no use for: after that unit has come,
+    // so that the word is for this turn of the ring.
+    auto full = [&](int u) { wait(b_full + 8 * (u % KP_RING), (u / KP_RING) & 1); };
+    auto done = [&](int u) { ap_commit(b_empty + 8 * (u % KP_RING)); };
+    if (n > 0) {
+      if (my_n > 0) wait(bar + 8, 0);  // queries are in shared memory: the softmax warps' first arrival at "P ready"
+      full(0);
+      if (my_n > 0 && good) scores(0);
+      done(0);
     }
     for (int j = 0; j < n && good; ++j) {
-      const int vs = (2 * j + 1) % KP_RING, ks = (2 * j + 2) % KP_RING;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        if (j < n_of[t] && good) {
-          good = wait(b_tile + 24 * t + 8, (j + 1) & 1);
-          if (good) good = wait(b_full + 8 * vs, ((2 * j + 1) / KP_RING) & 1);
-          if (good) values(t, j);
-        }
-        if (t == TILES - 1) ap_commit(b_empty + 8 * vs);
-        if (j + 1 < n_of[t] && good) {
-          good = wait(b_full + 8 * ks, ((2 * j + 2) / KP_RING) & 1);
-          if (good) good = wait(b_tile + 24 * t + 16, j & 1);
-          if (good) scores(t, j + 1);
-        }
-        if (t == TILES - 1 && j + 1 < n) ap_commit(b_empty + 8 * ks);
+      full(2 * j + 1);
+      if (j < my_n) {
+        wait(bar + 8, (j + 1) & 1);
+        if (good) values(j);
       }
+      done(2 * j + 1);
+      if (j + 1 == n || !good) break;
+      full(2 * j + 2);
+      if (j + 1 < my_n) {
+        wait(bar + 16, j & 1);
+        if (good) scores(j + 1);
+      }
+      done(2 * j + 2);
     }
     // every product and every arrival of a commit has to be over before this memory is another CTA's
-    ap_commit(b_end);
-    if (!__all_sync(0xffffffffu, ap_wait(b_end, 0, 1u << 18))) good = false;
+    ap_commit(bar + 24);
+    if (!__all_sync(0xffffffffu, ap_wait(bar + 24, 0, 1u << 18))) good = false;
     if (!good) fail_s = 1;
   } else {
     // ---- softmax: thread = packed row first + 128 t + (tid & 127); its tensor memory lanes are the warp's of its four
     const int t = warp >> 2, mine = tid & 127, tile0 = first + t * KP_BM;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + 256 * t + lanes, to = ts + 128, bar = b_tile + 24 * t;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + 256 * t + lanes, to = ts + 128, bar = b_tile + 32 * t;
     unsigned char *const q_s = smem + t * Z::Q_BYTES;
     const int my_n = n_of[t], packed = tile0 + mine, last = min(tile0 + KP_BM, rows) - 1;
     const int limit = packed <= last ? limit_of(packed) : 0;
@@ -340,12 +352,12 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
     if (my_n > 0) ask(0);
     float m = -CUDART_INF_F, l = 0.f;
     bool good = true;
-    float(&sc)[3][KP_BLOCKS] = scales_s[warp];
+    float4(&sc)[KP_BLOCKS] = scales_s[warp];
     for (int j = 0; j < my_n; ++j) {
       __syncwarp();
       if (lane < KP_BLOCKS) {
         const float vs = fmaxf(vs_next, KP_LEAST_SCALE);
-        sc[0][lane] = ks_next * scale, sc[1][lane] = __log2f(vs), sc[2][lane] = __fdividef(1.f, vs);
+        sc[lane] = make_float4(ks_next * scale, __log2f(vs), __fdividef(1.f, vs), 0.f);
       }
       __syncwarp();
       if (j + 1 < my_n) ask(j + 1);
@@ -356,85 +368,112 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int left = limit - (j0 + j) * KP_BN;  // keys of this tile the row attends to
       const bool all = __all_sync(0xffffffffu, left >= KP_BN || packed > last);
-      // the largest exponent of the row
-      float mx = -CUDART_INF_F;
-      uint32_t sr[2][32];
-      ap_ld32(ts, sr[0]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t(&s)[32] = sr[c & 1];
-        ap_wait_ld();
-        ap_ld32(ts + 32 * ((c + 1) & 3), sr[(c + 1) & 1]);  // after the last: the first again, for the second pass
+      // 32 keys of the row: y = x - m + 6, and P = 2^y where no y is above 14
+      auto chunk = [&](int c, uint32_t(&s)[32], uint32_t(&next)[32]) {
+        uint64_t y[16];
+        float f[2], lv[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float top = -CUDART_INF_F;
-          if (all) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(s[16 * h + i]), __uint_as_float(s[16 * h + i + 1])));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = 32 * c + 16 * h + i < left ? fmaxf(top, __uint_as_float(s[16 * h + i])) : top;
-          }
-          const float f = PARTS == 1 ? sc[0][2 * c + h] : sc[0][2 * c + h] * back;
-          const float x = fmaf(top, f, sc[1][2 * c + h]);
-          mx = top == -CUDART_INF_F ? mx : fmaxf(mx, x);
+          const float4 q = sc[2 * c + h];
+          f[h] = PARTS == 1 ? q.x : q.x * back, lv[h] = q.y;
         }
-      }
-      const bool raise = mx > m + KP_RAISE;
-      if (__any_sync(0xffffffffu, raise)) {
-        const float up = raise ? mx : m, f = up == m ? 1.f : m == -CUDART_INF_F ? 0.f : ap_ex2(m - up);
-        m = up;
-        l *= f;
-        if (j > 0) {  // these scores waited for the product of the tile before
+        auto exponents = [&](float shift) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint64_t f2 = kp_pack(f[h], f[h]), d2 = kp_pack(lv[h] - shift, lv[h] - shift);
+#pragma unroll
+            for (int i = 8 * h; i < 8 * h + 8; ++i) y[i] = kp_fma2(kp_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), f2, d2);
+          }
+          if (!all) {
+            const int mine = left - 32 * c;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const KpPair v = kp_unpack(y[i]);
+              y[i] = kp_pack(2 * i < mine ? v.a : -CUDART_INF_F, 2 * i + 1 < mine ? v.b : -CUDART_INF_F);
+            }
+          }
+          float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const KpPair v = kp_unpack(y[i]);
+            top[i & 1] = fmaxf(top[i & 1], fmaxf(v.a, v.b));
+          }
+          return fmaxf(top[0], top[1]);
+        };
+        const bool raise = exponents(m - KP_P_EXP) > KP_P_EXP + KP_RAISE;  // m = -inf: any key raises it
+        if (__any_sync(0xffffffffu, raise)) {
+          const float top = exponents(0.f), up = raise ? top : m, by = up == m ? 1.f : m == -CUDART_INF_F ? 0.f : ap_ex2(m - up);
+          m = up;
+          l *= by;
+          ap_wait_st();
+          if (j > 0) {  // O: these scores waited for the product of the tile before
 #pragma unroll 1
-          for (int d = 0; d < KV8_D; d += 16) {
-            uint32_t o[16];
-            ap_ld16(to + d, o);
+            for (int d = 0; d < KV8_D; d += 16) {
+              uint32_t o[16];
+              ap_ld16(to + d, o);
+              ap_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+              ap_st16(to + d, o);
+            }
+          }
+#pragma unroll 1
+          for (int b = 0; b < c; ++b) {  // P of this tile's earlier keys
+            uint32_t hi[16], lo[16];
+            ap_ld16(ts + (PARTS == 1 ? 16 : 32) * b, hi);
+            if constexpr (PARTS == 2) ap_ld16(ts + 32 * b + 16, lo);
             ap_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            ap_st16(to + d, o);
+            for (int i = 0; i < 16; ++i) {
+              float2 v = __half22float2(u2h2(hi[i]));
+              if constexpr (PARTS == 2) {
+                const float2 w = __half22float2(u2h2(lo[i]));
+                v.x = (v.x + w.x) * by, v.y = (v.y + w.y) * by;
+                const __half2 h = __floats2half2_rn(v.x, v.y);
+                const float2 hf = __half22float2(h);
+                hi[i] = h22u(h), lo[i] = h22u(__floats2half2_rn(v.x - hf.x, v.y - hf.y));
+              } else {
+                hi[i] = h22u(__floats2half2_rn(v.x * by, v.y * by));
+              }
+            }
+            ap_st16(ts + (PARTS == 1 ? 16 : 32) * b, hi);
+            if constexpr (PARTS == 2) ap_st16(ts + 32 * b + 16, lo);
           }
+          exponents(m == -CUDART_INF_F ? 0.f : m - KP_P_EXP);
         }
-      }
-      const float shift = m == -CUDART_INF_F ? 0.f : m - KP_P_EXP;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t(&s)[32] = sr[c & 1];
-        ap_wait_ld();
-        if (c < 3) ap_ld32(ts + 32 * (c + 1), sr[(c + 1) & 1]);
+        // the next 32 scores come while these become P.  Not earlier: their registers are not to be touched before they are
+        // there, not even to be spilled
+        if (c < 3) ap_ld32(ts + 32 * c + 32, next);
         uint32_t hi[16], lo[PARTS == 1 ? 1 : 16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float f = PARTS == 1 ? sc[0][2 * c + h] : sc[0][2 * c + h] * back, d = sc[1][2 * c + h] - shift;
-          const uint64_t f2 = kp_pack(f, f), d2 = kp_pack(d, d);
           uint64_t sum = kp_pack(0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = 16 * h + 2 * i;
-            KpPair x = kp_unpack(kp_fma2(kp_pack(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), f2, d2));
-            if (!all) {
-              x.a = 32 * c + at < left ? x.a : -CUDART_INF_F;
-              x.b = 32 * c + at + 1 < left ? x.b : -CUDART_INF_F;
-            }
-            const float a = ap_ex2(x.a), b = ap_ex2(x.b);
+          for (int i = 8 * h; i < 8 * h + 8; ++i) {
+            const KpPair v = kp_unpack(y[i]);
+            const float a = ap_ex2(v.a), b = ap_ex2(v.b);
             sum = kp_add2(sum, kp_pack(a, b));
             const __half2 hh = __floats2half2_rn(a, b);
-            hi[8 * h + i] = h22u(hh);
+            hi[i] = h22u(hh);
             if constexpr (PARTS == 2) {
               const float2 hf = __half22float2(hh);
-              lo[8 * h + i] = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
+              lo[i] = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
             }
           }
           const KpPair both = kp_unpack(sum);
-          l = fmaf(both.a + both.b, sc[2][2 * c + h], l);
+          l = fmaf(both.a + both.b, sc[2 * c + h].z, l);
         }
-        if constexpr (PARTS == 1) {
-          ap_st16(ts + 16 * c, hi);
-        } else {
-          ap_st16(ts + 32 * c, hi);
-          ap_st16(ts + 32 * c + 16, lo);
-        }
+        ap_st16(ts + (PARTS == 1 ? 16 : 32) * c, hi);
+        if constexpr (PARTS == 2) ap_st16(ts + 32 * c + 16, lo);
+      };
+      uint32_t s0[32], s1[32];
+      ap_ld32(ts, s0);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        kp_wait_ld(s0);
+        chunk(c, s0, s1);
+        kp_wait_ld(s1);
+        chunk(c + 1, s1, s0);
       }
       ap_wait_st();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
