@@ -2,6 +2,8 @@
 // mathematics: kv8_attention.cu): x = (q . k_code) scale log2(e) ks + log2(vs), P = 2^(x - m), O += P v_code, l += sum P / vs.
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "attention_mma.cuh"
 #include "kv8.cuh"
 #include "kv8_prefill.cuh"
@@ -54,6 +56,19 @@ __device__ __forceinline__ bool kp_wait(uint32_t bar, unsigned parity, const vol
   }
   return false;
 }
+// 2^y for two y of -126 .. 126 on the fused multiply-add pipes: y = n + r with r in -1/2 .. 1/2, a polynomial for 2^r fitted for the
+// least relative error (2.7e-6, a hundredth of a step of the fp16 it becomes), n added to its exponent.
+__device__ __forceinline__ uint64_t kp_exp2(uint64_t y) {
+  const uint64_t magic = kp_pack(12582912.f, 12582912.f), minus = kp_pack(-12582912.f, -12582912.f), neg = kp_pack(-1.f, -1.f);
+  auto both = [](float c) { return kp_pack(c, c); };
+  const uint64_t n = kp_add2(y, magic), r = kp_fma2(kp_add2(n, minus), neg, y);
+  uint64_t e = kp_fma2(both(0.00957010195f), r, both(0.0559178616f));
+  e = kp_fma2(e, r, both(0.240247448f));
+  e = kp_fma2(e, r, both(0.693121815f));
+  e = kp_fma2(e, r, both(0.999999261f));
+  const KpPair nn = kp_unpack(n), ee = kp_unpack(e);
+  return kp_pack(__int_as_float((__float_as_int(nn.a) << 23) + __float_as_int(ee.a)), __int_as_float((__float_as_int(nn.b) << 23) + __float_as_int(ee.b)));
+}
 // Nothing uses the loaded registers before this.
 __device__ __forceinline__ void kp_wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -72,8 +87,8 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   using Z = KpShape<TILES, PARTS>;
   extern __shared__ unsigned char kp_smem_raw[];
   unsigned char *smem = kp_smem_raw + ((1024u - (ap_smem_u32(kp_smem_raw) & 1023u)) & 1023u);  // swizzle atoms need 1024-byte alignment
-  // barriers: full[], empty[], then for each tile: scores ready, P ready, O done, the end of all its products
-  __shared__ __align__(8) uint64_t bars[2 * KP_RING + 4 * TILES];
+  // barriers: full[], empty[], then for each tile: scores of the first 64 keys, of the others, P ready, O done, the others' scores read, the end of all products
+  __shared__ __align__(8) uint64_t bars[2 * KP_RING + 6 * TILES];
   __shared__ uint32_t tmem_s;
   __shared__ int fail_s, seq_s;
   __shared__ float4 scales_s[4 * TILES][KP_BLOCKS];  // a softmax warp's own: factor of the scores, log2(vs), 1 / vs
@@ -121,12 +136,78 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b_empty + 8 * i), "n"(TILES));
     }
     for (int t = 0; t < TILES; ++t) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 32 * t));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(b_tile + 32 * t + 8));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 32 * t + 16));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(b_tile + 32 * t + 24));
+      for (int i = 0; i < 6; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b_tile + 48 * t + 8 * i), "r"(i == 2 || i == 4 ? 128 : 1));
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  float back = 1.f;  // fp32 queries: what undoes the power of two that a softmax thread's row is scaled by
+  if (warp < Z::SOFT_WARPS) {
+    // ---- the queries to shared memory: 16-byte chunk c of row i to half c / 8, chunk position (c % 8) ^ (i % 8)
+    const int t = warp >> 2, mine = tid & 127, tile0 = first + t * KP_BM, last = min(tile0 + KP_BM, rows) - 1;
+    unsigned char *const q_s = smem + t * Z::Q_BYTES;
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale is the queries': the scores' factors are not negative
+    if constexpr (PARTS == 1) {
+      const int c = mine & 15, i0 = mine >> 4;
+      const int step_t = 8 / p.group, step_h = 8 - step_t * p.group;
+      int token = (tile0 + i0) / p.group, head = tile0 + i0 - token * p.group;
+      uint4 v[KP_BM / 8];
+#pragma unroll
+      for (int n = 0; n < KP_BM / 8; ++n) {
+        v[n] = make_uint4(0, 0, 0, 0);
+        if (tile0 + i0 + 8 * n <= last)
+          v[n] = *reinterpret_cast<const uint4 *>((const __half *)p.q + (size_t)(row0 + token) * p.q_stride + (size_t)(hk * p.group + head) * KV8_D + c * 8);
+        token += step_t, head += step_h;
+        if (head >= p.group) head -= p.group, ++token;
+      }
+#pragma unroll
+      for (int n = 0; n < KP_BM / 8; ++n) {
+        const int i = i0 + 8 * n;
+        v[n].x ^= flip, v[n].y ^= flip, v[n].z ^= flip, v[n].w ^= flip;
+        *reinterpret_cast<uint4 *>(q_s + (c >> 3) * KP_HALF_BYTES + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = v[n];
+      }
+    } else {
+      const int packed = tile0 + mine;
+      if (packed <= last) {
+        // a row a thread: scaled by a power of two, its largest to 2^13 .. 2^14, and cut into two fp16 numbers
+        const int token = packed / p.group, head = hk * p.group + packed - token * p.group;
+        const float4 *q = reinterpret_cast<const float4 *>((const float *)p.q + (size_t)(row0 + token) * p.q_stride + (size_t)head * KV8_D);
+        uint32_t most = 0;
+#pragma unroll 8
+        for (int c = 0; c < KV8_D / 4; ++c) {
+          const float4 v = q[c];
+          most = max(max(most, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
+        }
+        const int e = max(-100, min(100, 13 - (int)(most >> 23) + 127));
+        const float up = __int_as_float((127 + e) << 23) * (flip ? -1.f : 1.f);
+        back = most >= 0x7f800000u ? CUDART_NAN_F : __int_as_float((127 - e) << 23);
+#pragma unroll 4
+        for (int c = 0; c < KV8_D / 8; ++c) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 v = q[2 * c + h];
+            const float x[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+              const float2 b = __half22float2(a);
+              hi[2 * h + i] = h22u(a);
+              lo[2 * h + i] = h22u(__floats2half2_rn(x[2 * i] - b.x, x[2 * i + 1] - b.y));
+            }
+          }
+          unsigned char *d = q_s + (c >> 3) * KP_HALF_BYTES + mine * 128 + (((c & 7) ^ (mine & 7)) << 4);
+          *reinterpret_cast<uint4 *>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4 *>(d + KP_STAGE_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      } else {
+#pragma unroll 4
+        for (int c = 0; c < KV8_D / 8; ++c) {
+          unsigned char *d = q_s + (c >> 3) * KP_HALF_BYTES + mine * 128 + (((c & 7) ^ (mine & 7)) << 4);
+          *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<uint4 *>(d + KP_STAGE_BYTES) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == Z::MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ap_smem_u32(&tmem_s)), "n"(Z::TMEM_COLS) : "memory");
@@ -209,133 +290,79 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (!good) fail_s = 1;
   } else if (warp >= Z::MMA_WARP) {
-    // ---- MMA issue, a warp for each tile of rows.  Its scores go where its P lay, so they wait for that P's product;
-    // meanwhile the other tile's are under way.
+    // ---- MMA issue, a warp for each tile of rows.  Scores of a tile of keys are two products, 64 keys each, in the two
+    // halves of the tile's columns; its P ends up in the half of the first 64.  The next tile's first 64 keys go where the
+    // others lay, as soon as those have been read; its others wait for P's product.  (Two parts of P fill both halves: nothing goes early.)
     const int t = warp - Z::MMA_WARP, my_n = n_of[t];
-    const uint32_t bar = b_tile + 32 * t;
-    constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_BN >> 3) << 17) | ((uint32_t)(KP_BM >> 4) << 24);
+    const uint32_t bar = b_tile + 48 * t, bar_p = bar + 16, bar_o = bar + 24, bar_r = bar + 32;
+    constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_BN / 2 >> 3) << 17) | ((uint32_t)(KP_BM >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(KV8_D >> 3) << 17) | ((uint32_t)(KP_BM >> 4) << 24);  // bit 16: B is MN-major
     bool good = true;
     auto wait = [&](uint32_t b, unsigned parity) { good = good && __all_sync(0xffffffffu, kp_wait(b, parity, &fail_s)); };
-    auto scores = [&](int j) {
+    auto scores = [&](int j, int half) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint64_t b0 = ap_desc(ring + (2 * j % KP_RING) * KP_STAGE_BYTES, 16);
+      const uint64_t b0 = ap_desc(ring + (2 * j % KP_RING) * KP_STAGE_BYTES + half * (KP_HALF_BYTES / 2), 16);
+      const uint32_t d = tmem + 256 * t + 64 * (PARTS == 1 ? (j & 1) ^ half : half);
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
         const uint64_t a0 = ap_desc(q_base + t * Z::Q_BYTES + part * KP_STAGE_BYTES, 16);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {  // 16 dims further: 32 B inside a swizzled row, four steps per 64-dim half
           const uint64_t step = (uint64_t)((k >> 2) * (KP_HALF_BYTES / 16) + (k & 3) * 2);
-          ap_mma_ss(tmem + 256 * t, a0 + step, b0 + step, ID_S, k > 0 || part > 0);
+          ap_mma_ss(d, a0 + step, b0 + step, ID_S, k > 0 || part > 0);
         }
       }
-      ap_commit(bar);
+      ap_commit(bar + 8 * half);
     };
     auto values = [&](int j) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint64_t b0 = ap_desc(ring + ((2 * j + 1) % KP_RING) * KP_STAGE_BYTES, KP_HALF_BYTES);
-      const uint32_t a0 = tmem + 256 * t, d = a0 + 128;
+      const uint32_t a0 = tmem + 256 * t + (PARTS == 1 ? 64 * (j & 1) : 0), d = tmem + 256 * t + 128;
 #pragma unroll
       for (int k = 0; k < 8; ++k)  // 16 keys: two swizzle atoms of V; P lies as 8 columns, of fp32 rows 16 with the first part, 16 with the second
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
           ap_mma_ts(d, a0 + (PARTS == 1 ? 8 * k : 32 * (k >> 1) + 16 * part + 8 * (k & 1)), b0 + (uint64_t)(k * (2048 / 16)), ID_O, j > 0 || k > 0 || part > 0);
-      ap_commit(bar + 16);
+      ap_commit(bar_o);
     };
     // A warp says of every unit that it is done with it, also of one that its tile has no use for: after that unit has come,
     // so that the word is for this turn of the ring.
     auto full = [&](int u) { wait(b_full + 8 * (u % KP_RING), (u / KP_RING) & 1); };
     auto done = [&](int u) { ap_commit(b_empty + 8 * (u % KP_RING)); };
     if (n > 0) {
-      if (my_n > 0) wait(bar + 8, 0);  // queries are in shared memory: the softmax warps' first arrival at "P ready"
       full(0);
-      if (my_n > 0 && good) scores(0);
+      if (my_n > 0 && good) scores(0, 0), scores(0, 1);
       done(0);
     }
     for (int j = 0; j < n && good; ++j) {
       full(2 * j + 1);
-      if (j < my_n) {
-        wait(bar + 8, (j + 1) & 1);
-        if (good) values(j);
+      if (j + 1 < n) full(2 * j + 2);
+      if (PARTS == 1 && j + 1 < my_n) {
+        wait(bar_r, j & 1);
+        if (good) scores(j + 1, 0);
       }
+      if (j < my_n) wait(bar_p, j & 1);
+      if (j < my_n && good) values(j);
       done(2 * j + 1);
       if (j + 1 == n || !good) break;
-      full(2 * j + 2);
       if (j + 1 < my_n) {
-        wait(bar + 16, j & 1);
-        if (good) scores(j + 1);
+        wait(bar_o, j & 1);
+        if (PARTS == 2 && good) scores(j + 1, 0);
+        if (good) scores(j + 1, 1);
       }
       done(2 * j + 2);
     }
     // every product and every arrival of a commit has to be over before this memory is another CTA's
-    ap_commit(bar + 24);
-    if (!__all_sync(0xffffffffu, ap_wait(bar + 24, 0, 1u << 18))) good = false;
+    ap_commit(bar + 40);
+    if (!__all_sync(0xffffffffu, ap_wait(bar + 40, 0, 1u << 18))) good = false;
     if (!good) fail_s = 1;
   } else {
     // ---- softmax: thread = packed row first + 128 t + (tid & 127); its tensor memory lanes are the warp's of its four
     const int t = warp >> 2, mine = tid & 127, tile0 = first + t * KP_BM;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + 256 * t + lanes, to = ts + 128, bar = b_tile + 32 * t;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + 256 * t + lanes, to = ts + 128, bar = b_tile + 48 * t, bar_p = bar + 16, bar_o = bar + 24, bar_r = bar + 32;
     unsigned char *const q_s = smem + t * Z::Q_BYTES;
     const int my_n = n_of[t], packed = tile0 + mine, last = min(tile0 + KP_BM, rows) - 1;
     const int limit = packed <= last ? limit_of(packed) : 0;
-    float back = 1.f;
-    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale is the queries': factors below are not negative
-    if (my_n > 0) {
-      if constexpr (PARTS == 1) {
-        // 16-byte chunk c of row i to half c / 8, chunk position (c % 8) ^ (i % 8)
-        const int c = mine & 15;
-#pragma unroll 4
-        for (int i = mine >> 4; i < KP_BM; i += 8) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (tile0 + i <= last) {
-            const int token = (tile0 + i) / p.group, head = hk * p.group + tile0 + i - token * p.group;
-            v = *reinterpret_cast<const uint4 *>((const __half *)p.q + (size_t)(row0 + token) * p.q_stride + (size_t)head * KV8_D + c * 8);
-          }
-          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-          *reinterpret_cast<uint4 *>(q_s + (c >> 3) * KP_HALF_BYTES + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = v;
-        }
-      } else if (packed <= last) {
-        // a row a thread: scaled by a power of two, its largest to 2^13 .. 2^14, and cut into two fp16 numbers
-        const int token = packed / p.group, head = hk * p.group + packed - token * p.group;
-        const float4 *q = reinterpret_cast<const float4 *>((const float *)p.q + (size_t)(row0 + token) * p.q_stride + (size_t)head * KV8_D);
-        uint32_t most = 0;
-#pragma unroll 8
-        for (int c = 0; c < KV8_D / 4; ++c) {
-          const float4 v = q[c];
-          most = max(max(most, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
-        }
-        const int e = max(-100, min(100, 13 - (int)(most >> 23) + 127));
-        const float up = __int_as_float((127 + e) << 23) * (flip ? -1.f : 1.f);
-        back = most >= 0x7f800000u ? CUDART_NAN_F : __int_as_float((127 - e) << 23);
-#pragma unroll 4
-        for (int c = 0; c < KV8_D / 8; ++c) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 v = q[2 * c + h];
-            const float x[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-              const float2 b = __half22float2(a);
-              hi[2 * h + i] = h22u(a);
-              lo[2 * h + i] = h22u(__floats2half2_rn(x[2 * i] - b.x, x[2 * i + 1] - b.y));
-            }
-          }
-          unsigned char *d = q_s + (c >> 3) * KP_HALF_BYTES + mine * 128 + (((c & 7) ^ (mine & 7)) << 4);
-          *reinterpret_cast<uint4 *>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4 *>(d + KP_STAGE_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-      } else {
-#pragma unroll 4
-        for (int c = 0; c < KV8_D / 8; ++c) {
-          unsigned char *d = q_s + (c >> 3) * KP_HALF_BYTES + mine * 128 + (((c & 7) ^ (mine & 7)) << 4);
-          *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<uint4 *>(d + KP_STAGE_BYTES) = make_uint4(0, 0, 0, 0);
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      ap_arrive(bar + 8);
-    }
     const float scale = fabsf(p.scale);
     float ks_next = 0.f, vs_next = 1.f;
     auto ask = [&](int j) {  // the scales of key tile j0 + j, a block each for the first eight lanes
@@ -368,45 +395,51 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int left = limit - (j0 + j) * KP_BN;  // keys of this tile the row attends to
       const bool all = __all_sync(0xffffffffu, left >= KP_BN || packed > last);
-      // 32 keys of the row: y = x - m + 6, and P = 2^y where no y is above 14
-      auto chunk = [&](int c, uint32_t(&s)[32], uint32_t(&next)[32]) {
-        uint64_t y[16];
-        float f[2], lv[2];
+      const uint32_t t_first = ts + (PARTS == 1 ? 64 * (j & 1) : 0), t_other = ts + (PARTS == 1 ? 64 * (j & 1 ^ 1) : 64);
+      auto p_at = [&](int c) { return PARTS == 1 ? t_first + 16 * c : ts + 32 * c; };  // P of 32 keys
+      // 64 keys of the row: their largest exponent, then P = 2^(x - m + 6)
+      auto half = [&](int hb, auto all_keys) {
+        constexpr bool ALL = decltype(all_keys)::value;
+        uint32_t s[64];
+        uint32_t(&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
+        uint32_t(&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
+        const uint32_t at = hb ? t_other : t_first;
+        ap_ld32(at, s0);
+        ap_ld32(at + 32, s1);
+        float f[4], lv[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 q = sc[2 * c + h];
-          f[h] = PARTS == 1 ? q.x : q.x * back, lv[h] = q.y;
+        for (int b = 0; b < 4; ++b) {
+          const float4 q = sc[4 * hb + b];
+          f[b] = PARTS == 1 ? q.x : q.x * back, lv[b] = q.y;
         }
-        auto exponents = [&](float shift) {
+        const int mine = left - 64 * hb;
+        kp_wait_ld(s0);
+        kp_wait_ld(s1);
+        if (PARTS == 1 && hb == 1) {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          ap_arrive(bar_r);
+        }
+        float mx = -CUDART_INF_F;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint64_t f2 = kp_pack(f[h], f[h]), d2 = kp_pack(lv[h] - shift, lv[h] - shift);
-#pragma unroll
-            for (int i = 8 * h; i < 8 * h + 8; ++i) y[i] = kp_fma2(kp_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), f2, d2);
-          }
-          if (!all) {
-            const int mine = left - 32 * c;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const KpPair v = kp_unpack(y[i]);
-              y[i] = kp_pack(2 * i < mine ? v.a : -CUDART_INF_F, 2 * i + 1 < mine ? v.b : -CUDART_INF_F);
-            }
-          }
+        for (int b = 0; b < 4; ++b) {
           float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const KpPair v = kp_unpack(y[i]);
-            top[i & 1] = fmaxf(top[i & 1], fmaxf(v.a, v.b));
+          for (int i = 16 * b; i < 16 * b + 16; i += 2) {
+            const float u = ALL || i < mine ? __uint_as_float(s[i]) : -CUDART_INF_F, v = ALL || i + 1 < mine ? __uint_as_float(s[i + 1]) : -CUDART_INF_F;
+            top[i >> 1 & 1] = fmaxf(top[i >> 1 & 1], fmaxf(u, v));
           }
-          return fmaxf(top[0], top[1]);
-        };
-        const bool raise = exponents(m - KP_P_EXP) > KP_P_EXP + KP_RAISE;  // m = -inf: any key raises it
+          const float t = fmaxf(top[0], top[1]);
+          mx = fmaxf(mx, !ALL && t == -CUDART_INF_F ? t : fmaf(t, f[b], lv[b]));
+        }
+        const bool raise = mx > m + KP_RAISE;
         if (__any_sync(0xffffffffu, raise)) {
-          const float top = exponents(0.f), up = raise ? top : m, by = up == m ? 1.f : m == -CUDART_INF_F ? 0.f : ap_ex2(m - up);
+          const float up = raise ? mx : m, by = up == m ? 1.f : m == -CUDART_INF_F ? 0.f : ap_ex2(m - up);
           m = up;
           l *= by;
           ap_wait_st();
-          if (j > 0) {  // O: these scores waited for the product of the tile before
+          if (j > 0) {  // O: the other half of these scores waits for the product of the tile before
+            if (PARTS == 1 && hb == 0 && !__all_sync(0xffffffffu, kp_wait(bar_o, (j - 1) & 1, &fail_s))) fail_s = 1;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int d = 0; d < KV8_D; d += 16) {
               uint32_t o[16];
@@ -418,10 +451,11 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
             }
           }
 #pragma unroll 1
-          for (int b = 0; b < c; ++b) {  // P of this tile's earlier keys
-            uint32_t hi[16], lo[16];
-            ap_ld16(ts + (PARTS == 1 ? 16 : 32) * b, hi);
-            if constexpr (PARTS == 2) ap_ld16(ts + 32 * b + 16, lo);
+          for (int c = 0; c < 2 * hb; ++c) {  // P of this tile's first keys
+            uint32_t hi[16];
+            [[maybe_unused]] uint32_t lo[PARTS == 1 ? 1 : 16];
+            ap_ld16(p_at(c), hi);
+            if constexpr (PARTS == 2) ap_ld16(p_at(c) + 16, lo);
             ap_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -436,52 +470,73 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
                 hi[i] = h22u(__floats2half2_rn(v.x * by, v.y * by));
               }
             }
-            ap_st16(ts + (PARTS == 1 ? 16 : 32) * b, hi);
-            if constexpr (PARTS == 2) ap_st16(ts + 32 * b + 16, lo);
+            ap_st16(p_at(c), hi);
+            if constexpr (PARTS == 2) ap_st16(p_at(c) + 16, lo);
           }
-          exponents(m == -CUDART_INF_F ? 0.f : m - KP_P_EXP);
         }
-        // the next 32 scores come while these become P.  Not earlier: their registers are not to be touched before they are
-        // there, not even to be spilled
-        if (c < 3) ap_ld32(ts + 32 * c + 32, next);
-        uint32_t hi[16], lo[PARTS == 1 ? 1 : 16];
+        const float shift = m == -CUDART_INF_F ? 0.f : m - KP_P_EXP;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint64_t sum = kp_pack(0.f, 0.f);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t hi[16];
+          [[maybe_unused]] uint32_t lo[PARTS == 1 ? 1 : 16];
 #pragma unroll
-          for (int i = 8 * h; i < 8 * h + 8; ++i) {
-            const KpPair v = kp_unpack(y[i]);
-            const float a = ap_ex2(v.a), b = ap_ex2(v.b);
-            sum = kp_add2(sum, kp_pack(a, b));
-            const __half2 hh = __floats2half2_rn(a, b);
-            hi[i] = h22u(hh);
-            if constexpr (PARTS == 2) {
-              const float2 hf = __half22float2(hh);
-              lo[i] = h22u(__floats2half2_rn(a - hf.x, b - hf.y));
+          for (int h = 0; h < 2; ++h) {
+            const int b = 2 * c + h;
+            const uint64_t f2 = kp_pack(f[b], f[b]), d2 = kp_pack(lv[b] - shift, lv[b] - shift);
+            uint64_t sum = kp_pack(0.f, 0.f);
+#pragma unroll
+            for (int i = 8 * h; i < 8 * h + 8; ++i) {
+              const int k = 32 * c + 2 * i;
+              KpPair v = kp_unpack(kp_fma2(kp_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, d2));
+              if constexpr (!ALL) v.a = k < mine ? v.a : -CUDART_INF_F, v.b = k + 1 < mine ? v.b : -CUDART_INF_F;
+              float a, b2;
+              if (PARTS == 1 && i % 4 == 3) {  // a quarter of them off the exponential unit
+                const KpPair e = kp_unpack(kp_exp2(kp_pack(fmaxf(v.a, -126.f), fmaxf(v.b, -126.f))));
+                a = e.a, b2 = e.b;
+              } else {
+                a = ap_ex2(v.a), b2 = ap_ex2(v.b);
+              }
+              sum = kp_add2(sum, kp_pack(a, b2));
+              const __half2 hh = __floats2half2_rn(a, b2);
+              hi[i] = h22u(hh);
+              if constexpr (PARTS == 2) {
+                const float2 hf = __half22float2(hh);
+                lo[i] = h22u(__floats2half2_rn(a - hf.x, b2 - hf.y));
+              }
             }
+            const KpPair both = kp_unpack(sum);
+            l = fmaf(both.a + both.b, sc[4 * hb + b].z, l);
           }
-          const KpPair both = kp_unpack(sum);
-          l = fmaf(both.a + both.b, sc[2 * c + h].z, l);
+          ap_st16(p_at(2 * hb + c), hi);
+          if constexpr (PARTS == 2) ap_st16(p_at(2 * hb + c) + 16, lo);
         }
-        ap_st16(ts + (PARTS == 1 ? 16 : 32) * c, hi);
-        if constexpr (PARTS == 2) ap_st16(ts + 32 * c + 16, lo);
       };
-      uint32_t s0[32], s1[32];
-      ap_ld32(ts, s0);
 #pragma unroll 1
-      for (int c = 0; c < 4; c += 2) {
-        kp_wait_ld(s0);
-        chunk(c, s0, s1);
-        kp_wait_ld(s1);
-        chunk(c + 1, s1, s0);
+      for (int hb = 0; hb < 2; ++hb) {
+        if (hb > 0) {
+          good = __all_sync(0xffffffffu, kp_wait(bar + 8, j & 1, &fail_s));
+          if (!good) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (all) {
+          half(hb, std::true_type{});
+        } else if (__any_sync(0xffffffffu, left > 64 * hb)) {
+          half(hb, std::false_type{});
+        } else {  // no row of the warp attends to any of these keys
+          const uint32_t none[16] = {};
+#pragma unroll
+          for (int c = 0; c < (PARTS == 1 ? 2 : 4); ++c) ap_st16((PARTS == 1 ? t_first + 32 * hb : ts + 64 * hb) + 16 * c, none);
+          if (PARTS == 1 && hb == 1) ap_arrive(bar_r);
+        }
       }
+      if (!good) break;
       ap_wait_st();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      ap_arrive(bar + 8);
+      ap_arrive(bar_p);
     }
     // ---- O / l: a thread's row through its own idle query memory, then stored as whole rows; or its part, to be joined
-    if (good && my_n > 1) good = __all_sync(0xffffffffu, kp_wait(bar + 16, (my_n - 2) & 1, &fail_s));
-    if (good && my_n > 0) good = __all_sync(0xffffffffu, kp_wait(bar + 16, (my_n - 1) & 1, &fail_s));
+    if (good && my_n > 1) good = __all_sync(0xffffffffu, kp_wait(bar_o, (my_n - 2) & 1, &fail_s));
+    if (good && my_n > 0) good = __all_sync(0xffffffffu, kp_wait(bar_o, (my_n - 1) & 1, &fail_s));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (!good) {
       fail_s = 1;
@@ -532,13 +587,15 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
         __syncwarp();
         // the warp's 32 rows, CHUNKS lanes a row
         const int c = lane % CHUNKS;
+        constexpr int STEP = 32 / CHUNKS;
+        const int from = (warp & 3) * 32 + lane / CHUNKS, step_t = STEP / p.group, step_h = STEP - step_t * p.group;
+        int token = (tile0 + from) / p.group, head = tile0 + from - token * p.group;
 #pragma unroll 4
-        for (int i = lane / CHUNKS; i < 32; i += 32 / CHUNKS) {
-          const int in_tile = (warp & 3) * 32 + i, pk = tile0 + in_tile;
-          if (pk > last) break;
+        for (int in_tile = from; in_tile < from + 32 && tile0 + in_tile <= last; in_tile += STEP) {
           const uint4 v = *reinterpret_cast<const uint4 *>(q_s + in_tile * (KV8_D * sizeof(T)) + ((c ^ (in_tile & 7)) << 4));
-          const int token = pk / p.group, head = hk * p.group + pk - token * p.group;
-          *reinterpret_cast<uint4 *>((T *)p.out + ((size_t)(row0 + token) * p.Hq + head) * KV8_D + c * EACH) = v;
+          *reinterpret_cast<uint4 *>((T *)p.out + ((size_t)(row0 + token) * p.Hq + hk * p.group + head) * KV8_D + c * EACH) = v;
+          token += step_t, head += step_h;
+          if (head >= p.group) head -= p.group, ++token;
         }
       }
     }
