@@ -147,7 +147,7 @@ def fast():
             from . import _fastcall, build
             if _fastcall.built_for() != build.built_for():
                 raise ImportError("built for %s" % _fastcall.built_for())
-            _fastcall.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in SIGNATURES})
+            _fastcall.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in list(SIGNATURES) + ["ab200_kv8_attention_workspace_bytes"]})
             _fast = _fastcall
         except ImportError as e:
             import warnings

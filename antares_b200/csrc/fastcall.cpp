@@ -31,6 +31,16 @@ typedef int (*AttendAtFn)(const void *, const void *, const void *, void *, int,
 typedef int (*EltwiseFn)(const void *, const void *, int, const void *, int, const void *, const void *, int, void *, int, size_t, void *);
 typedef int (*RowFn)(const void *, const void *, const void *, const void *, int, const void *, int, const void *, const void *, int, const void *, const void *,
                      int, void *, int, int, int, void *);
+typedef int (*Kv8AppendFn)(void *, void *, void *, void *, int, int, int, const void *, long, int, const void *, const void *, int, int, const void *, const void *, long,
+                           long, const void *, long, void *, long, int, const void *, int, void *);
+typedef int (*Kv8ReadFn)(const void *, const void *, const void *, const void *, int, int, int, const void *, long, int, const void *, const void *, int, int, void *, void *,
+                         int, void *);
+typedef int (*Kv8AttendFn)(const void *, long, void *, const void *, const void *, const void *, const void *, int, int, int, const void *, long, int, const void *,
+                           const void *, int, int, int, int, int, float, int, void *, size_t, void *);
+typedef int (*Kv8StepFn)(const void *, const void *, const void *, long, long, long, void *, void *, void *, void *, void *, int, int, int, const void *, long, int,
+                         const void *, int, int, int, int, const void *, float, int, void *, size_t, void *);
+typedef size_t (*Kv8BytesFn)(int, int, int, int, int);
+typedef int (*CopyPagesFn)(int, void *const *, const int *, const long *, const long *, const long *, int, const int32_t *, const int32_t *, int, void *);
 struct Entries {
   GemvFn gemv, gemm;
   SigmoidFn sigmoid;
@@ -42,6 +52,12 @@ struct Entries {
   AttendAtFn attend_at;
   EltwiseFn eltwise;
   RowFn row;
+  Kv8AppendFn kv8_append;
+  Kv8ReadFn kv8_read;
+  Kv8AttendFn kv8_attend;
+  Kv8StepFn kv8_step;
+  Kv8BytesFn kv8_bytes;
+  CopyPagesFn copy_pages;
 } E;
 
 #define NOT_HERE Py_RETURN_NONE
@@ -356,6 +372,235 @@ PyObject *py_run(PyObject *, PyObject *const *a, Py_ssize_t n) {
   })
 }
 
+// ---- the 8-bit paged cache ---------------------------------------------------------------------------------------------
+constexpr int64_t KV8_D = 128;
+
+// A plain tensor on the current GPU, of any strides; else nullptr.
+inline const Tensor *plain_strided(PyObject *o, int device) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const Tensor &t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.get_device() != device || !t.has_storage()) return nullptr;
+  constexpr c10::DispatchKeySet odd({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                     c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+  return t.key_set().has_any(odd) ? nullptr : &t;
+}
+// [rows, heads, 128] with the heads of a row together; *stride: from row to row
+inline bool rows3(const Tensor &t, at::ScalarType type, int64_t rows, int64_t heads, long *stride) {
+  if (t.dim() != 3 || t.scalar_type() != type || t.size(2) != KV8_D || t.size(0) != rows || (heads >= 0 && t.size(1) != heads) || t.numel() <= 0) return false;
+  if (t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != KV8_D)) return false;
+  *stride = t.size(0) > 1 ? t.stride(0) : t.size(1) * KV8_D;
+  return true;
+}
+
+struct Kv8Call {
+  void *k, *v, *ks, *vs;
+  int pages, page_rows, heads, max_pages, S;
+  long table_stride;
+  const void *table, *pos0, *cu;
+};
+// the cache (a tuple or list of four), page table, positions and offsets (or None) of a call
+bool kv8_call(PyObject *cache, PyObject *table, PyObject *pos0, PyObject *cu, int device, Kv8Call *c) {
+  if (!PyTuple_Check(cache) && !PyList_Check(cache)) return false;
+  if (PySequence_Fast_GET_SIZE(cache) != 4) return false;
+  const Tensor *t[4], *tab, *pos, *off = nullptr;
+  for (int i = 0; i < 4; ++i)
+    if (!(t[i] = plain_strided(PySequence_Fast_GET_ITEM(cache, i), device)) || !t[i]->is_contiguous()) return false;
+  const Tensor &k = *t[0], &s = *t[2];
+  if (k.dim() != 4 || k.scalar_type() != at::kChar || t[1]->scalar_type() != at::kChar || t[1]->sizes() != k.sizes() || k.size(3) != KV8_D) return false;
+  const int64_t rows = k.size(2);
+  if (rows < 16 || (rows & (rows - 1)) || s.dim() != 3 || s.scalar_type() != at::kFloat || t[3]->scalar_type() != at::kFloat || t[3]->sizes() != s.sizes() ||
+      s.size(0) != k.size(0) || s.size(1) != k.size(1) || s.size(2) != rows / 16)
+    return false;
+  if (!(tab = plain_strided(table, device)) || tab->dim() != 2 || tab->scalar_type() != at::kInt || (tab->size(1) > 1 && tab->stride(1) != 1)) return false;
+  const int64_t S = tab->size(0);
+  if (S <= 0 || !(pos = plain_strided(pos0, device)) || !pos->is_contiguous() || pos->scalar_type() != at::kInt || pos->numel() != S) return false;
+  if (cu != Py_None && (!(off = plain_strided(cu, device)) || !off->is_contiguous() || off->scalar_type() != at::kInt || off->numel() != S + 1)) return false;
+  if (k.size(0) > INT32_MAX || k.size(1) > INT32_MAX || rows > INT32_MAX || tab->size(1) > INT32_MAX || S > INT32_MAX) return false;
+  *c = Kv8Call{k.data_ptr(), t[1]->data_ptr(), s.data_ptr(), t[3]->data_ptr(), (int)k.size(0), (int)rows, (int)k.size(1), (int)tab->size(1), (int)S,
+               std::max<long>(tab->stride(0), tab->size(1)), tab->data_ptr(), pos->data_ptr(), off ? off->data_ptr() : nullptr};
+  return true;
+}
+inline int current_device() { return c10::cuda::current_device(); }
+inline bool float_arg(PyObject *o, float none, float *f) {
+  if (o == Py_None) *f = none;
+  else if (PyFloat_Check(o)) *f = (float)PyFloat_AS_DOUBLE(o);
+  else return false;
+  return true;
+}
+inline const Tensor *inv_freq_arg(PyObject *o, int device) {
+  const Tensor *f = plain_strided(o, device);
+  return f && f->is_contiguous() && f->scalar_type() == at::kFloat && f->numel() >= KV8_D / 2 ? f : nullptr;
+}
+inline Tensor rows_like(const Tensor &x, bool zero) {
+  const auto o = at::TensorOptions().dtype(x.scalar_type()).device(x.device());
+  return zero ? at::zeros(x.sizes(), o) : at::empty(x.sizes(), o);
+}
+
+// kv8_attention(q, cache, page_table, pos0, cu_rows, max_rows, scale)
+PyObject *py_kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  GUARDED({
+    const int device = current_device();
+    const Tensor *q;
+    Kv8Call c;
+    long stride, most;
+    float scale;
+    if (n != 7 || !(q = plain_strided(a[0], device)) || q->dim() != 3 || !kv8_call(a[1], a[2], a[3], a[4], device, &c)) NOT_HERE;
+    const int code = code_of(*q);
+    const int64_t T = q->size(0), hq = q->size(1);
+    if (code < 0 || !rows3(*q, q->scalar_type(), T, -1, &stride) || hq % c.heads || T > INT32_MAX || hq > INT32_MAX || (!c.cu && T % c.S)) NOT_HERE;
+    if (!float_arg(a[6], 0.08838834764831845f, &scale)) NOT_HERE;
+    if (a[5] == Py_None) most = c.cu ? T : T / c.S;
+    else if (PyLong_CheckExact(a[5])) most = PyLong_AsLong(a[5]);
+    else NOT_HERE;
+    if (most < 0 || most > INT32_MAX) {
+      PyErr_Clear();
+      NOT_HERE;
+    }
+    Tensor out = rows_like(*q, c.cu != nullptr);
+    const size_t bytes = E.kv8_bytes(c.S, (int)T, (int)most, (int)hq, c.heads);
+    Tensor ws = fresh({(int64_t)bytes}, at::kByte, *q);
+    const void *qp = q->data_ptr();
+    void *op = out.data_ptr(), *wp = ws.data_ptr(), *st = stream();
+    if (enter([&] {
+          return E.kv8_attend(qp, stride, op, c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, (int)most,
+                              (int)hq, (int)KV8_D, scale, code, wp, bytes, st);
+        }))
+      NOT_HERE;
+    return THPVariable_Wrap(std::move(out));
+  })
+}
+
+// kv8_step(q, k, v, cache, page_table, pos0, inv_freq, scale)
+PyObject *py_kv8_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  GUARDED({
+    const int device = current_device();
+    const Tensor *q, *k, *v, *f = nullptr;
+    Kv8Call c;
+    long qs, ks, vs;
+    float scale;
+    if (n != 8 || !(q = plain_strided(a[0], device)) || !(k = plain_strided(a[1], device)) || !(v = plain_strided(a[2], device)) || q->dim() != 3) NOT_HERE;
+    if (!kv8_call(a[3], a[4], a[5], Py_None, device, &c) || (a[6] != Py_None && !(f = inv_freq_arg(a[6], device)))) NOT_HERE;
+    const int code = code_of(*q);
+    const int64_t T = q->size(0), hq = q->size(1);
+    if (code < 0 || !rows3(*q, q->scalar_type(), T, -1, &qs) || !rows3(*k, q->scalar_type(), T, c.heads, &ks) || !rows3(*v, q->scalar_type(), T, c.heads, &vs)) NOT_HERE;
+    if (hq % c.heads || T > INT32_MAX || hq > INT32_MAX || T % c.S || !float_arg(a[7], 0.08838834764831845f, &scale)) NOT_HERE;
+    Tensor out = rows_like(*q, false);
+    const size_t bytes = E.kv8_bytes(c.S, (int)T, (int)(T / c.S), (int)hq, c.heads);
+    Tensor ws = fresh({(int64_t)bytes}, at::kByte, *q);
+    const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr(), *fp = f ? f->data_ptr() : nullptr;
+    void *op = out.data_ptr(), *wp = ws.data_ptr(), *st = stream();
+    if (enter([&] {
+          return E.kv8_step(qp, kp, vp, qs, ks, vs, op, c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.S, (int)T, (int)hq,
+                            (int)KV8_D, fp, scale, code, wp, bytes, st);
+        }))
+      NOT_HERE;
+    return THPVariable_Wrap(std::move(out));
+  })
+}
+
+// kv8_append(cache, k, v, page_table, pos0, cu_rows, q, inv_freq): True, or the rotated queries
+PyObject *py_kv8_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  GUARDED({
+    const int device = current_device();
+    const Tensor *k, *v, *q = nullptr, *f = nullptr;
+    Kv8Call c;
+    long ks, vs, qs = 0;
+    if (n != 8 || !(k = plain_strided(a[1], device)) || !(v = plain_strided(a[2], device)) || k->dim() != 3 || !kv8_call(a[0], a[3], a[4], a[5], device, &c)) NOT_HERE;
+    if ((a[6] != Py_None && !(q = plain_strided(a[6], device))) || (a[7] != Py_None && !(f = inv_freq_arg(a[7], device))) || (q && !f)) NOT_HERE;
+    const int code = code_of(*k);
+    const int64_t T = k->size(0);
+    if (code < 0 || !rows3(*k, k->scalar_type(), T, c.heads, &ks) || !rows3(*v, k->scalar_type(), T, c.heads, &vs) || (q && !rows3(*q, k->scalar_type(), T, -1, &qs))) NOT_HERE;
+    if (T > INT32_MAX || (!c.cu && T % c.S) || (q && q->size(1) > INT32_MAX)) NOT_HERE;
+    Tensor out;
+    if (q) out = rows_like(*q, c.cu != nullptr);
+    const void *kp = k->data_ptr(), *vp = v->data_ptr(), *qp = q ? q->data_ptr() : nullptr, *fp = f ? f->data_ptr() : nullptr;
+    void *op = q ? out.data_ptr() : nullptr, *st = stream();
+    const int hq = q ? (int)q->size(1) : 0;
+    if (enter([&] {
+          return E.kv8_append(c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, kp, vp, ks, vs, qp, qs, op,
+                              hq * (long)KV8_D, hq, fp, code, st);
+        }))
+      NOT_HERE;
+    if (!q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(out));
+  })
+}
+
+// kv8_read(cache, page_table, pos0, rows, cu_rows, type code): (k, v)
+PyObject *py_kv8_read(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  GUARDED({
+    const int device = current_device();
+    Kv8Call c;
+    if (n != 6 || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[5]) || !kv8_call(a[0], a[1], a[2], a[4], device, &c)) NOT_HERE;
+    const long T = PyLong_AsLong(a[3]), code = PyLong_AsLong(a[5]);
+    if (PyErr_Occurred() || T <= 0 || T > INT32_MAX || code < 0 || code > 1 || (!c.cu && T % c.S)) {
+      PyErr_Clear();
+      NOT_HERE;
+    }
+    const auto o = at::TensorOptions().dtype(code ? at::kFloat : at::kHalf).device(at::Device(at::kCUDA, (c10::DeviceIndex)device));
+    Tensor out[2];
+    for (Tensor &t : out) t = c.cu ? at::zeros({T, c.heads, KV8_D}, o) : at::empty({T, c.heads, KV8_D}, o);
+    void *kp = out[0].data_ptr(), *vp = out[1].data_ptr(), *st = stream();
+    if (enter([&] {
+          return E.kv8_read(c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, kp, vp, (int)code, st);
+        }))
+      NOT_HERE;
+    PyObject *pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    for (int i = 0; i < 2; ++i) {
+      PyObject *t = THPVariable_Wrap(std::move(out[i]));
+      if (!t) {
+        Py_DECREF(pair);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(pair, i, t);
+    }
+    return pair;
+  })
+}
+
+// kv_copy_pages(buffers, src, dst): True
+PyObject *py_kv_copy_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  GUARDED({
+    const int device = current_device();
+    if (n != 3 || (!PyTuple_Check(a[0]) && !PyList_Check(a[0])) || (!PyTuple_Check(a[1]) && !PyList_Check(a[1])) || (!PyTuple_Check(a[2]) && !PyList_Check(a[2]))) NOT_HERE;
+    const Py_ssize_t buffers = PySequence_Fast_GET_SIZE(a[0]), pairs = PySequence_Fast_GET_SIZE(a[1]);
+    if (buffers < 1 || buffers > 8 || pairs != PySequence_Fast_GET_SIZE(a[2]) || pairs > INT32_MAX) NOT_HERE;
+    void *base[8];
+    int layers[8];
+    long ls[8], ps[8], size[8];
+    int64_t pages = 0;
+    for (Py_ssize_t b = 0; b < buffers; ++b) {
+      const Tensor *t = plain_strided(PySequence_Fast_GET_ITEM(a[0], b), device);
+      if (!t || t->dim() < 3 || t->numel() <= 0 || t->size(0) > INT32_MAX || (b && t->size(1) != pages)) NOT_HERE;
+      pages = t->size(1);
+      int64_t elements = 1;  // a page's lie together
+      for (int64_t d = t->dim() - 1; d >= 2; --d) {
+        if (t->size(d) > 1 && t->stride(d) != elements) NOT_HERE;
+        elements *= t->size(d);
+      }
+      const long e = (long)t->element_size();
+      base[b] = t->data_ptr(), layers[b] = (int)t->size(0), size[b] = elements * e;
+      ls[b] = t->size(0) > 1 ? t->stride(0) * e : 0, ps[b] = pages > 1 ? t->stride(1) * e : size[b];
+    }
+    if (pages > INT32_MAX) NOT_HERE;
+    std::vector<int32_t> list(2 * pairs);
+    for (int which = 0; which < 2; ++which)
+      for (Py_ssize_t i = 0; i < pairs; ++i) {
+        PyObject *o = PySequence_Fast_GET_ITEM(a[1 + which], i);
+        const long v = PyLong_CheckExact(o) ? PyLong_AsLong(o) : -1;
+        if (v < 0 || v >= pages) {
+          PyErr_Clear();
+          NOT_HERE;
+        }
+        list[which * pairs + i] = (int32_t)v;
+      }
+    void *st = stream();
+    if (enter([&] { return E.copy_pages((int)buffers, base, layers, ls, ps, size, (int)pages, list.data(), list.data() + pairs, (int)pairs, st); })) NOT_HERE;
+    Py_RETURN_TRUE;
+  })
+}
+
 // bind({name: address})
 PyObject *py_bind(PyObject *, PyObject *d) {
   auto get = [&](const char *name, auto &slot) {
@@ -366,7 +611,9 @@ PyObject *py_bind(PyObject *, PyObject *d) {
   };
   if (!PyDict_Check(d) || !get("ab200_w4a16_gemv", E.gemv) || !get("ab200_w4a16_gemm", E.gemm) || !get("ab200_sigmoid", E.sigmoid) || !get("ab200_softmax", E.softmax) ||
       !get("ab200_rmsnorm", E.rmsnorm) || !get("ab200_rmsnorm_vsum", E.rmsnorm_vsum) || !get("ab200_rope", E.rope) || !get("ab200_rope_at", E.rope_at) ||
-      !get("ab200_attention_decode_at", E.attend_at) || !get("ab200_eltwise_vm", E.eltwise) || !get("ab200_rowreduce_vm", E.row))
+      !get("ab200_attention_decode_at", E.attend_at) || !get("ab200_eltwise_vm", E.eltwise) || !get("ab200_rowreduce_vm", E.row) || !get("ab200_kv8_append", E.kv8_append) ||
+      !get("ab200_kv8_read", E.kv8_read) || !get("ab200_kv8_attention", E.kv8_attend) || !get("ab200_kv8_step", E.kv8_step) ||
+      !get("ab200_kv8_attention_workspace_bytes", E.kv8_bytes) || !get("ab200_kv_copy_pages", E.copy_pages))
     return PyErr_Format(PyExc_KeyError, "bind: an entry point is missing");
   Py_RETURN_NONE;
 }
@@ -387,6 +634,11 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          FAST(rope_at),
                          FAST(attend_at),
                          FAST(run),
+                         FAST(kv8_append),
+                         FAST(kv8_read),
+                         FAST(kv8_attention),
+                         FAST(kv8_step),
+                         FAST(kv_copy_pages),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -34,6 +34,7 @@ struct DecodeParams {
   float scale;               // times log2(e)
   const float *inv_freq;     // rotate the queries, or nullptr
   int few;                   // sequences with more rows than this (rows x group) are another kernel's
+  int beside;                // that kernel is the one before in the stream: this one runs beside it and only ends after it
   float *partial;            // [CTAs][2][rows][128], then [CTAs][2][rows][2]: maximum, sum
   int4 *split;               // [CTAs]: what is begun in CTA c and ended in a later one: CTAs, first row, kv head | rows - 1 << 16 |
                              // rows with nothing to attend to << 20, first packed row
@@ -146,7 +147,9 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j4 = lane & 3;
   const Kv8Rows &r = p.r;
   pdl_launch_dependents();
-  pdl_wait();
+  // The prompt kernel releases its dependents after its own wait: whatever came before it is complete by then, and what it
+  // writes is not read here.  What comes after this kernel waits for it, so it waits for the prompt kernel before it ends.
+  if (!p.beside) pdl_wait();
 
   // ---- this CTA's share: w0 .. w1 - 1 of all work, ordered by sequence, kv head, tile, block
   long total = 0, start = 0, weight = 0;
@@ -158,7 +161,10 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
   const long per = max((long)kd_div(total + gridDim.x - 1, gridDim.x), (long)KD_LEAST);
   const long w0 = blockIdx.x * per, w1 = min(w0 + per, total);
   if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if (w0 >= w1) return;
+  if (w0 >= w1) {
+    if (p.beside) pdl_wait();
+    return;
+  }
   if (r.S > KD_THREADS) total = 0;
   for (int base = 0;;) {
     if (r.S > KD_THREADS) {
@@ -532,6 +538,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       p.split[blockIdx.x] = make_int4((int)kd_div(done.item + KD_ITEM + done.blocks - 1, per) - (int)blockIdx.x + 1, done.row0,
                                       done.hk | (done.last - done.first) << 16 | empty << 20, done.first);
   }
+  if (p.beside) pdl_wait();
 }
 
 // Joins the parts of the items that several CTAs share.  A CTA has one row of the items begun in eight CTAs of the first
@@ -638,7 +645,7 @@ static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const vo
     const int rc = kv8_prefill(Kv8PrefillParams{c, r, q, q_stride, out, Hq, group, scale2, KD_FEW, nullptr, nullptr, status, 0, 0, 1}, dtype, stream);
     if (rc || !r.cu) return rc;
   }
-  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, prompts ? KD_FEW : 0x7fffffff, (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
+  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, prompts ? KD_FEW : 0x7fffffff, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
   if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8>(p, d, stream) : decode_launch<float, 16>(p, d, stream);
   return d.rows == 8 ? decode_launch<__half, 8>(p, d, stream) : decode_launch<__half, 16>(p, d, stream);
 }
@@ -686,6 +693,8 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   int rc = kv8_check("kv8_step", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_step", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc || S == 0 || T == 0) return rc;
+  const size_t need = decode_plan(S, T, T / S, Hq, Hkv).bytes;
+  AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
   rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
                         nullptr, 0, nullptr, 0, 0, inv_freq, dtype, stream);
   if (rc) return rc;

@@ -374,6 +374,10 @@ def _disjoint(out, name, *others):
 def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=None, q_out=None):
     """Writes rows k, v [T, kv heads, 128] into the cache; with inv_freq, k rotated by halves at its positions, and q [T, query
     heads, 128] too: returns the rotated queries (q_out, which may be q), else None."""
+    if q_out is None:
+        y = fast().kv8_append(cache, k, v, page_table, pos0, cu_rows, q, inv_freq)
+        if y is not None:
+            return None if q is None else y
     T = k.shape[0]
     if q_out is not None and q is None:
         raise ValueError("q_out without q")
@@ -405,6 +409,10 @@ def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=Non
 def kv8_read(cache, page_table, pos0, rows, cu_rows=None, dtype=torch.float16, out=None):
     """The values held at the rows' positions, (k, v) [rows, kv heads, 128] each; zeros outside the table.  out: a pair of
     tensors to write to, whose rows behind the last sequence's stay as they are (new tensors: zeros)."""
+    if out is None:
+        y = fast().kv8_read(cache, page_table, pos0, rows, cu_rows, _DT.get(dtype, -1))
+        if y is not None:
+            return y
     args = _kv8_args(cache, page_table, pos0, cu_rows, rows)
     if out is None:
         make = torch.empty if cu_rows is None and rows else torch.zeros
@@ -441,6 +449,10 @@ def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale
     (kv8_append); kv head = query head // (query heads / kv heads).  Rows with no position to attend to are zeros, and so are
     rows behind the last sequence's in a new result (in `out` they stay as they are).  max_rows: the most rows of a sequence,
     a hint.  out may be q where q is contiguous."""
+    if out is None and workspace is None:
+        y = fast().kv8_attention(q, cache, page_table, pos0, cu_rows, max_rows, scale)
+        if y is not None:
+            return y
     T, hq = q.shape[0], q.shape[1]
     args = _kv8_args(cache, page_table, pos0, cu_rows, T, q)
     qp, q_stride = _rows3(q, "q", q.dtype)
@@ -467,6 +479,10 @@ def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale
 def kv8_step(q, k, v, cache, page_table, pos0, inv_freq=None, scale=None, out=None, workspace=None):
     """A decode step's kv8_append and kv8_attention in one call: q [T, query heads, 128], k, v [T, kv heads, 128], T / S rows of
     each sequence, rotated if inv_freq is given."""
+    if out is None and workspace is None:
+        y = fast().kv8_step(q, k, v, cache, page_table, pos0, inv_freq, scale)
+        if y is not None:
+            return y
     T, hq = q.shape[0], q.shape[1]
     args = _kv8_args(cache, page_table, pos0, None, T, q)
     qp, q_stride = _rows3(q, "q", q.dtype)
@@ -502,6 +518,8 @@ def kv_copy_pages(buffers, src, dst):
     """Copies the pages src[i] to dst[i] (host integers) inside every buffer [layers, pages, ...]: caches of any type, all in
     one launch.  A page's elements lie together.  No destination may occur twice or be a source too."""
     import ctypes
+    if fast().kv_copy_pages(buffers, src, dst) is not None:
+        return
     if len(src) != len(dst):
         raise ValueError("%d sources and %d destinations" % (len(src), len(dst)))
     buffers = list(buffers)
