@@ -85,9 +85,9 @@ SIGNATURES = {
     "ab200_module_info": [_i, _vp, _vp, _vp, _i],
     "ab200_module_tensor": [_i, _i, _vp, _i, _vp, _i, _vp, _vp],
     "ab200_forward_host_ns": [_i, _vp, _i, _vp, _i, _vp],
-    "ab200_kv8_append": [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _vp, _vp, _l, _l, _vp, _l, _vp, _l, _i, _vp, _i, _vp],
-    "ab200_kv8_read": [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp],
-    "ab200_kv8_attention": [_vp, _l, _vp] + [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp],
+    "ab200_kv8_append": [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _vp, _vp, _l, _l, _vp, _l, _vp, _l, _i, _vp, _i, _i, _vp],
+    "ab200_kv8_read": [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _vp],
+    "ab200_kv8_attention": [_vp, _l, _vp] + [_vp] * 4 + [_i] * 3 + [_vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _sz, _vp],
     "ab200_kv8_step": [_vp] * 3 + [_l] * 3 + [_vp] * 5 + [_i] * 3 + [_vp, _l, _i, _vp, _i, _i, _i, _i, _vp, _f, _i, _vp, _sz, _vp],
     "ab200_kv_copy_pages": [_i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp],
     "ab200_greedy_next": [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp],

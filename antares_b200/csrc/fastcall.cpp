@@ -32,11 +32,11 @@ typedef int (*EltwiseFn)(const void *, const void *, int, const void *, int, con
 typedef int (*RowFn)(const void *, const void *, const void *, const void *, int, const void *, int, const void *, const void *, int, const void *, const void *,
                      int, void *, int, int, int, void *);
 typedef int (*Kv8AppendFn)(void *, void *, void *, void *, int, int, int, const void *, long, int, const void *, const void *, int, int, const void *, const void *, long,
-                           long, const void *, long, void *, long, int, const void *, int, void *);
+                           long, const void *, long, void *, long, int, const void *, int, int, void *);
 typedef int (*Kv8ReadFn)(const void *, const void *, const void *, const void *, int, int, int, const void *, long, int, const void *, const void *, int, int, void *, void *,
-                         int, void *);
+                         int, int, void *);
 typedef int (*Kv8AttendFn)(const void *, long, void *, const void *, const void *, const void *, const void *, int, int, int, const void *, long, int, const void *,
-                           const void *, int, int, int, int, int, float, int, void *, size_t, void *);
+                           const void *, int, int, int, int, int, float, int, int, void *, size_t, void *);
 typedef int (*Kv8StepFn)(const void *, const void *, const void *, long, long, long, void *, void *, void *, void *, void *, int, int, int, const void *, long, int,
                          const void *, int, int, int, int, const void *, float, int, void *, size_t, void *);
 typedef size_t (*Kv8BytesFn)(int, int, int, int, int);
@@ -431,10 +431,7 @@ inline const Tensor *inv_freq_arg(PyObject *o, int device) {
   const Tensor *f = plain_strided(o, device);
   return f && f->is_contiguous() && f->scalar_type() == at::kFloat && f->numel() >= KV8_D / 2 ? f : nullptr;
 }
-inline Tensor rows_like(const Tensor &x, bool zero) {
-  const auto o = at::TensorOptions().dtype(x.scalar_type()).device(x.device());
-  return zero ? at::zeros(x.sizes(), o) : at::empty(x.sizes(), o);
-}
+inline Tensor rows_like(const Tensor &x) { return at::empty(x.sizes(), at::TensorOptions().dtype(x.scalar_type()).device(x.device())); }
 
 // kv8_attention(q, cache, page_table, pos0, cu_rows, max_rows, scale)
 PyObject *py_kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -456,14 +453,14 @@ PyObject *py_kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
       PyErr_Clear();
       NOT_HERE;
     }
-    Tensor out = rows_like(*q, c.cu != nullptr);
+    Tensor out = rows_like(*q);
     const size_t bytes = E.kv8_bytes(c.S, (int)T, (int)most, (int)hq, c.heads);
     Tensor ws = fresh({(int64_t)bytes}, at::kByte, *q);
     const void *qp = q->data_ptr();
     void *op = out.data_ptr(), *wp = ws.data_ptr(), *st = stream();
     if (enter([&] {
           return E.kv8_attend(qp, stride, op, c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, (int)most,
-                              (int)hq, (int)KV8_D, scale, code, wp, bytes, st);
+                              (int)hq, (int)KV8_D, scale, 1, code, wp, bytes, st);
         }))
       NOT_HERE;
     return THPVariable_Wrap(std::move(out));
@@ -484,7 +481,7 @@ PyObject *py_kv8_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int64_t T = q->size(0), hq = q->size(1);
     if (code < 0 || !rows3(*q, q->scalar_type(), T, -1, &qs) || !rows3(*k, q->scalar_type(), T, c.heads, &ks) || !rows3(*v, q->scalar_type(), T, c.heads, &vs)) NOT_HERE;
     if (hq % c.heads || T > INT32_MAX || hq > INT32_MAX || T % c.S || !float_arg(a[7], 0.08838834764831845f, &scale)) NOT_HERE;
-    Tensor out = rows_like(*q, false);
+    Tensor out = rows_like(*q);
     const size_t bytes = E.kv8_bytes(c.S, (int)T, (int)(T / c.S), (int)hq, c.heads);
     Tensor ws = fresh({(int64_t)bytes}, at::kByte, *q);
     const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr(), *fp = f ? f->data_ptr() : nullptr;
@@ -512,13 +509,13 @@ PyObject *py_kv8_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (code < 0 || !rows3(*k, k->scalar_type(), T, c.heads, &ks) || !rows3(*v, k->scalar_type(), T, c.heads, &vs) || (q && !rows3(*q, k->scalar_type(), T, -1, &qs))) NOT_HERE;
     if (T > INT32_MAX || (!c.cu && T % c.S) || (q && q->size(1) > INT32_MAX)) NOT_HERE;
     Tensor out;
-    if (q) out = rows_like(*q, c.cu != nullptr);
+    if (q) out = rows_like(*q);
     const void *kp = k->data_ptr(), *vp = v->data_ptr(), *qp = q ? q->data_ptr() : nullptr, *fp = f ? f->data_ptr() : nullptr;
     void *op = q ? out.data_ptr() : nullptr, *st = stream();
     const int hq = q ? (int)q->size(1) : 0;
     if (enter([&] {
           return E.kv8_append(c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, kp, vp, ks, vs, qp, qs, op,
-                              hq * (long)KV8_D, hq, fp, code, st);
+                              hq * (long)KV8_D, hq, fp, 1, code, st);
         }))
       NOT_HERE;
     if (!q) Py_RETURN_TRUE;
@@ -539,10 +536,10 @@ PyObject *py_kv8_read(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     const auto o = at::TensorOptions().dtype(code ? at::kFloat : at::kHalf).device(at::Device(at::kCUDA, (c10::DeviceIndex)device));
     Tensor out[2];
-    for (Tensor &t : out) t = c.cu ? at::zeros({T, c.heads, KV8_D}, o) : at::empty({T, c.heads, KV8_D}, o);
+    for (Tensor &t : out) t = at::empty({T, c.heads, KV8_D}, o);
     void *kp = out[0].data_ptr(), *vp = out[1].data_ptr(), *st = stream();
     if (enter([&] {
-          return E.kv8_read(c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, kp, vp, (int)code, st);
+          return E.kv8_read(c.k, c.v, c.ks, c.vs, c.pages, c.page_rows, c.heads, c.table, c.table_stride, c.max_pages, c.pos0, c.cu, c.S, (int)T, kp, vp, 1, (int)code, st);
         }))
       NOT_HERE;
     PyObject *pair = PyTuple_New(2);

@@ -6,13 +6,15 @@
 
 namespace ab200 {
 
-constexpr int KA_THREADS = 128, KA_HEADS = 4, KA_Q_HEADS = 8;
+constexpr int KA_WARPS = 8, KA_THREADS = KA_WARPS * 32, KA_HEADS = KA_WARPS / 2, KA_Q_HEADS = 8;
 constexpr float KA_LEAST_SCALE = 0x1p-100f;  // below it a block is held as zeros: quotients stay clear of subnormal arithmetic
+constexpr float KA_MAGIC = 12582912.f;       // 1.5 * 2^23: a number of less than 2^22 added to it is rounded to an integer, in the low bits
 
 // The code of x at scale s: the quotient x / s rounded to the nearest, ties to even, as if it had all its digits.  `inv` is
 // about 1 / s, so k is off by one at most; the two sums (each one rounding, so their signs are exact) say which side of the
 // middle between two codes x lies on.
-__device__ __forceinline__ int kv8_code(float x, float s, float inv) {
+__device__ __noinline__ int kv8_code(float x, float s, float inv) {
+  if (s == 0.f) return 0;
   if (!(fabsf(x) < CUDART_INF_F)) return x > 0.f ? 127 : x < 0.f ? -127 : 0;
   float k = rintf(x * inv);
   const float up = fmaf(-(k + 0.5f), s, x), down = fmaf(-(k - 0.5f), s, x);
@@ -21,11 +23,25 @@ __device__ __forceinline__ int kv8_code(float x, float s, float inv) {
   else if (down < 0.f || (down == 0.f && odd)) k -= 1.f;
   return (int)fminf(fmaxf(k, -127.f), 127.f);
 }
-__device__ __forceinline__ uint32_t kv8_code4(const float (&x)[8], int at, float s, float inv) {
-  uint32_t w = 0;
+// Eight of them, as two words.  What is left of x behind k s says whether k can be wrong: only next to half a step, where
+// the slow way decides.  (In full for each value it was most of the kernel's instructions.)
+__device__ __forceinline__ uint2 kv8_codes(const float (&x)[8], float s, float inv, bool finite) {
+  float far = 0.f;
+  uint32_t t[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w |= (uint32_t)(kv8_code(x[at + i], s, inv) & 255) << (8 * i);
-  return s == 0.f ? 0u : w;
+  for (int i = 0; i < 8; ++i) {
+    const float k = fmaf(x[i], inv, KA_MAGIC);
+    t[i] = __float_as_uint(k);
+    far = fmaxf(far, fabsf(fmaf(-(k - KA_MAGIC), s, x[i])));
+  }
+  if (!finite || s == 0.f || far > 0.49999f * s) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (uint32_t)kv8_code(x[i], s, inv);
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) w[h] = __byte_perm(__byte_perm(t[4 * h], t[4 * h + 1], 0x0040), __byte_perm(t[4 * h + 2], t[4 * h + 3], 0x0040), 0x5410);
+  return make_uint2(w[0], w[1]);
 }
 
 // dims 4 sub .. 4 sub + 3 and 64 + the same of a row: a rotated pair is one thread's
@@ -81,10 +97,24 @@ struct AppendParams {
   long k_stride, v_stride, q_stride, q_out_stride;
   int Hq;
   const float *inv_freq;
+  int zero_rest;
   int slots_per_seq;  // cu == nullptr
   int kv_groups;
   int *status;
 };
+
+// Whose the rows row0 .. row0 + n - 1 are (-1: nobody's), to shared memory.
+template <int N, int THREADS>
+__device__ __forceinline__ void kv8_rows_of(const Kv8Rows &r, int row0, int (&row_seq)[N]) {
+  const int tid = threadIdx.x;
+  if (tid < N) row_seq[tid] = r.cu || row0 + tid >= r.T ? -1 : (row0 + tid) / r.n;
+  __syncthreads();
+  if (r.cu) {
+    for (int s = tid; s < r.S; s += THREADS)
+      for (int i = max(r.begin(s) - row0, 0), e = min(r.end(s) - row0, N); i < e; ++i) row_seq[i] = s;
+    __syncthreads();
+  }
+}
 
 // Grid: x = slot, y = group of KA_HEADS kv heads, then groups of KA_Q_HEADS query heads.
 // kv: a slot is a block of 16 positions that new rows of one sequence lie in.  Sequence s owns the slots from
@@ -92,10 +122,11 @@ struct AppendParams {
 // A warp takes a block of one head of K or of V: half a warp per row, 8 rows each, in registers: one pass for the largest
 // value, then the codes.  Older rows of the block are only read and written when its scale grows.
 // q: a slot is 16 consecutive rows.
+// Rows are asked for before the sines are made.
 template <typename T>
-__global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(AppendParams<T> p) {
+__global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(const __grid_constant__ AppendParams<T> p) {
   typedef typename KaAngle<T>::type A;
-  __shared__ A sn[KV8_BLOCK][KV8_D / 2], cs[KV8_BLOCK][KV8_D / 2];
+  __shared__ __align__(16) A sn[KV8_BLOCK][KV8_D / 2], cs[KV8_BLOCK][KV8_D / 2];
   __shared__ int seq_s, row_seq[KV8_BLOCK];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane & 15, hw = lane >> 4;
   const Kv8Rows &r = p.r;
@@ -105,27 +136,32 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(AppendParams<T> 
   if ((int)blockIdx.y >= p.kv_groups) {  // ---- rotate query rows
     const int row0 = blockIdx.x * KV8_BLOCK;
     if (row0 >= r.T) return;
-    if (tid < KV8_BLOCK) row_seq[tid] = r.cu ? -1 : min((row0 + tid) / max(r.n, 1), r.S - 1);
-    __syncthreads();
-    if (r.cu) {
-      for (int s = tid; s < r.S; s += KA_THREADS)
-        for (int i = max(r.begin(s) - row0, 0), e = min(r.end(s) - row0, KV8_BLOCK); i < e; ++i) row_seq[i] = s;
-      __syncthreads();
+    kv8_rows_of<KV8_BLOCK, KA_THREADS>(r, row0, row_seq);
+    const int h0 = ((int)blockIdx.y - p.kv_groups) * KA_Q_HEADS;
+    constexpr int EACH = KV8_BLOCK * KA_Q_HEADS / (KA_THREADS / 16);  // rows of heads that a half-warp has
+    float f[EACH][8];
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const int i = (tid >> 4) + n * (KA_THREADS / 16), row = i / KA_Q_HEADS, h = h0 + i % KA_Q_HEADS;
+      if (row0 + row < r.T && row_seq[row] >= 0 && h < p.Hq) ka_load(p.q + (size_t)(row0 + row) * p.q_stride + (size_t)h * KV8_D, sub, f[n]);
     }
     for (int i = tid; i < KV8_BLOCK * KV8_D / 2; i += KA_THREADS) {
       const int row = i >> 6, s = row_seq[row];
-      if (row0 + row >= r.T || s < 0) continue;
-      ka_sincos((float)(r.pos0[s] + row0 + row - r.begin(s)) * p.inv_freq[i & 63], &sn[row][i & 63], &cs[row][i & 63]);
+      if (s >= 0) ka_sincos((float)(r.pos0[s] + row0 + row - r.begin(s)) * p.inv_freq[i & 63], &sn[row][i & 63], &cs[row][i & 63]);
     }
     __syncthreads();
-    const int h0 = ((int)blockIdx.y - p.kv_groups) * KA_Q_HEADS;
-    for (int i = tid >> 4; i < KV8_BLOCK * KA_Q_HEADS; i += KA_THREADS / 16) {
-      const int row = i / KA_Q_HEADS, h = h0 + i % KA_Q_HEADS;
-      if (row0 + row >= r.T || row_seq[row] < 0 || h >= p.Hq) continue;
-      float f[8];
-      ka_load(p.q + (size_t)(row0 + row) * p.q_stride + (size_t)h * KV8_D, sub, f);
-      ka_turn(f, sn[row], cs[row], sub);
-      ka_store(p.q_out + (size_t)(row0 + row) * p.q_out_stride + (size_t)h * KV8_D, sub, f);
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const int i = (tid >> 4) + n * (KA_THREADS / 16), row = i / KA_Q_HEADS, h = h0 + i % KA_Q_HEADS;
+      if (row0 + row >= r.T || h >= p.Hq) continue;
+      T *out = p.q_out + (size_t)(row0 + row) * p.q_out_stride + (size_t)h * KV8_D;
+      if (row_seq[row] >= 0) {
+        ka_turn(f[n], sn[row], cs[row], sub);
+        ka_store(out, sub, f[n]);
+      } else if (p.zero_rest) {
+        const float none[8] = {};
+        ka_store(out, sub, none);
+      }
     }
     return;
   }
@@ -152,79 +188,84 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(AppendParams<T> 
   if (first > last || block > (last >> 4)) return;
   const int at = (int)(block << 4);  // the block's first position
   const int lo = (int)(max(first, (long)at) - at), hi = (int)(min(last, (long)at + 15) - at);  // its rows lo .. hi are new
+  const int h = blockIdx.y * KA_HEADS + (warp >> 1);
+  const bool is_v = warp & 1, turn = !is_v && p.inv_freq != nullptr;
+  float f[8][8];
+  if (h < p.c.H) {
+    const T *src = (is_v ? p.v : p.k) + (size_t)h * KV8_D;
+    const long stride = is_v ? p.v_stride : p.k_stride;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = 2 * j + hw;
+      if (i >= lo && i <= hi) ka_load(src + (size_t)(row0 + (at + i - pos0)) * stride, sub, f[j]);
+    }
+  }
   if (p.inv_freq) {
     for (int i = tid + lo * (KV8_D / 2); i < (hi + 1) * (KV8_D / 2); i += KA_THREADS)
       ka_sincos((float)(at + (i >> 6)) * p.inv_freq[i & 63], &sn[i >> 6][i & 63], &cs[i >> 6][i & 63]);
   }
-  __syncthreads();
   const long page = kv8_page(p.c, r, s, at, tid == 0 ? p.status : nullptr);
-  if (page < 0) return;
+  __syncthreads();
+  if (page < 0 || h >= p.c.H) return;
   const int in_page = at & ((1 << p.c.shift) - 1);
   const bool older = pos0 > at;  // rows before the new ones: they count for the scale
-  for (int item = warp; item < 2 * KA_HEADS; item += KA_THREADS / 32) {
-    const int h = blockIdx.y * KA_HEADS + (item >> 1);
-    const bool is_v = item & 1;
-    if (h >= p.c.H) break;
-    const T *src = (is_v ? p.v + (size_t)h * KV8_D : p.k + (size_t)h * KV8_D);
-    const long stride = is_v ? p.v_stride : p.k_stride;
-    const size_t at_head = (size_t)page * p.c.H + h;
-    int8_t *dst = (is_v ? p.c.v : p.c.k) + ((at_head << p.c.shift) + in_page) * KV8_D;
-    float *scale = (is_v ? p.c.vs : p.c.ks) + (at_head << (p.c.shift - 4)) + (in_page >> 4);
-    float f[8][8], most = 0.f;
+  const size_t at_head = (size_t)page * p.c.H + h;
+  int8_t *dst = (is_v ? p.c.v : p.c.k) + ((at_head << p.c.shift) + in_page) * KV8_D;
+  float *scale = (is_v ? p.c.vs : p.c.ks) + (at_head << (p.c.shift - 4)) + (in_page >> 4);
+  const float was = older ? *scale : 0.f;
+  float most = 0.f;
+  bool finite = true;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = 2 * j + hw;
-      if (i >= lo && i <= hi) {
-        ka_load(src + (size_t)(row0 + (at + i - pos0)) * stride, sub, f[j]);
-        if (!is_v && p.inv_freq) ka_turn(f[j], sn[i], cs[i], sub);
+  for (int j = 0; j < 8; ++j) {
+    const int i = 2 * j + hw;
+    if (i >= lo && i <= hi) {
+      if (turn) ka_turn(f[j], sn[i], cs[i], sub);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e]) < CUDART_INF_F ? fabsf(f[j][e]) : 0.f);
+      for (int e = 0; e < 8; ++e) {
+        const bool ok = fabsf(f[j][e]) < CUDART_INF_F;
+        most = fmaxf(most, ok ? fabsf(f[j][e]) : 0.f);
+        finite = finite && ok;
       }
     }
-    most = warp_max(most);
-    const float was = older ? *scale : 0.f;
-    float now = most * (1.f / 127.f);
-    now = now < KA_LEAST_SCALE ? 0.f : now;
-    now = fmaxf(was, now);
-    const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f;
-    __syncwarp();  // every lane has read the scale
-    if (lane == 0) *scale = now;
+  }
+  most = warp_max(most);
+  float now = most * (1.f / 127.f);
+  now = now < KA_LEAST_SCALE ? 0.f : now;
+  now = fmaxf(was, now);
+  const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f;
+  __syncwarp();  // every lane has read the scale
+  if (lane == 0) *scale = now;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = 2 * j + hw;
-      uint32_t *d = reinterpret_cast<uint32_t *>(dst + i * KV8_D) + sub;
-      if (i >= lo && i <= hi) {
-        d[0] = kv8_code4(f[j], 0, now, inv);
-        d[16] = kv8_code4(f[j], 4, now, inv);
-      } else if (i < lo && older && now > was) {  // the values they stood for, at the new scale
-        const uint32_t a = d[0], b = d[16];
+  for (int j = 0; j < 8; ++j) {
+    const int i = 2 * j + hw;
+    uint32_t *d = reinterpret_cast<uint32_t *>(dst + i * KV8_D) + sub;
+    const bool again = i < lo && older && now > was;
+    if (again) {  // the values they stood for, at the new scale
+      const uint32_t a = d[0], b = d[16];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[j][e] = (float)(int8_t)(a >> (8 * e)) * was, f[j][4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
-        d[0] = kv8_code4(f[j], 0, now, inv);
-        d[16] = kv8_code4(f[j], 4, now, inv);
-      }
+      for (int e = 0; e < 4; ++e) f[j][e] = (float)(int8_t)(a >> (8 * e)) * was, f[j][4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
+    }
+    if (again || (i >= lo && i <= hi)) {
+      const uint2 w = kv8_codes(f[j], now, inv, finite);
+      d[0] = w.x, d[16] = w.y;
     }
   }
 }
 
 // k_out, v_out [T][H][128] = the values at the rows' positions; a position outside the table reads as zeros.  A CTA takes
-// 16 rows; a thread 16 codes at a time.
+// 8 rows, a thread 16 bytes of the result of each, K and V: 16 loads on their way at once.
+constexpr int KR_ROWS = 8, KR_THREADS = 128;
 template <typename T>
-__global__ void __launch_bounds__(KA_THREADS) kv8_read_kernel(Kv8Cache c, Kv8Rows r, T *k_out, T *v_out, int *status) {
-  __shared__ int row_seq[KV8_BLOCK];
-  __shared__ long row_at[KV8_BLOCK];  // page * H, or -1
-  __shared__ int row_in[KV8_BLOCK];
-  const int tid = threadIdx.x, row0 = blockIdx.x * KV8_BLOCK;
+__global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(const __grid_constant__ Kv8Cache c, const __grid_constant__ Kv8Rows r, T *k_out, T *v_out, int zero_rest, int *status) {
+  constexpr int EACH = 16 / sizeof(T);  // codes that a thread has of a row
+  __shared__ int row_seq[KR_ROWS];
+  __shared__ long row_at[KR_ROWS];  // page * H, or -1
+  __shared__ int row_in[KR_ROWS];
+  const int tid = threadIdx.x, row0 = blockIdx.x * KR_ROWS;
   pdl_launch_dependents();
   pdl_wait();
-  if (tid < KV8_BLOCK) row_seq[tid] = r.cu || row0 + tid >= r.T ? -1 : (row0 + tid) / r.n;
-  __syncthreads();
-  if (r.cu) {
-    for (int s = tid; s < r.S; s += KA_THREADS)
-      for (int i = max(r.begin(s) - row0, 0), e = min(r.end(s) - row0, KV8_BLOCK); i < e; ++i) row_seq[i] = s;
-    __syncthreads();
-  }
-  if (tid < KV8_BLOCK) {
+  kv8_rows_of<KR_ROWS, KR_THREADS>(r, row0, row_seq);
+  if (tid < KR_ROWS) {
     const int s = row_seq[tid];
     long at = -1;
     if (s >= 0) {
@@ -238,42 +279,47 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_read_kernel(Kv8Cache c, Kv8Row
     row_at[tid] = at;
   }
   __syncthreads();
-  const int per_row = c.H * (KV8_D / 16), total = KV8_BLOCK * per_row;
-  for (int i = blockIdx.y * KA_THREADS + tid; i < total; i += gridDim.y * KA_THREADS) {
-    const int row = i / per_row, piece = i - row * per_row, h = piece >> 3;
-    if (row_seq[row] < 0) continue;
-    const long at = row_at[row];
+  const int per_row = c.H * (KV8_D / EACH), piece = blockIdx.y * KR_THREADS + tid;
+  if (piece >= per_row) return;
+  const int h = piece / (KV8_D / EACH), in_head = piece % (KV8_D / EACH) * EACH;
+  uint2 w[KR_ROWS][2];
+  float f[KR_ROWS][2];
+#pragma unroll
+  for (int i = 0; i < KR_ROWS; ++i) {
+    const long at = row_at[i];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      uint4 codes = make_uint4(0, 0, 0, 0);
-      float f = 0.f;
+      w[i][which] = make_uint2(0, 0), f[i][which] = 0.f;
       if (at >= 0) {
-        codes = ldg_stream_v4((which ? c.v : c.k) + (((at + h) << c.shift) + row_in[row]) * KV8_D + (piece & 7) * 16);
-        f = (which ? c.vs : c.ks)[((at + h) << (c.shift - 4)) + (row_in[row] >> 4)];
+        const int8_t *src = (which ? c.v : c.k) + (((at + h) << c.shift) + row_in[i]) * KV8_D + in_head;
+        if constexpr (EACH == 8) w[i][which] = ldg_nc_v2(src);
+        else w[i][which].x = __ldg(reinterpret_cast<const uint32_t *>(src));
+        f[i][which] = (which ? c.vs : c.ks)[((at + h) << (c.shift - 4)) + (row_in[i] >> 4)];
       }
-      T *out = (which ? v_out : k_out) + ((size_t)(row0 + row) * per_row + piece) * 16;
-      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-      float x[16];
+    }
+  }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * f;
-      if constexpr (sizeof(T) == 2) {
-        uint32_t u[8];
+  for (int i = 0; i < KR_ROWS; ++i) {
+    if (row0 + i >= r.T || (row_seq[i] < 0 && !zero_rest)) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = h22u(__floats2half2_rn(x[2 * e], x[2 * e + 1]));
-        reinterpret_cast<uint4 *>(out)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-        reinterpret_cast<uint4 *>(out)[1] = make_uint4(u[4], u[5], u[6], u[7]);
-      } else {
+    for (int which = 0; which < 2; ++which) {
+      float x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) reinterpret_cast<float4 *>(out)[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-      }
+      for (int e = 0; e < EACH; ++e) x[e] = (float)(int8_t)((e < 4 ? w[i][which].x : w[i][which].y) >> (8 * (e & 3))) * f[i][which];
+      T *out = (which ? v_out : k_out) + ((size_t)(row0 + i) * per_row + piece) * EACH;
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint4 *>(out) = make_uint4(h22u(__floats2half2_rn(x[0], x[1])), h22u(__floats2half2_rn(x[2], x[3])), h22u(__floats2half2_rn(x[4], x[5])),
+                                                     h22u(__floats2half2_rn(x[6], x[7])));
+      else
+        *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
     }
   }
 }
 
 template <typename T>
 static int append_launch(const Kv8Cache &c, const Kv8Rows &r, const void *k, const void *v, long k_stride, long v_stride, const void *q, long q_stride, void *q_out,
-                         long q_out_stride, int Hq, const float *inv_freq, cudaStream_t stream) {
-  AppendParams<T> p{c, r, (const T *)k, (const T *)v, (const T *)q, (T *)q_out, k_stride, v_stride, q_stride, q_out_stride, Hq, inv_freq, (r.n + 14) / 16 + 1,
+                         long q_out_stride, int Hq, const float *inv_freq, int zero_rest, cudaStream_t stream) {
+  AppendParams<T> p{c, r, (const T *)k, (const T *)v, (const T *)q, (T *)q_out, k_stride, v_stride, q_stride, q_out_stride, Hq, inv_freq, zero_rest, (r.n + 14) / 16 + 1,
                     (c.H + KA_HEADS - 1) / KA_HEADS, kernel_error_ptr()};
   const long slots = r.cu ? (long)r.T / 16 + 2l * r.S : (long)r.S * p.slots_per_seq;
   const int q_groups = q ? (Hq + KA_Q_HEADS - 1) / KA_Q_HEADS : 0;
@@ -283,11 +329,11 @@ static int append_launch(const Kv8Cache &c, const Kv8Rows &r, const void *k, con
 }
 
 template <typename T>
-static int read_launch(const Kv8Cache &c, const Kv8Rows &r, void *k_out, void *v_out, cudaStream_t stream) {
-  const int chunks = (r.T + KV8_BLOCK - 1) / KV8_BLOCK, pieces = KV8_BLOCK * c.H * (KV8_D / 16);
-  int y = (pieces + KA_THREADS * 4 - 1) / (KA_THREADS * 4);  // four pieces of K and of V a thread
-  if (y > 65535) y = 65535;
-  AB200_CUDA(launch_pdl(kv8_read_kernel<T>, dim3(chunks, y), dim3(KA_THREADS), 0, stream, c, r, (T *)k_out, (T *)v_out, kernel_error_ptr()));
+static int read_launch(const Kv8Cache &c, const Kv8Rows &r, void *k_out, void *v_out, int zero_rest, cudaStream_t stream) {
+  const int chunks = (r.T + KR_ROWS - 1) / KR_ROWS, pieces = c.H * (KV8_D * (int)sizeof(T) / 16);
+  AB200_REQUIRE((pieces + KR_THREADS - 1) / KR_THREADS <= 65535, "kv8_read: %d heads are beyond the built limits", c.H);
+  AB200_CUDA(launch_pdl(kv8_read_kernel<T>, dim3(chunks, (pieces + KR_THREADS - 1) / KR_THREADS), dim3(KR_THREADS), 0, stream, c, r, (T *)k_out, (T *)v_out, zero_rest,
+                        kernel_error_ptr()));
   return AB200_OK;
 }
 
@@ -297,8 +343,8 @@ using namespace ab200;
 
 extern "C" int ab200_kv8_append(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int pages, int page_rows, int Hkv, const int32_t *page_table,
                                 long table_stride, int max_pages, const int32_t *pos0_dev, const int32_t *cu_rows_dev, int S, int T, const void *k, const void *v,
-                                long k_stride, long v_stride, const void *q, long q_stride, void *q_out, long q_out_stride, int Hq, const float *inv_freq, int dtype,
-                                void *stream) {
+                                long k_stride, long v_stride, const void *q, long q_stride, void *q_out, long q_out_stride, int Hq, const float *inv_freq, int zero_rest,
+                                int dtype, void *stream) {
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
@@ -315,13 +361,13 @@ extern "C" int ab200_kv8_append(void *k_cache, void *v_cache, float *k_scale, fl
     AB200_REQUIRE(Hq > 0 && Hq <= 65535 && q_stride % vec == 0 && q_out_stride % vec == 0 && q_stride >= (long)Hq * KV8_D && q_out_stride >= (long)Hq * KV8_D && aligned16(q) &&
                       aligned16(q_out), "kv8_append: q and q_out must be 16-byte aligned rows of at least %d values, a multiple of 16 bytes apart", Hq * KV8_D);
   }
-  if (dtype == AB200_F16) return append_launch<__half>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, (cudaStream_t)stream);
-  return append_launch<float>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, (cudaStream_t)stream);
+  if (dtype == AB200_F16) return append_launch<__half>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, zero_rest, (cudaStream_t)stream);
+  return append_launch<float>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, zero_rest, (cudaStream_t)stream);
 }
 
 extern "C" int ab200_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages, int page_rows, int Hkv,
                               const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev, const int32_t *cu_rows_dev, int S, int T, void *k_out,
-                              void *v_out, int dtype, void *stream) {
+                              void *v_out, int zero_rest, int dtype, void *stream) {
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
@@ -330,6 +376,6 @@ extern "C" int ab200_kv8_read(const void *k_cache, const void *v_cache, const fl
   AB200_REQUIRE(dtype == AB200_F16 || dtype == AB200_F32, "kv8_read: unknown dtype %d", dtype);
   if (S == 0 || T == 0) return AB200_OK;
   AB200_REQUIRE(k_out && v_out && aligned16(k_out) && aligned16(v_out), "kv8_read: k_out and v_out must be 16-byte aligned");
-  if (dtype == AB200_F16) return read_launch<__half>(c, r, k_out, v_out, (cudaStream_t)stream);
-  return read_launch<float>(c, r, k_out, v_out, (cudaStream_t)stream);
+  if (dtype == AB200_F16) return read_launch<__half>(c, r, k_out, v_out, zero_rest, (cudaStream_t)stream);
+  return read_launch<float>(c, r, k_out, v_out, zero_rest, (cudaStream_t)stream);
 }

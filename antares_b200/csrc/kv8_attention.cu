@@ -33,6 +33,7 @@ struct DecodeParams {
   int Hq, group;
   float scale;               // times log2(e)
   const float *inv_freq;     // rotate the queries, or nullptr
+  int zero_rest;             // rows behind the last sequence's become zeros
   int few;                   // sequences with more rows than this (rows x group) are another kernel's
   int beside;                // that kernel is the one before in the stream: this one runs beside it and only ends after it
   float *partial;            // [CTAs][2][rows][128], then [CTAs][2][rows][2]: maximum, sum
@@ -150,6 +151,12 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
   // The prompt kernel releases its dependents after its own wait: whatever came before it is complete by then, and what it
   // writes is not read here.  What comes after this kernel waits for it, so it waits for the prompt kernel before it ends.
   if (!p.beside) pdl_wait();
+
+  if (p.zero_rest) {
+    const long row16 = (long)p.Hq * KV8_D * sizeof(T) / 16;
+    for (long i = r.end(r.S - 1) * row16 + (long)blockIdx.x * KD_THREADS + tid; i < r.T * row16; i += (long)gridDim.x * KD_THREADS)
+      reinterpret_cast<uint4 *>(p.out)[i] = make_uint4(0, 0, 0, 0);
+  }
 
   // ---- this CTA's share: w0 .. w1 - 1 of all work, ordered by sequence, kv head, tile, block
   long total = 0, start = 0, weight = 0;
@@ -631,7 +638,7 @@ static int decode_launch(const DecodeParams &p, const DecodePlan &d, cudaStream_
 // Sequences of up to KD_FEW packed rows go through the kernel above, longer ones through the prompt kernel.
 constexpr int KD_FEW = 64;
 static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, int D, float scale, int dtype,
-                  const float *inv_freq, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+                  const float *inv_freq, int zero_rest, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (r.T == 0 || r.S == 0) return AB200_OK;
   const DecodePlan d = decode_plan(r.S, r.T, max_rows, Hq, c.H);
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= d.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, d.bytes, workspace_bytes);
@@ -645,7 +652,7 @@ static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const vo
     const int rc = kv8_prefill(Kv8PrefillParams{c, r, q, q_stride, out, Hq, group, scale2, KD_FEW, nullptr, nullptr, status, 0, 0, 1}, dtype, stream);
     if (rc || !r.cu) return rc;
   }
-  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, prompts ? KD_FEW : 0x7fffffff, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
+  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, zero_rest && r.cu, prompts ? KD_FEW : 0x7fffffff, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
   if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8>(p, d, stream) : decode_launch<float, 16>(p, d, stream);
   return d.rows == 8 ? decode_launch<__half, 8>(p, d, stream) : decode_launch<__half, 16>(p, d, stream);
 }
@@ -673,14 +680,15 @@ extern "C" size_t ab200_kv8_attention_workspace_bytes(int S, int T, int max_rows
 
 extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages,
                                    int page_rows, int Hkv, const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev, const int32_t *cu_rows_dev,
-                                   int S, int T, int max_rows, int Hq, int D, float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+                                   int S, int T, int max_rows, int Hq, int D, float scale, int zero_rest, int dtype, void *workspace, size_t workspace_bytes,
+                                   void *stream) {
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
   int rc = kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_attention", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc) return rc;
-  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, D, scale, dtype, nullptr, workspace, workspace_bytes, (cudaStream_t)stream);
+  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, D, scale, dtype, nullptr, zero_rest, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long q_stride, long k_stride, long v_stride, void *out, void *k_cache, void *v_cache,
@@ -696,7 +704,7 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   const size_t need = decode_plan(S, T, T / S, Hq, Hkv).bytes;
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
   rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
-                        nullptr, 0, nullptr, 0, 0, inv_freq, dtype, stream);
+                        nullptr, 0, nullptr, 0, 0, inv_freq, 0, dtype, stream);
   if (rc) return rc;
-  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, D, scale, dtype, inv_freq, workspace, workspace_bytes, (cudaStream_t)stream);
+  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, D, scale, dtype, inv_freq, 0, workspace, workspace_bytes, (cudaStream_t)stream);
 }

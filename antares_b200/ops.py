@@ -391,18 +391,18 @@ def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=Non
         fp = _chk(inv_freq, "inv_freq", torch.float32)
         if inv_freq.numel() < 64:
             raise ValueError("inv_freq must hold 64 values")
-    qp = q_stride = qo = qo_stride = hq = 0
+    qp = q_stride = qo = qo_stride = hq = zero = 0
     if q is not None:
         qp, q_stride = _rows3(q, "q", k.dtype, T)
         hq = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if cu_rows is None else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+            zero, q_out = 1, torch.empty(q.shape, dtype=q.dtype, device=q.device)
         qo, qo_stride = _rows3(q_out, "q_out", k.dtype, T, hq)
     for t in (v, q, q_out, inv_freq):
         if t is not None and t.device != k.device:
             raise ValueError("the tensors of a kv8 call lie on one device")
     with torch.cuda.device(k.device):
-        call("ab200_kv8_append", *args, kp, vp, k_stride, v_stride, qp, q_stride, qo, qo_stride, hq, fp, _code(k.dtype), _stream())
+        call("ab200_kv8_append", *args, kp, vp, k_stride, v_stride, qp, q_stride, qo, qo_stride, hq, fp, zero, _code(k.dtype), _stream())
     return q_out
 
 
@@ -414,8 +414,9 @@ def kv8_read(cache, page_table, pos0, rows, cu_rows=None, dtype=torch.float16, o
         if y is not None:
             return y
     args = _kv8_args(cache, page_table, pos0, cu_rows, rows)
+    zero = out is None
     if out is None:
-        make = torch.empty if cu_rows is None and rows else torch.zeros
+        make = torch.empty if args[12] else torch.zeros
         out = tuple(make((rows, args[6], 128), dtype=dtype, device=cache[0].device) for _ in range(2))
     dtype = out[0].dtype
     for t in out:
@@ -423,7 +424,7 @@ def kv8_read(cache, page_table, pos0, rows, cu_rows=None, dtype=torch.float16, o
         if not t.is_contiguous() or t.device != cache[0].device:
             raise ValueError("out must be contiguous and on the cache's device")
     with torch.cuda.device(cache[0].device):
-        call("ab200_kv8_read", *args, out[0].data_ptr(), out[1].data_ptr(), _code(dtype), _stream())
+        call("ab200_kv8_read", *args, out[0].data_ptr(), out[1].data_ptr(), int(zero), _code(dtype), _stream())
     return out[0], out[1]
 
 
@@ -461,8 +462,9 @@ def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale
     S = args[12]
     if max_rows is None:
         max_rows = T if cu_rows is not None else (T // S if S else 0)
+    zero = out is None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if cu_rows is None and S else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        out = (torch.empty if S else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
     else:
         if out.shape != q.shape or out.device != q.device:
             raise ValueError("out must be %s on %s" % (tuple(q.shape), q.device))
@@ -472,7 +474,7 @@ def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale
     scale = 128 ** -0.5 if scale is None else scale
     with torch.cuda.device(q.device):
         ws, ws_bytes, held = _kv8_workspace(workspace, S, T, max_rows, hq, args[6], q.device)
-        call("ab200_kv8_attention", qp, q_stride, out.data_ptr(), *args, int(max_rows), hq, 128, float(scale), _code(q.dtype), ws, ws_bytes, _stream())
+        call("ab200_kv8_attention", qp, q_stride, out.data_ptr(), *args, int(max_rows), hq, 128, float(scale), int(zero), _code(q.dtype), ws, ws_bytes, _stream())
     return out
 
 

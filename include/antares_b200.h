@@ -436,7 +436,7 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
  * ab200_kernel_status.
  * The call's rows: T rows of S sequences, sequence s has rows cu_rows_dev[s] .. cu_rows_dev[s + 1] - 1 (int32 [S + 1];
  * NULL: T / S each) at the positions pos0_dev[s], pos0_dev[s] + 1, ... (int32 [S]).  Rows behind the last sequence's are
- * left as they were.  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the results; rows may be
+ * left as they were (zero_rest: become zeros).  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the results; rows may be
  * strided (in elements, a multiple of 16 bytes), the heads of a row lie together. */
 
 /* Writes the rows of k and v [T][Hkv][128] into the cache.  inv_freq (fp32, 64 values used; NULL: none) rotates k by halves
@@ -449,14 +449,14 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
 int ab200_kv8_append(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int pages, int page_rows, int Hkv,
                      const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev,
                      const int32_t *cu_rows_dev, int S, int T, const void *k, const void *v, long k_stride, long v_stride,
-                     const void *q, long q_stride, void *q_out, long q_out_stride, int Hq, const float *inv_freq, int dtype,
-                     void *stream);
+                     const void *q, long q_stride, void *q_out, long q_out_stride, int Hq, const float *inv_freq,
+                     int zero_rest, int dtype, void *stream);
 
 /* k_out, v_out [T][Hkv][128] = the values held at the rows' positions (zeros outside the table). */
 int ab200_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages,
                    int page_rows, int Hkv, const int32_t *page_table, long table_stride, int max_pages,
-                   const int32_t *pos0_dev, const int32_t *cu_rows_dev, int S, int T, void *k_out, void *v_out, int dtype,
-                   void *stream);
+                   const int32_t *pos0_dev, const int32_t *cu_rows_dev, int S, int T, void *k_out, void *v_out,
+                   int zero_rest, int dtype, void *stream);
 
 /* out [T][Hq][128]: row r of sequence s over the positions 0 .. pos0_dev[s] + r (those of the table), query head h over kv
  * head h / (Hq / Hkv); zeros where there is none.  The cache holds the call's own rows already (ab200_kv8_append).
@@ -466,8 +466,8 @@ int ab200_kv8_read(const void *k_cache, const void *v_cache, const float *k_scal
 int ab200_kv8_attention(const void *q, long q_stride, void *out, const void *k_cache, const void *v_cache,
                         const float *k_scale, const float *v_scale, int pages, int page_rows, int Hkv,
                         const int32_t *page_table, long table_stride, int max_pages, const int32_t *pos0_dev,
-                        const int32_t *cu_rows_dev, int S, int T, int max_rows, int Hq, int D, float scale, int dtype,
-                        void *workspace, size_t workspace_bytes, void *stream);
+                        const int32_t *cu_rows_dev, int S, int T, int max_rows, int Hq, int D, float scale,
+                        int zero_rest, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 size_t ab200_kv8_attention_workspace_bytes(int S, int T, int max_rows, int Hq, int Hkv);
 
 /* A decode step's ab200_kv8_append and ab200_kv8_attention in one call: T / S rows of each sequence.  q, k and v may be

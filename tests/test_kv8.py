@@ -21,13 +21,13 @@ ROWS = dict(table=4096, stride=4, max_pages=4, pos0=4096, cu=None, S=2, T=2)
 def _attention(q=4096, q_stride=512, out=4096, max_rows=1, Hq=4, D=128, dtype=0, **kw):
     a = {**CACHE, **ROWS, **kw}
     return _entry("ab200_kv8_attention", q, q_stride, out, a["k"], a["v"], a["ks"], a["vs"], a["pages"], a["page_rows"], a["H"], a["table"], a["stride"], a["max_pages"],
-                  a["pos0"], a["cu"], a["S"], a["T"], max_rows, Hq, D, 0.1, dtype, None, 0, None)
+                  a["pos0"], a["cu"], a["S"], a["T"], max_rows, Hq, D, 0.1, 0, dtype, None, 0, None)
 
 
 def _append(k=4096, v=4096, k_stride=256, v_stride=256, q=None, q_stride=0, q_out=None, qo_stride=0, Hq=0, freq=None, dtype=0, **kw):
     a = {**CACHE, **ROWS, **kw}
     return _entry("ab200_kv8_append", CACHE["k"], CACHE["v"], a["ks"], a["vs"], a["pages"], a["page_rows"], a["H"], a["table"], a["stride"], a["max_pages"], a["pos0"], a["cu"],
-                  a["S"], a["T"], k, v, k_stride, v_stride, q, q_stride, q_out, qo_stride, Hq, freq, dtype, None)
+                  a["S"], a["T"], k, v, k_stride, v_stride, q, q_stride, q_out, qo_stride, Hq, freq, 0, dtype, None)
 
 
 @pytest.mark.parametrize("change,code,word", [
