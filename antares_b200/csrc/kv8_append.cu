@@ -23,24 +23,44 @@ __device__ __noinline__ int kv8_code(float x, float s, float inv) {
   else if (down < 0.f || (down == 0.f && odd)) k -= 1.f;
   return (int)fminf(fmaxf(k, -127.f), 127.f);
 }
-// Eight of them, as two words.  What is left of x behind k s says whether k can be wrong: only next to half a step, where
-// the slow way decides.  (In full for each value it was most of the kernel's instructions.)
-__device__ __forceinline__ uint2 kv8_codes(const float (&x)[8], float s, float inv, bool finite) {
-  float far = 0.f;
-  uint32_t t[8];
+// Eight of them, as two words.  Where the quotients by a scale 2^-20 smaller and larger round alike, so does the exact one;
+// elsewhere, about once in 10000 values, the slow way decides.  (It was most of the kernel's instructions for every value.)
+__device__ __forceinline__ uint64_t ka_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void ka_round(const uint64_t (&x)[4], float inv, uint32_t (&w)[2]) {
+  const uint64_t f = ka_pair(inv, inv), magic = ka_pair(KA_MAGIC, KA_MAGIC);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float k = fmaf(x[i], inv, KA_MAGIC);
-    t[i] = __float_as_uint(k);
-    far = fmaxf(far, fabsf(fmaf(-(k - KA_MAGIC), s, x[i])));
+  for (int h = 0; h < 2; ++h) {
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint64_t r;
+      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x[2 * h + i]), "l"(f), "l"(magic));
+      asm("mov.b64 {%0, %1}, %2;" : "=r"(t[2 * i]), "=r"(t[2 * i + 1]) : "l"(r));
+    }
+    w[h] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
   }
-  if (!finite || s == 0.f || far > 0.49999f * s) {
+}
+__device__ __forceinline__ uint2 kv8_codes(const float (&x)[8], float s, float inv_less, float inv_more, bool slow) {
+  const uint64_t v[4] = {ka_pair(x[0], x[1]), ka_pair(x[2], x[3]), ka_pair(x[4], x[5]), ka_pair(x[6], x[7])};
+  uint32_t w[2], u[2];
+  ka_round(v, inv_less, w);
+  ka_round(v, inv_more, u);
+  if (slow || w[0] != u[0] || w[1] != u[1]) {
+    const float inv = s > 0.f ? __fdividef(1.f, s) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = (uint32_t)kv8_code(x[i], s, inv);
+    for (int h = 0; h < 2; ++h) {
+      w[h] = 0;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const float y = i == 0 ? x[4 * h] : i == 1 ? x[4 * h + 1] : i == 2 ? x[4 * h + 2] : x[4 * h + 3];
+        w[h] |= (uint32_t)(kv8_code(y, s, inv) & 255) << (8 * i);
+      }
+    }
   }
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) w[h] = __byte_perm(__byte_perm(t[4 * h], t[4 * h + 1], 0x0040), __byte_perm(t[4 * h + 2], t[4 * h + 3], 0x0040), 0x5410);
   return make_uint2(w[0], w[1]);
 }
 
@@ -78,11 +98,21 @@ template <> struct KaAngle<float> { typedef double type; };
 __device__ __forceinline__ void ka_sincos(float a, float *s, float *c) { sincosf(a, s, c); }
 __device__ __forceinline__ void ka_sincos(float a, double *s, double *c) { sincos((double)a, s, c); }
 
+__device__ __forceinline__ void ka_four(const float *p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4 *>(p);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+}
+__device__ __forceinline__ void ka_four(const double *p, double (&v)[4]) {
+  const double2 a = reinterpret_cast<const double2 *>(p)[0], b = reinterpret_cast<const double2 *>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
 template <typename A>
 __device__ __forceinline__ void ka_turn(float (&f)[8], const A *sn, const A *cs, int sub) {
+  A s4[4], c4[4];
+  ka_four(sn + 4 * sub, s4), ka_four(cs + 4 * sub, c4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const A s = sn[4 * sub + i], c = cs[4 * sub + i], x = f[i], y = f[4 + i];
+    const A s = s4[i], c = c4[i], x = f[i], y = f[4 + i];
     f[i] = (float)(x * c - y * s);
     f[4 + i] = (float)(y * c + x * s);
   }
@@ -124,7 +154,7 @@ __device__ __forceinline__ void kv8_rows_of(const Kv8Rows &r, int row0, int (&ro
 // q: a slot is 16 consecutive rows.
 // Rows are asked for before the sines are made.
 template <typename T>
-__global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(const __grid_constant__ AppendParams<T> p) {
+__global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 3 : 1) kv8_append_kernel(const __grid_constant__ AppendParams<T> p) {
   typedef typename KaAngle<T>::type A;
   __shared__ __align__(16) A sn[KV8_BLOCK][KV8_D / 2], cs[KV8_BLOCK][KV8_D / 2];
   __shared__ int seq_s, row_seq[KV8_BLOCK];
@@ -191,20 +221,29 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(const __grid_con
   const int h = blockIdx.y * KA_HEADS + (warp >> 1);
   const bool is_v = warp & 1, turn = !is_v && p.inv_freq != nullptr;
   float f[8][8];
+  const bool whole = lo == 0 && hi == 15;
   if (h < p.c.H) {
-    const T *src = (is_v ? p.v : p.k) + (size_t)h * KV8_D;
+    const T *src = (is_v ? p.v : p.k) + (size_t)h * KV8_D + (size_t)(row0 + (at - pos0)) * (is_v ? p.v_stride : p.k_stride);
     const long stride = is_v ? p.v_stride : p.k_stride;
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = 2 * j + hw;
-      if (i >= lo && i <= hi) ka_load(src + (size_t)(row0 + (at + i - pos0)) * stride, sub, f[j]);
+      for (int j = 0; j < 8; ++j) ka_load(src + (2 * j + hw) * stride, sub, f[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = 2 * j + hw;
+        if (i >= lo && i <= hi) ka_load(src + i * stride, sub, f[j]);
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[j][e] = 0.f;  // counts for nothing
+      }
     }
   }
+  const long page = kv8_page(p.c, r, s, at, tid == 0 ? p.status : nullptr);
   if (p.inv_freq) {
     for (int i = tid + lo * (KV8_D / 2); i < (hi + 1) * (KV8_D / 2); i += KA_THREADS)
       ka_sincos((float)(at + (i >> 6)) * p.inv_freq[i & 63], &sn[i >> 6][i & 63], &cs[i >> 6][i & 63]);
   }
-  const long page = kv8_page(p.c, r, s, at, tid == 0 ? p.status : nullptr);
   __syncthreads();
   if (page < 0 || h >= p.c.H) return;
   const int in_page = at & ((1 << p.c.shift) - 1);
@@ -213,28 +252,41 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(const __grid_con
   int8_t *dst = (is_v ? p.c.v : p.c.k) + ((at_head << p.c.shift) + in_page) * KV8_D;
   float *scale = (is_v ? p.c.vs : p.c.ks) + (at_head << (p.c.shift - 4)) + (in_page >> 4);
   const float was = older ? *scale : 0.f;
-  float most = 0.f;
-  bool finite = true;
+  if (turn) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = 2 * j + hw;
-    if (i >= lo && i <= hi) {
-      if (turn) ka_turn(f[j], sn[i], cs[i], sub);
+    for (int j = 0; j < 8; ++j)
+      if (whole || (2 * j + hw >= lo && 2 * j + hw <= hi)) ka_turn(f[j], sn[2 * j + hw], cs[2 * j + hw], sub);
+  }
+  float most = 0.f, odd = 0.f;  // the largest; not 0 if a value is not finite
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool ok = fabsf(f[j][e]) < CUDART_INF_F;
-        most = fmaxf(most, ok ? fabsf(f[j][e]) : 0.f);
-        finite = finite && ok;
-      }
-    }
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e])), odd = fmaf(f[j][e], 0.f, odd);
+  const bool finite = odd == 0.f;
+  if (!finite) {
+    most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e]) < CUDART_INF_F ? fabsf(f[j][e]) : 0.f);
   }
   most = warp_max(most);
   float now = most * (1.f / 127.f);
   now = now < KA_LEAST_SCALE ? 0.f : now;
   now = fmaxf(was, now);
-  const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f;
+  const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f, less = inv * (1.f - 0x1p-20f), more = inv * (1.f + 0x1p-20f);
+  const bool slow = !finite || now == 0.f;
   __syncwarp();  // every lane has read the scale
   if (lane == 0) *scale = now;
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t *d = reinterpret_cast<uint32_t *>(dst + (2 * j + hw) * KV8_D) + sub;
+      const uint2 w = kv8_codes(f[j], now, less, more, slow);
+      d[0] = w.x, d[16] = w.y;
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int i = 2 * j + hw;
@@ -246,7 +298,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_append_kernel(const __grid_con
       for (int e = 0; e < 4; ++e) f[j][e] = (float)(int8_t)(a >> (8 * e)) * was, f[j][4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
     }
     if (again || (i >= lo && i <= hi)) {
-      const uint2 w = kv8_codes(f[j], now, inv, finite);
+      const uint2 w = kv8_codes(f[j], now, less, more, slow);
       d[0] = w.x, d[16] = w.y;
     }
   }
