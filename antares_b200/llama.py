@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from . import packing
-from ._lib import call
+from ._lib import call, load
 
 
 @dataclass
@@ -140,10 +140,12 @@ class LlamaInt4Decoder:
     `comm` is None for world=1, otherwise an object with
       all_reduce_sum_(t_f32)  and  all_gather_into(out, t)   (see parallel.py).
     `weights` selects the checkpoint (gptq.GptqLlamaWeights); None = seeded synthetic weights.
+    `kv_bits` 8 keeps the cache in 8 bits with a scale for each 16 rows and head (ops.kv8_*): pages of kv_page_rows rows,
+    64 unless given.
     """
 
     def __init__(self, cfg, device, rank=0, world=1, comm=None, max_tokens=1024, prefetch=0, weights=None, tiled=True,
-                 fused_allreduce=True, kv_page_rows=0, kv_page_table=None):
+                 fused_allreduce=True, kv_page_rows=0, kv_page_table=None, kv_bits=16):
         assert cfg.dim % (world * cfg.group) == 0 and cfg.n_heads % world == 0 and cfg.vocab % world == 0
         self.cfg, self.dev, self.rank, self.world, self.comm = cfg, device, rank, world, comm
         self.hl = cfg.n_heads // world            # local heads
@@ -169,7 +171,12 @@ class LlamaInt4Decoder:
         z = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device=device)
         # KV cache: contiguous [layer, max_seq, dl], or paged: kv_page_rows (a power of two) rows per page and a
         # table logical page -> physical page (identity unless kv_page_table is given; the same table for every layer)
-        self.kv_page_rows = int(kv_page_rows)
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits must be 16 or 8, got %r" % (kv_bits,))
+        self.kv_bits = int(kv_bits)
+        self.kv_page_rows = int(kv_page_rows) or (64 if kv_bits == 8 else 0)
+        if kv_bits == 8 and (self.kv_page_rows < 16 or self.kv_page_rows & (self.kv_page_rows - 1)):
+            raise ValueError("an 8-bit cache's pages hold a power of two of rows, 16 or more; got %d" % self.kv_page_rows)
         self.page_table = None
         phys_rows = cfg.max_seq
         if self.kv_page_rows:
@@ -178,8 +185,14 @@ class LlamaInt4Decoder:
             assert table.shape == (n_pages,) and sorted(table.tolist()) == list(range(n_pages)), "kv_page_table must be a permutation of the pages"
             self.page_table = torch.from_numpy(table).to(device)
             phys_rows = n_pages * self.kv_page_rows
-        self.k_cache = z(cfg.n_layers, phys_rows, self.dl)
-        self.v_cache = z(cfg.n_layers, phys_rows, self.dl)
+        if kv_bits == 8:
+            pr = self.kv_page_rows
+            self.k_cache, self.v_cache = (z(cfg.n_layers, phys_rows // pr, self.hl, pr, cfg.head_dim, dt=torch.int8) for _ in range(2))
+            self.k_scale, self.v_scale = (z(cfg.n_layers, phys_rows // pr, self.hl, pr // 16, dt=torch.float32) for _ in range(2))
+            self._kv8_ws = z(load().ab200_kv8_attention_workspace_bytes(1, 1, 1, self.hl, self.hl), dt=torch.uint8)
+        else:
+            self.k_cache = z(cfg.n_layers, phys_rows, self.dl)
+            self.v_cache = z(cfg.n_layers, phys_rows, self.dl)
         self.x = z(cfg.dim, dt=torch.float32)
         self.xb = z(cfg.dim)
         self.vqk = z(3 * self.dl)
@@ -252,6 +265,12 @@ class LlamaInt4Decoder:
             call("ab200_residual_add", self.x.data_ptr(), self.partial.data_ptr(), self.cfg.dim, self._st)
             self._n += 1
 
+    def _kv8_cache(self, l):
+        """Layer l's cache and rows, as the ab200_kv8_* entry points take them (one sequence)."""
+        pages = self.page_table.numel()
+        return (self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(), self.k_scale[l].data_ptr(), self.v_scale[l].data_ptr(), pages, self.kv_page_rows, self.hl,
+                self.page_table.data_ptr(), pages, pages, self.pos.data_ptr())
+
     def step_eager(self):
         cfg = self.cfg
         self._st = torch.cuda.current_stream().cuda_stream
@@ -262,7 +281,12 @@ class LlamaInt4Decoder:
         self._n += 1
         for l, w in enumerate(self.layers):
             self._proj(self.x, w["vqk_q"], w["vqk_s"], self.vqk, 1, 0, w["att_norm"])        # RMSNorm + V|Q|K
-            if self.page_table is None:
+            if self.kv_bits == 8:
+                v, q, k = (self.vqk.data_ptr() + 2 * i * self.dl for i in range(3))
+                call("ab200_kv8_step", q, k, v, self.dl, self.dl, self.dl, self.att.data_ptr(), *self._kv8_cache(l), 1, 1, self.hl, cfg.head_dim,
+                     self.inv_freq.data_ptr(), self.att_scale, 0, self._kv8_ws.data_ptr(), self._kv8_ws.numel(), st)   # RoPE + cache, attention, join
+                self._n += 2
+            elif self.page_table is None:
                 call("ab200_attention_fused", self.vqk.data_ptr(), self.inv_freq.data_ptr(), self.pos.data_ptr(),
                      self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(), self.att.data_ptr(), self.hl, cfg.head_dim,
                      self.dl, cfg.max_seq, self.att_scale, st)                              # RoPE + cache + attention
@@ -343,8 +367,11 @@ class LlamaInt4Decoder:
     def _prefill_buffers(self, T):
         d, dl, f, dev = self.cfg.dim, self.dl, self.fl, self.dev
         h16 = lambda *shape: torch.empty(*shape, dtype=torch.float16, device=dev)
-        return dict(x=torch.empty(T, d, dtype=torch.float32, device=dev), xb=h16(T, d), vqk=h16(T, 3 * dl), q=h16(T, dl), att=h16(T, dl),
-                    o=h16(T, d), hh=h16(T, f))
+        b = dict(x=torch.empty(T, d, dtype=torch.float32, device=dev), xb=h16(T, d), vqk=h16(T, 3 * dl), q=h16(T, dl), att=h16(T, dl),
+                 o=h16(T, d), hh=h16(T, f))
+        if self.kv_bits == 8:
+            b["ws"] = torch.empty(load().ab200_kv8_attention_workspace_bytes(1, T, T, self.hl, self.hl), dtype=torch.uint8, device=dev)
+        return b
 
     def _prefill_pass(self, T, b):
         """The launches of one batched prompt pass on torch's current stream; reads self.prompt[:T], pos = 0."""
@@ -375,7 +402,13 @@ class LlamaInt4Decoder:
             call("ab200_rmsnorm", x.data_ptr(), 1, self.layers[0]["att_norm"].data_ptr(), xb.data_ptr(), T, d, cfg.eps, st)
         for l, w in enumerate(self.layers):
             gemm(xb, l, "vqk", vqk)
-            if self.page_table is None:
+            if self.kv_bits == 8:
+                vp, qp, kp = (vqk.data_ptr() + 2 * i * self.dl for i in range(3))
+                cache = self._kv8_cache(l)
+                call("ab200_kv8_append", *cache, 0, 1, T, kp, vp, 3 * self.dl, 3 * self.dl, qp, 3 * self.dl, q.data_ptr(), self.dl, self.hl, self.inv_freq.data_ptr(), 0, 0, st)
+                call("ab200_kv8_attention", q.data_ptr(), self.dl, att.data_ptr(), *cache, 0, 1, T, T, self.hl, cfg.head_dim, self.att_scale, 0, 0, b["ws"].data_ptr(),
+                     b["ws"].numel(), st)
+            elif self.page_table is None:
                 call("ab200_rope_kv_store_rows", vqk.data_ptr(), self.inv_freq.data_ptr(), self.pos.data_ptr(), q.data_ptr(),
                      self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(), T, self.hl, cfg.head_dim, self.dl, cfg.max_seq, st)
                 call("ab200_attention_prefill", q.data_ptr(), self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(), att.data_ptr(),
@@ -487,5 +520,6 @@ class LlamaInt4Decoder:
         def lin(K, N):
             return K * N // 2 + (K // g) * N * 2 + K * 2 + N * 2
         per_layer = lin(cfg.dim, 3 * self.dl) + lin(self.dl, cfg.dim) + lin(cfg.dim, 2 * self.fl) + lin(self.fl, cfg.dim)
-        per_layer += 2 * (pos + 1) * self.dl * 2  # K and V rows read by attention
+        # K and V rows read by attention: fp16, or codes and a scale for each 16 rows of a head
+        per_layer += 2 * (pos + 1) * self.dl * 2 if self.kv_bits == 16 else 2 * (pos + 1) * self.dl + 2 * ((pos + 16) // 16) * self.hl * 4
         return cfg.n_layers * per_layer + self.vl * cfg.dim * 2

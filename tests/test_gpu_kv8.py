@@ -433,3 +433,66 @@ def test_a_long_cache(cuda):
     back, _ = ops.kv8_read((k, v, ks, vs), table, _ints([past]), 1)
     assert torch.equal(back, (kk[-1:].float()).half())
     assert (back.float() - x.float()).abs().max() <= 0.5 * max(float(ks.max()), float(x.float().abs().max()) / 127) + 0.002
+
+
+def test_pages_of_many_sequences(cuda):
+    """The operators together, as a server uses them: prompts, decode steps, a fork, drafted tokens taken back, a request that
+    ends, compaction; every sequence's rows read back as they were written, attention as over a cache of its own."""
+    from antares_b200.kv_cache import PagedKV8Cache
+    L, H, HQ = 2, 2, 4
+    c = PagedKV8Cache(L, 24, H, page_rows=16, max_seqs=6, max_seq=128)
+    g = torch.Generator().manual_seed(0)
+    seen = {}   # sequence -> k, v rows of layer 1
+
+    def write(need):
+        c.reserve(need)
+        seqs = sorted(need)
+        table, pos0 = c.batch(seqs)
+        rows = [need[s] for s in seqs]
+        cu = _cu(rows)
+        for l in range(L):
+            k, v = (torch.randn(sum(rows), H, 128, generator=g).half().cuda() for _ in range(2))
+            ops.kv8_append(c.layer(l), k, v, table, pos0, cu_rows=cu)
+        at = 0
+        for s, n in zip(seqs, rows):
+            c.advance(s, n)
+            seen[s] = torch.cat([seen.get(s, torch.zeros(0, 2, H, 128).cuda()), torch.stack([k[at:at + n], v[at:at + n]], 1)])
+            at += n
+
+    def check():
+        seqs = sorted(seen)
+        table, pos0 = c.batch(seqs)
+        rows = [c.rows(s) for s in seqs]
+        assert rows == [len(seen[s]) for s in seqs]
+        k, v = ops.kv8_read(c.layer(1), table, torch.zeros_like(pos0), sum(rows), cu_rows=_cu(rows), dtype=F32)
+        at = 0
+        for s, n in zip(seqs, rows):
+            for i, got in enumerate((k, v)):
+                # a row is rounded once when it is written and again whenever its block's scale grows: half a step each, steps
+                # that grow; the last is the largest |value| of 16 rows over 127, below 4.6 / 127 here, and 16 rows bring few records
+                assert (got[at:at + n] - seen[s][:, i]).abs().max() <= 3 * 4.6 / 127
+            at += n
+        q = torch.randn(len(seqs), HQ, 128, generator=g).half().cuda()
+        got = ops.kv8_attention(q, c.layer(1), table, pos0 - 1)
+        _check_attention(got, _ref(c.layer(1), table), q, [r - 1 for r in rows], None, max(rows), F16)
+
+    a, b = c.add(), c.add()
+    write({a: 37, b: 5})
+    check()
+    d = c.fork(a)
+    seen[d] = seen[a].clone()
+    write({a: 1, b: 1, d: 1})
+    check()
+    write({d: 4})
+    c.truncate(d, c.rows(d) - 3)
+    seen[d] = seen[d][:-3]
+    check()
+    e = c.add()
+    write({e: 60, d: 20})
+    c.free(a)
+    del seen[a]
+    assert c.compact() > 0
+    check()
+    write({b: 30, d: 1, e: 1})
+    check()
+    assert ops.kernel_status() == 0
