@@ -12,6 +12,8 @@
 // fp16 numbers, 22 bits.
 #include <math_constants.h>
 
+#include <cooperative_groups.h>
+
 #include "kv8.cuh"
 #include "kv8_prefill.cuh"
 
@@ -35,6 +37,7 @@ struct DecodeParams {
   const float *inv_freq;     // rotate the queries, or nullptr
   int zero_rest;             // rows behind the last sequence's become zeros
   int few;                   // sequences with more rows than this (rows x group) are another kernel's
+  int splits, tiles;         // FIXED: CTAs of an item; tiles of a sequence's rows
   int beside;                // that kernel is the one before in the stream: this one runs beside it and only ends after it
   float *partial;            // [CTAs][2][rows][128], then [CTAs][2][rows][2]: maximum, sum
   int4 *split;               // [CTAs]: what is begun in CTA c and ended in a later one: CTAs, first row, kv head | rows - 1 << 16 |
@@ -134,7 +137,9 @@ __device__ __forceinline__ void kd_store4(__half *out, float4 v, float f) {
 // ROWS: packed query rows of a tile.  With 8, rows 8-15 of the tensor cores' tile carry second parts: the second byte of
 // q, the second half of P; with 16, each part is a product of its own.
 // A warp takes two blocks at a time: two independent chains of products and exponentials.
-template <typename T, int ROWS>
+// FIXED: an item is a cluster of p.splits CTAs, which take its blocks in equal shares and join them through each other's
+// shared memory: one launch, nothing to look up first.  Else every CTA takes an equal share of all work.
+template <typename T, int ROWS, bool FIXED>
 __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int NR = ROWS / 8;  // query rows a thread holds: lane / 4, and 8 more
@@ -159,33 +164,35 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
   }
 
   // ---- this CTA's share: w0 .. w1 - 1 of all work, ordered by sequence, kv head, tile, block
-  long total = 0, start = 0, weight = 0;
-  for (int base = 0; base < r.S; base += KD_THREADS) {
-    weight = base + tid < r.S ? kd_weight<ROWS>(p, base + tid) * p.c.H : 0;
-    const long before = total;
-    start = before + kd_scan(weight, scan_s, &total);
-  }
-  const long per = max((long)kd_div(total + gridDim.x - 1, gridDim.x), (long)KD_LEAST);
-  const long w0 = blockIdx.x * per, w1 = min(w0 + per, total);
-  if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if (w0 >= w1) {
-    if (p.beside) pdl_wait();
-    return;
-  }
-  if (r.S > KD_THREADS) total = 0;
-  for (int base = 0;;) {
-    if (r.S > KD_THREADS) {
+  long total = 0, start = 0, weight = 0, per = 1, w0 = 0, w1 = 0;
+  if constexpr (!FIXED) {
+    for (int base = 0; base < r.S; base += KD_THREADS) {
       weight = base + tid < r.S ? kd_weight<ROWS>(p, base + tid) * p.c.H : 0;
       const long before = total;
       start = before + kd_scan(weight, scan_s, &total);
     }
-    if (w0 >= start && w0 < start + weight) found_s = base + tid, found_start = start;
-    base += KD_THREADS;
-    if (total > w0 || base >= r.S) break;
+    per = max((long)kd_div(total + gridDim.x - 1, gridDim.x), (long)KD_LEAST);
+    w0 = blockIdx.x * per, w1 = min(w0 + per, total);
+    if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (w0 >= w1) {
+      if (p.beside) pdl_wait();
+      return;
+    }
+    if (r.S > KD_THREADS) total = 0;
+    for (int base = 0;;) {
+      if (r.S > KD_THREADS) {
+        weight = base + tid < r.S ? kd_weight<ROWS>(p, base + tid) * p.c.H : 0;
+        const long before = total;
+        start = before + kd_scan(weight, scan_s, &total);
+      }
+      if (w0 >= start && w0 < start + weight) found_s = base + tid, found_start = start;
+      base += KD_THREADS;
+      if (total > w0 || base >= r.S) break;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  int s = found_s;
-  start = found_start;
+  int s = FIXED ? 0 : found_s;
+  start = FIXED ? 0 : found_start;
   long w = w0;
   const long cap = (long)r.max_pages << p.c.shift;
   // the next item, or part of one, in the share
@@ -270,7 +277,17 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
     issue();
   };
 
-  bool more = next(it);
+  bool more = true;
+  if constexpr (FIXED) {
+    const int item = blockIdx.x / p.splits, z = blockIdx.x - item * p.splits, t = item % p.tiles, head = item / p.tiles;
+    it.hk = head % p.c.H, it.seq = head / p.c.H;
+    it.row0 = r.begin(it.seq), it.rows = (r.end(it.seq) - it.row0) * p.group, it.pos0 = r.pos0[it.seq];
+    it.first = t * ROWS, it.last = min(it.first + ROWS, it.rows) - 1;
+    it.blocks = kd_blocks<ROWS>(p, it.pos0, it.rows, t);
+    it.b0 = (int)((long)it.blocks * z / p.splits), it.b1 = (int)((long)it.blocks * (z + 1) / p.splits);
+  } else {
+    more = next(it);
+  }
   if (more) begin();
   while (more) {
     // ---- queries, meanwhile.  A warp takes the pieces warp and warp + 4 (a rotated pair is one thread's): thread's row(s),
@@ -491,7 +508,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
     // other half
     const Part done = it;
     const int empty = (int)max(0l, min((long)ROWS, -it.pos0 * p.group - it.first));  // leading rows with nothing to attend to
-    more = next(it);
+    more = FIXED ? false : next(it);
     __syncwarp();
     if (more) begin();
 #pragma unroll
@@ -510,7 +527,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       }
     }
     __syncthreads();
-    const bool whole = done.b0 == 0 && done.b1 == done.blocks;
+    const bool whole = FIXED ? p.splits == 1 : done.b0 == 0 && done.b1 == done.blocks;
     const int slot = done.b0 == 0 ? 1 : 0;
     constexpr int PER_ROW = KD_THREADS / ROWS, PIECES = KV8_D / 4 / PER_ROW;  // threads of a row, four dims at a time
     const int row = tid / PER_ROW, col = tid % PER_ROW * 4;
@@ -525,7 +542,8 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       }
       const int packed = done.first + row, token = packed / p.group, head = done.hk * p.group + packed - token * p.group;
       T *out = (T *)p.out + ((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + col;
-      float *part = p.partial + (((size_t)blockIdx.x * 2 + slot) * ROWS + row) * KV8_D + col;
+      // a part to be joined: FIXED into the ring's other half, else to memory
+      float *part = FIXED ? reinterpret_cast<float *>(smem) + row * KV8_D + col : p.partial + (((size_t)blockIdx.x * 2 + slot) * ROWS + row) * KV8_D + col;
       const float over = row < empty ? 0.f : 1.f / sum;
 #pragma unroll
       for (int c = 0; c < PIECES; ++c) {
@@ -538,10 +556,31 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
         if (whole) kd_store4(out + c * PER_ROW * 4, acc, over);
         else *reinterpret_cast<float4 *>(part + c * PER_ROW * 4) = acc;
       }
-      if (!whole && col == 0)
+      if (FIXED) {
+        if (col == 0) q_max_s[0][row] = mx, q_max_s[1][row] = sum;
+      } else if (!whole && col == 0)
         reinterpret_cast<float2 *>(p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D)[((size_t)blockIdx.x * 2 + slot) * ROWS + row] = make_float2(mx, sum);
     }
-    if (!whole && slot == 1 && tid == 0)  // begun here: the CTAs up to the one with the item's last block have the rest
+    if constexpr (FIXED) {
+      if (p.splits > 1) {
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const int z = (int)cluster.block_rank(), mine = ROWS / p.splits;  // a CTA joins its share of the rows, a thread a dim
+        for (int row = z * mine; row < (z + 1) * mine && row <= done.last - done.first; ++row) {
+          float mx = -CUDART_INF_F, sum = 0.f, acc = 0.f;
+          for (int i = 0; i < p.splits; ++i) mx = fmaxf(mx, *cluster.map_shared_rank(&q_max_s[0][row], i));
+          for (int i = 0; i < p.splits; ++i) {
+            const float m = *cluster.map_shared_rank(&q_max_s[0][row], i), f = m == -CUDART_INF_F ? 0.f : kd_ex2(m - mx);
+            sum = fmaf(*cluster.map_shared_rank(&q_max_s[1][row], i), f, sum);
+            acc = fmaf(*cluster.map_shared_rank(reinterpret_cast<float *>(smem) + row * KV8_D + tid, i), f, acc);
+          }
+          const int packed = done.first + row, token = packed / p.group, head = done.hk * p.group + packed - token * p.group;
+          ((T *)p.out)[((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + tid] = (T)(row < empty ? 0.f : acc / sum);
+        }
+        cluster.sync();  // nobody leaves while its memory is read
+      }
+    } else if (!whole && slot == 1 && tid == 0)  // begun here: the CTAs up to the one with the item's last block have the rest
       p.split[blockIdx.x] = make_int4((int)kd_div(done.item + KD_ITEM + done.blocks - 1, per) - (int)blockIdx.x + 1, done.row0,
                                       done.hk | (done.last - done.first) << 16 | empty << 20, done.first);
   }
@@ -613,24 +652,54 @@ __global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_const
 // ---- host --------------------------------------------------------------------------------------------------------
 struct DecodePlan {
   int rows, ctas;
+  int splits;  // > 0: an item to a cluster of this many CTAs; 0: equal shares and a second launch that joins them
+  int tiles;
   size_t partial_bytes, bytes;
 };
-static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv) {
+static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool uniform, long capacity) {
   DecodePlan d;
   const long group = Hq / Hkv;
   d.rows = (long)max_rows * group <= 8 ? 8 : 16;
   d.ctas = sm_count() * (d.rows == 8 ? 3 : 2);
   d.partial_bytes = (size_t)d.ctas * 2 * d.rows * (KV8_D + 2) * sizeof(float);
   d.bytes = d.partial_bytes + (size_t)d.ctas * sizeof(int4);
+  // One launch where no CTA then has KD_ITEM blocks more to do than its equal share would be if all sequences filled their
+  // pages; where they do not, it only takes less.
+  const long tiles = ((long)(T / S) * group + d.rows - 1) / d.rows, items = S * Hkv * tiles, blocks = (capacity + 15) / 16;
+  d.tiles = (int)tiles;
+  d.splits = 0;
+  if (uniform && items <= d.ctas) {
+    int c = 1;
+    while (c < 8 && items * c * 2 <= d.ctas) c *= 2;
+    if ((blocks + c - 1) / c <= items * blocks / d.ctas + 24) d.splits = c;
+  }
   return d;
 }
 
 template <typename T, int ROWS>
-static int decode_launch(const DecodeParams &p, const DecodePlan &d, cudaStream_t stream) {
+static int decode_launch(DecodeParams p, const DecodePlan &d, cudaStream_t stream) {
   constexpr int smem = KD_WARPS * KD_STAGES * KD_STAGE_BYTES;
-  static_assert(smem >= KD_WARPS * ROWS * KV8_D * (int)sizeof(float), "the warps' parts fit into the ring");
-  AB200_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<T, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  AB200_CUDA(launch_pdl(kv8_decode_kernel<T, ROWS>, dim3(d.ctas), dim3(KD_THREADS), smem, stream, p));
+  static_assert(KD_STAGES / 2 * KD_STAGE_BYTES >= ROWS * KV8_D * (int)sizeof(float), "a warp's part fits into half its ring");
+  if (d.splits > 0) {
+    p.splits = d.splits, p.tiles = d.tiles;
+    AB200_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<T, ROWS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long)p.r.S * p.c.H * d.tiles * d.splits));
+    cfg.blockDim = dim3(KD_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = d.splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    AB200_CUDA(cudaLaunchKernelEx(&cfg, kv8_decode_kernel<T, ROWS, true>, p));
+    return AB200_OK;
+  }
+  AB200_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<T, ROWS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  AB200_CUDA(launch_pdl(kv8_decode_kernel<T, ROWS, false>, dim3(d.ctas), dim3(KD_THREADS), smem, stream, p));
   AB200_CUDA(launch_pdl(kv8_join_kernel<T, ROWS>, dim3((d.ctas + KJ_WARPS - 1) / KJ_WARPS, ROWS), dim3(KJ_THREADS), 0, stream, p, d.ctas));
   return AB200_OK;
 }
@@ -640,7 +709,7 @@ constexpr int KD_FEW = 64;
 static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, int D, float scale, int dtype,
                   const float *inv_freq, int zero_rest, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (r.T == 0 || r.S == 0) return AB200_OK;
-  const DecodePlan d = decode_plan(r.S, r.T, max_rows, Hq, c.H);
+  const DecodePlan d = decode_plan(r.S, r.T, r.cu ? max_rows : r.n, Hq, c.H, r.cu == nullptr, (long)r.max_pages << c.shift);
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= d.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, d.bytes, workspace_bytes);
   const int group = Hq / c.H;
   int *status = kernel_error_ptr();
@@ -652,7 +721,7 @@ static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const vo
     const int rc = kv8_prefill(Kv8PrefillParams{c, r, q, q_stride, out, Hq, group, scale2, KD_FEW, nullptr, nullptr, status, 0, 0, 1}, dtype, stream);
     if (rc || !r.cu) return rc;
   }
-  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, zero_rest && r.cu, prompts ? KD_FEW : 0x7fffffff, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
+  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, zero_rest && r.cu, prompts ? KD_FEW : 0x7fffffff, 0, 0, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
   if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8>(p, d, stream) : decode_launch<float, 16>(p, d, stream);
   return d.rows == 8 ? decode_launch<__half, 8>(p, d, stream) : decode_launch<__half, 16>(p, d, stream);
 }
@@ -675,7 +744,7 @@ using namespace ab200;
 
 extern "C" size_t ab200_kv8_attention_workspace_bytes(int S, int T, int max_rows, int Hq, int Hkv) {
   if (S <= 0 || T <= 0 || Hkv <= 0 || Hq < Hkv) return 0;
-  return decode_plan(S, T, max_rows, Hq, Hkv).bytes;
+  return decode_plan(S, T, max_rows, Hq, Hkv, false, 0).bytes;
 }
 
 extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages,
@@ -701,7 +770,7 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   int rc = kv8_check("kv8_step", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_step", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc || S == 0 || T == 0) return rc;
-  const size_t need = decode_plan(S, T, T / S, Hq, Hkv).bytes;
+  const size_t need = decode_plan(S, T, T / S, Hq, Hkv, false, 0).bytes;
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
   rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
                         nullptr, 0, nullptr, 0, 0, inv_freq, 0, dtype, stream);
