@@ -16,6 +16,7 @@
 
 #include "kv8.cuh"
 #include "kv8_prefill.cuh"
+#include "kv8_quant.cuh"
 
 namespace ab200 {
 
@@ -35,6 +36,8 @@ struct DecodeParams {
   int Hq, group;
   float scale;               // times log2(e)
   const float *inv_freq;     // rotate the queries, or nullptr
+  const void *k_new, *v_new;  // this step's rows of keys and values, written first; nullptr: the cache holds them
+  long k_stride, v_stride;
   int zero_rest;             // rows behind the last sequence's become zeros
   int few;                   // sequences with more rows than this (rows x group) are another kernel's
   int splits, tiles;         // FIXED: CTAs of an item; tiles of a sequence's rows
@@ -132,6 +135,62 @@ __device__ __forceinline__ long kd_scan(long v, long (&s)[KD_WARPS], long *total
 __device__ __forceinline__ void kd_store4(float *out, float4 v, float f) { *reinterpret_cast<float4 *>(out) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 __device__ __forceinline__ void kd_store4(__half *out, float4 v, float f) {
   *reinterpret_cast<uint2 *>(out) = make_uint2(h22u(__floats2half2_rn(v.x * f, v.y * f)), h22u(__floats2half2_rn(v.z * f, v.w * f)));
+}
+
+// A decode step's new rows go into the cache here, block by block: a block is one CTA's, which writes it before it reads it.
+// One warp, one block of one head of K or V; rows lo .. hi of it are new (as in kv8_append.cu, which takes longer pieces).
+__device__ __noinline__ void kd_append(int8_t *dst, float *scale, const __half *src, long stride, int lo, int hi, bool older, int at, const float *inv_freq) {
+  const int lane = threadIdx.x & 31, sub = lane & 15, hw = lane >> 4;
+  float f[8][8], most = 0.f, odd = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = 2 * j + hw;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[j][e] = 0.f;
+    if (i < lo || i > hi) continue;
+    ka_load(src + (i - lo) * stride, sub, f[j]);
+    if (inv_freq) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float sn, cs;
+        sincosf((float)(at + i) * inv_freq[4 * sub + e], &sn, &cs);
+        ka_rotate(f[j][e], f[j][4 + e], sn, cs);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e])), odd = fmaf(f[j][e], 0.f, odd);
+  }
+  const bool finite = odd == 0.f;
+  if (!finite) {
+    most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e]) < CUDART_INF_F ? fabsf(f[j][e]) : 0.f);
+  }
+  most = warp_max(most);
+  const float was = older ? *scale : 0.f;
+  float now = most * (1.f / 127.f);
+  now = now < KA_LEAST_SCALE ? 0.f : now;
+  now = fmaxf(was, now);
+  const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f, less = inv * (1.f - 0x1p-20f), more = inv * (1.f + 0x1p-20f);
+  __syncwarp();  // every lane has read the scale
+  if (lane == 0) *scale = now;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = 2 * j + hw;
+    uint32_t *d = reinterpret_cast<uint32_t *>(dst + i * KV8_D) + sub;
+    const bool again = i < lo && older && now > was;
+    if (again) {  // the values they stood for, at the new scale
+      const uint32_t a = d[0], b = d[16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[j][e] = (float)(int8_t)(a >> (8 * e)) * was, f[j][4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
+    }
+    if (again || (i >= lo && i <= hi)) {
+      const uint2 w = kv8_codes(f[j], now, less, more, !finite || now == 0.f);
+      d[0] = w.x, d[16] = w.y;
+    }
+  }
 }
 
 // ROWS: packed query rows of a tile.  With 8, rows 8-15 of the tensor cores' tile carry second parts: the second byte of
@@ -271,6 +330,28 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   auto begin = [&]() {
+    if (FIXED && sizeof(T) == 2 && p.k_new) {
+      // positions that are stored, and the two blocks at most that they lie in; a warp has K or V of one of them
+      const long from = max(it.pos0, 0l), to = min(it.pos0 + it.rows / p.group, cap) - 1;
+      const int block = (int)(from >> 4) + (warp >> 1);
+      const bool here = from <= to && (int)(from >> 4) < it.b1 && (int)(to >> 4) >= it.b0;
+      if (here && block <= (int)(to >> 4) && block >= it.b0 && block < it.b1) {
+        const long page = kv8_page(p.c, r, it.seq, block << 4, p.status);
+        if (page >= 0) {
+          const int at = block << 4, in_page = at & ((1 << p.c.shift) - 1), lo = (int)(max(from, (long)at) - at), hi = (int)(min(to, (long)at + 15) - at);
+          const bool is_v = warp & 1;
+          const size_t head = (size_t)page * p.c.H + it.hk;
+          const long stride = is_v ? p.v_stride : p.k_stride;
+          kd_append((is_v ? p.c.v : p.c.k) + ((head << p.c.shift) + in_page) * KV8_D, (is_v ? p.c.vs : p.c.ks) + (head << (p.c.shift - 4)) + (in_page >> 4),
+                    (const __half *)(is_v ? p.v_new : p.k_new) + (size_t)(it.row0 + (at + lo - it.pos0)) * stride + (size_t)it.hk * KV8_D, stride, lo, hi, it.pos0 > at, at,
+                    is_v ? nullptr : p.inv_freq);
+        }
+      }
+      if (here) {
+        __threadfence();
+        __syncthreads();
+      }
+    }
     live = min(it.b1, (limit_of(it.last) + 15) >> 4);  // blocks that hold a key some row attends to
     pairs = max(0, ((live - it.b0 + 1) / 2 - warp + KD_WARPS - 1) / KD_WARPS);
     asked = 0, put = 0;
@@ -321,9 +402,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
         for (int e = 0; e < 4; ++e) {
           float sn, cs;
           sincosf(pos * p.inv_freq[16 * warp + 4 * j4 + e], &sn, &cs);
-          const float a = f[i][0][e], b = f[i][1][e];
-          f[i][0][e] = a * cs - b * sn;
-          f[i][1][e] = b * cs + a * sn;
+          ka_rotate(f[i][0][e], f[i][1][e], sn, cs);
         }
       }
       // a row that is not finite is made of NaN: its largest, as a bit pattern, is above that of every number
@@ -510,7 +589,6 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
     const int empty = (int)max(0l, min((long)ROWS, -it.pos0 * p.group - it.first));  // leading rows with nothing to attend to
     more = FIXED ? false : next(it);
     __syncwarp();
-    if (more) begin();
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
@@ -526,6 +604,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
         *reinterpret_cast<float4 *>(ring_mine + 2 * KD_STAGE_BYTES + ((8 * n + g) * KV8_D + 16 * c + 4 * j4) * 4) = v;
       }
     }
+    if (more) begin();
     __syncthreads();
     const bool whole = FIXED ? p.splits == 1 : done.b0 == 0 && done.b1 == done.blocks;
     const int slot = done.b0 == 0 ? 1 : 0;
@@ -663,15 +742,17 @@ static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool 
   d.ctas = sm_count() * (d.rows == 8 ? 3 : 2);
   d.partial_bytes = (size_t)d.ctas * 2 * d.rows * (KV8_D + 2) * sizeof(float);
   d.bytes = d.partial_bytes + (size_t)d.ctas * sizeof(int4);
-  // One launch where no CTA then has KD_ITEM blocks more to do than its equal share would be if all sequences filled their
-  // pages; where they do not, it only takes less.
+  // One launch where no CTA then has 24 blocks more to do than its equal share (what the lookups and the second launch take):
+  // one sequence as long as its pages allow, of several the longest so long and half as much in the mean.
+  // us, clusters / equal shares: one request of 384 positions and 32 heads 6.7 / 10.8; five of up to 1000 12.8 / 16.1;
+  // 16 times four rows of up to 3000 29 / 22.
   const long tiles = ((long)(T / S) * group + d.rows - 1) / d.rows, items = S * Hkv * tiles, blocks = (capacity + 15) / 16;
   d.tiles = (int)tiles;
   d.splits = 0;
   if (uniform && items <= d.ctas) {
     int c = 1;
     while (c < 8 && items * c * 2 <= d.ctas) c *= 2;
-    if ((blocks + c - 1) / c <= items * blocks / d.ctas + 24) d.splits = c;
+    if ((blocks + c - 1) / c <= items * blocks / (S == 1 ? 1 : 2) / d.ctas + 24) d.splits = c;
   }
   return d;
 }
@@ -706,8 +787,12 @@ static int decode_launch(DecodeParams p, const DecodePlan &d, cudaStream_t strea
 
 // Sequences of up to KD_FEW packed rows go through the kernel above, longer ones through the prompt kernel.
 constexpr int KD_FEW = 64;
+struct NewRows {
+  const void *k, *v;
+  long k_stride, v_stride;
+};
 static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, int D, float scale, int dtype,
-                  const float *inv_freq, int zero_rest, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+                  const float *inv_freq, NewRows new_rows, int zero_rest, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (r.T == 0 || r.S == 0) return AB200_OK;
   const DecodePlan d = decode_plan(r.S, r.T, r.cu ? max_rows : r.n, Hq, c.H, r.cu == nullptr, (long)r.max_pages << c.shift);
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= d.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, d.bytes, workspace_bytes);
@@ -721,7 +806,7 @@ static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const vo
     const int rc = kv8_prefill(Kv8PrefillParams{c, r, q, q_stride, out, Hq, group, scale2, KD_FEW, nullptr, nullptr, status, 0, 0, 1}, dtype, stream);
     if (rc || !r.cu) return rc;
   }
-  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, zero_rest && r.cu, prompts ? KD_FEW : 0x7fffffff, 0, 0, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
+  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, new_rows.k, new_rows.v, new_rows.k_stride, new_rows.v_stride, zero_rest && r.cu, prompts ? KD_FEW : 0x7fffffff, 0, 0, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
   if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8>(p, d, stream) : decode_launch<float, 16>(p, d, stream);
   return d.rows == 8 ? decode_launch<__half, 8>(p, d, stream) : decode_launch<__half, 16>(p, d, stream);
 }
@@ -757,7 +842,7 @@ extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, cons
   int rc = kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_attention", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc) return rc;
-  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, D, scale, dtype, nullptr, zero_rest, workspace, workspace_bytes, (cudaStream_t)stream);
+  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, D, scale, dtype, nullptr, NewRows{}, zero_rest, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long q_stride, long k_stride, long v_stride, void *out, void *k_cache, void *v_cache,
@@ -770,10 +855,21 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   int rc = kv8_check("kv8_step", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_step", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc || S == 0 || T == 0) return rc;
+  const long vec = dtype == AB200_F16 ? 8 : 4;
+  AB200_REQUIRE(k && v && k_stride % vec == 0 && v_stride % vec == 0 && k_stride >= (long)Hkv * KV8_D && v_stride >= (long)Hkv * KV8_D && aligned16(k) && aligned16(v),
+                "kv8_step: k and v must be 16-byte aligned rows of at least %d values, a multiple of 16 bytes apart", Hkv * KV8_D);
   const size_t need = decode_plan(S, T, T / S, Hq, Hkv, false, 0).bytes;
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
-  rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
-                        nullptr, 0, nullptr, 0, 0, inv_freq, 0, dtype, stream);
-  if (rc) return rc;
-  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, D, scale, dtype, inv_freq, 0, workspace, workspace_bytes, (cudaStream_t)stream);
+  // fp16 rows that fit into one tile are written by the attention kernel itself where an item is a cluster's; else by a launch
+  // before it: us, together / apart: one request of 384 positions and 32 heads 11.0 / 12.9, 48 ragged ones in equal shares
+  // 69 / 55 (each new block's 4 us then is one CTA's, and the others wait for it at the end)
+  const DecodePlan plan = decode_plan(S, T, T / S, Hq, Hkv, true, (long)max_pages * page_rows);
+  const bool together = dtype == AB200_F16 && plan.splits > 0 && plan.tiles == 1;
+  if (!together) {
+    rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
+                          nullptr, 0, nullptr, 0, 0, inv_freq, 0, dtype, stream);
+    if (rc) return rc;
+  }
+  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, D, scale, dtype, inv_freq, together ? NewRows{k, v, k_stride, v_stride} : NewRows{}, 0, workspace, workspace_bytes,
+                (cudaStream_t)stream);
 }
