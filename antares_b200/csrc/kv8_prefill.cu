@@ -51,7 +51,7 @@ __device__ __forceinline__ uint64_t kp_add2(uint64_t a, uint64_t b) {
 // Waits for a barrier's phase; gives up after a while (some milliseconds at least), or soon after another warp has.
 __device__ __forceinline__ bool kp_wait(uint32_t bar, unsigned parity, const volatile int *failed) {
   for (int i = 0; i < 64; ++i) {
-    if (ap_wait(bar, parity, 1u << 12)) return true;
+    if (ap_wait(bar, parity, 1u << 12)) return true;  // a poll may suspend the warp until the phase ends
     if (*failed) return false;
   }
   return false;
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   __shared__ __align__(8) uint64_t bars[2 * KP_RING + 6 * TILES];
   __shared__ uint32_t tmem_s;
   __shared__ int fail_s, seq_s;
-  __shared__ float4 scales_s[4 * TILES][KP_BLOCKS];  // a softmax warp's own: factor of the scores, log2(vs), 1 / vs
+  __shared__ float2 scales_s[4 * TILES][2][KP_BLOCKS];  // a softmax warp's own, of two tiles: factor of the scores, log2(vs)
+  __shared__ float over_s[4 * TILES][2][KP_BLOCKS];     // 1 / vs
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Kv8Rows &r = p.r;
   pdl_wait();
@@ -113,6 +114,22 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   const int row0 = r.begin(seq), rows = max(0, r.end(seq) - row0) * p.group;
   const int first = (int)(r.cu ? slot - ((long)row0 * p.group / ROWS + seq) : slot % p.slots_per_seq) * ROWS;
   if (first >= rows || rows <= p.few) return;
+  if (PARTS == 1 && warp < Z::SOFT_WARPS) {
+    // ---- the queries are on their way first: 16-byte chunk c of row i to half c / 8, chunk position (c % 8) ^ (i % 8)
+    const int tile0 = first + (warp >> 2) * KP_BM, last = min(tile0 + KP_BM, rows) - 1, c = tid & 15, i0 = (tid & 127) >> 4;
+    const uint32_t dst = ap_smem_u32(smem) + (warp >> 2) * Z::Q_BYTES + (c >> 3) * KP_HALF_BYTES;
+    const int step_t = 8 / p.group, step_h = 8 - step_t * p.group;
+    int token = (tile0 + i0) / p.group, head = tile0 + i0 - token * p.group;
+#pragma unroll 4
+    for (int i = i0; i < KP_BM; i += 8) {
+      const bool in = tile0 + i <= last;
+      const __half *src = (const __half *)p.q + (in ? (size_t)(row0 + token) * p.q_stride + (size_t)(hk * p.group + head) * KV8_D + c * 8 : 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * 128 + (((c & 7) ^ (i & 7)) << 4)), "l"(src), "r"(in ? 16 : 0) : "memory");
+      token += step_t, head += step_h;
+      if (head >= p.group) head -= p.group, ++token;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
   const long pos0 = r.pos0[seq], cap = (long)r.max_pages << p.c.shift;
   auto limit_of = [&](int packed) { return (int)max(0l, min(pos0 + packed / p.group + 1, cap)); };
   // key tiles of each tile of rows; this CTA's share of them
@@ -124,7 +141,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
     any = max(any, lim);
   }
   const int n_all = n_of[TILES - 1] > n_of[0] ? n_of[TILES - 1] : n_of[0];
-  const int j0 = (int)((long)n_all * blockIdx.y / p.splits), j1 = (int)((long)n_all * (blockIdx.y + 1) / p.splits);
+  const int j0 = p.splits == 1 ? 0 : (int)((long)n_all * blockIdx.y / p.splits), j1 = p.splits == 1 ? n_all : (int)((long)n_all * (blockIdx.y + 1) / p.splits);
 #pragma unroll
   for (int t = 0; t < TILES; ++t) n_of[t] = max(0, min(n_of[t], j1) - j0);
   const int n = j1 - j0;
@@ -142,30 +159,19 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   }
   float back = 1.f;  // fp32 queries: what undoes the power of two that a softmax thread's row is scaled by
   if (warp < Z::SOFT_WARPS) {
-    // ---- the queries to shared memory: 16-byte chunk c of row i to half c / 8, chunk position (c % 8) ^ (i % 8)
-    const int t = warp >> 2, mine = tid & 127, tile0 = first + t * KP_BM, last = min(tile0 + KP_BM, rows) - 1;
+    const int t = warp >> 2, mine = tid & 127;
     unsigned char *const q_s = smem + t * Z::Q_BYTES;
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale is the queries': the scores' factors are not negative
     if constexpr (PARTS == 1) {
-      const int c = mine & 15, i0 = mine >> 4;
-      const int step_t = 8 / p.group, step_h = 8 - step_t * p.group;
-      int token = (tile0 + i0) / p.group, head = tile0 + i0 - token * p.group;
-      uint4 v[KP_BM / 8];
-#pragma unroll
-      for (int n = 0; n < KP_BM / 8; ++n) {
-        v[n] = make_uint4(0, 0, 0, 0);
-        if (tile0 + i0 + 8 * n <= last)
-          v[n] = *reinterpret_cast<const uint4 *>((const __half *)p.q + (size_t)(row0 + token) * p.q_stride + (size_t)(hk * p.group + head) * KV8_D + c * 8);
-        token += step_t, head += step_h;
-        if (head >= p.group) head -= p.group, ++token;
-      }
-#pragma unroll
-      for (int n = 0; n < KP_BM / 8; ++n) {
-        const int i = i0 + 8 * n;
-        v[n].x ^= flip, v[n].y ^= flip, v[n].z ^= flip, v[n].w ^= flip;
-        *reinterpret_cast<uint4 *>(q_s + (c >> 3) * KP_HALF_BYTES + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = v[n];
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (flip) {  // what this thread brought in
+        for (int i = mine >> 4; i < KP_BM; i += 8) {
+          uint4 &v = *reinterpret_cast<uint4 *>(q_s + ((mine & 15) >> 3) * KP_HALF_BYTES + i * 128 + (((mine & 7) ^ (i & 7)) << 4));
+          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        }
       }
     } else {
+      const int tile0 = first + t * KP_BM, last = min(tile0 + KP_BM, rows) - 1;
       const int packed = tile0 + mine;
       if (packed <= last) {
         // a row a thread: scaled by a power of two, its largest to 2^13 .. 2^14, and cut into two fp16 numbers
@@ -209,6 +215,48 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  // ---- the loading warps' way into the cache, and their first three units
+  const int32_t *const table = r.table + (size_t)seq * r.table_stride;
+  const int lw = warp - Z::LOAD_WARP, row = ((lane >> 2) & 1) + ((lane >> 4) << 1) + 4 * lw, piece = (lane & 3) | (lane >> 3 & 1) << 2;
+  const uint32_t sw = row & 7;
+  // piece i: chunks 2 i and 2 i + 1 (8 dims each) of the row, in half i / 4
+  const uint32_t put = (piece >> 2) * KP_HALF_BYTES + row * 128, c0 = ((2 * piece & 7) ^ sw) << 4, c1 = ((2 * piece + 1 & 7) ^ sw) << 4;
+  int where = 0, page = 0, page_at = 0;
+  auto ask = [&](int j) {  // the pages of key tile j0 + j's blocks, one a lane of the first eight
+    page_at = (j0 + j) * KP_BLOCKS + (lane & 7);
+    page = page_at * KV8_BLOCK < any ? table[page_at >> (p.c.shift - 4)] : -1;
+  };
+  auto lookup = [&](int j) {  // where the blocks lie whose pages were asked for; then asks for the next tile's
+    where = -1;
+    if (page_at * KV8_BLOCK < any) {
+      if ((unsigned)page >= (unsigned)p.c.pages) {
+        atomicExch(p.status, KV8_BAD_PAGE);
+        page = 0;
+      }
+      where = ((page * p.c.H + hk) << (p.c.shift - 4)) + (page_at & ((1 << (p.c.shift - 4)) - 1));
+    }
+    ask(j + 1);
+  };
+  // a thread's own 16 bytes of each block of a unit: it reads back what it asked for itself
+  const uint32_t raw = ap_smem_u32(smem) + TILES * Z::Q_BYTES + KP_RING * KP_STAGE_BYTES + (tid & 127) * 16;
+  auto load = [&](int u) {
+    if (u < 2 * n) {
+      if ((u & 1) == 0) lookup(u >> 1);
+      const int8_t *src = (u & 1 ? p.c.v : p.c.k) + row * KV8_D + piece * 16;
+#pragma unroll
+      for (int i = 0; i < KP_BLOCKS; ++i) {
+        const int blk = __shfl_sync(0xffffffffu, where, i);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + u % KP_RAW * KP_RAW_BYTES + i * 2048), "l"(src + (size_t)max(blk, 0) * (KV8_BLOCK * KV8_D)), "r"(blk < 0 ? 0 : 16)
+                     : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (warp >= Z::LOAD_WARP && warp < Z::MMA_WARP && n > 0) {
+    ask(0);
+#pragma unroll
+    for (int u = 0; u < KP_RAW - 1; ++u) load(u);
+  }
   if (warp == Z::MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ap_smem_u32(&tmem_s)), "n"(Z::TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -220,51 +268,12 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0);
   const uint32_t q_base = ap_smem_u32(smem), ring = q_base + TILES * Z::Q_BYTES;
   unsigned char *const ring_p = smem + TILES * Z::Q_BYTES;
-  const int32_t *const table = r.table + (size_t)seq * r.table_stride;
 
   if (warp >= Z::LOAD_WARP && warp < Z::MMA_WARP) {
     // ---- K and V tiles in turn through one ring: unit 2 j is K of tile j, 2 j + 1 its V.  The codes of the next three units
     // are on their way while this one's become fp16.  A quarter of a warp stores four even pieces of two neighbouring rows: no
     // two in one bank.
-    const int lw = warp - Z::LOAD_WARP, row = ((lane >> 2) & 1) + ((lane >> 4) << 1) + 4 * lw, piece = (lane & 3) | (lane >> 3 & 1) << 2;
-    const uint32_t sw = row & 7;
-    // piece i: chunks 2 i and 2 i + 1 (8 dims each) of the row, in half i / 4
-    const uint32_t put = (piece >> 2) * KP_HALF_BYTES + row * 128, c0 = ((2 * piece & 7) ^ sw) << 4, c1 = ((2 * piece + 1 & 7) ^ sw) << 4;
-    int where = 0, page = 0, page_at = 0;
-    auto ask = [&](int j) {  // the pages of key tile j0 + j's blocks, one a lane of the first eight
-      page_at = (j0 + j) * KP_BLOCKS + (lane & 7);
-      page = page_at * KV8_BLOCK < any ? table[page_at >> (p.c.shift - 4)] : -1;
-    };
-    auto lookup = [&](int j) {  // where the blocks lie whose pages were asked for; then asks for the next tile's
-      where = -1;
-      if (page_at * KV8_BLOCK < any) {
-        if ((unsigned)page >= (unsigned)p.c.pages) {
-          atomicExch(p.status, KV8_BAD_PAGE);
-          page = 0;
-        }
-        where = ((page * p.c.H + hk) << (p.c.shift - 4)) + (page_at & ((1 << (p.c.shift - 4)) - 1));
-      }
-      ask(j + 1);
-    };
-    // a thread's own 16 bytes of each block of a unit: it reads back what it asked for itself
-    const uint32_t raw = ap_smem_u32(smem) + TILES * Z::Q_BYTES + KP_RING * KP_STAGE_BYTES + (tid - Z::LOAD_WARP * 32) * 16;
-    auto load = [&](int u) {
-      if (u < 2 * n) {
-        if ((u & 1) == 0) lookup(u >> 1);
-        const int8_t *src = (u & 1 ? p.c.v : p.c.k) + row * KV8_D + piece * 16;
-#pragma unroll
-        for (int i = 0; i < KP_BLOCKS; ++i) {
-          const int blk = __shfl_sync(0xffffffffu, where, i);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + u % KP_RAW * KP_RAW_BYTES + i * 2048), "l"(src + (size_t)max(blk, 0) * (KV8_BLOCK * KV8_D)), "r"(blk < 0 ? 0 : 16)
-                       : "memory");
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     bool good = true;
-    if (n > 0) ask(0);
-#pragma unroll
-    for (int u = 0; u < KP_RAW - 1; ++u) load(u);
     for (int u = 0; u < 2 * n; ++u) {
       asm volatile("cp.async.wait_group %0;" ::"n"(KP_RAW - 2) : "memory");
       uint4 now[KP_BLOCKS];
@@ -365,29 +374,32 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
     const int limit = packed <= last ? limit_of(packed) : 0;
     const float scale = fabsf(p.scale);
     float ks_next = 0.f, vs_next = 1.f;
-    auto ask = [&](int j) {  // the scales of key tile j0 + j, a block each for the first eight lanes
-      const int b = (j0 + j) * KP_BLOCKS + lane;
+    int page = 0;
+    auto block_of = [&](int j) { return (j0 + j) * KP_BLOCKS + lane; };  // a block of key tile j0 + j for each of the first eight lanes
+    auto ask_page = [&](int j) { page = lane < KP_BLOCKS && block_of(j) * KV8_BLOCK < any ? table[block_of(j) >> (p.c.shift - 4)] : -1; };
+    auto ask = [&](int j) {  // the scales of tile j, whose pages have come; then the pages of the next
       ks_next = 0.f, vs_next = 1.f;
-      if (lane < KP_BLOCKS && b * KV8_BLOCK < any) {
-        const int page = table[b >> (p.c.shift - 4)];
-        if ((unsigned)page < (unsigned)p.c.pages) {
-          const size_t at = ((size_t)(page * p.c.H + hk) << (p.c.shift - 4)) + (b & ((1 << (p.c.shift - 4)) - 1));
-          ks_next = p.c.ks[at], vs_next = p.c.vs[at];
-        }
+      if ((unsigned)page < (unsigned)p.c.pages) {
+        const size_t at = ((size_t)(page * p.c.H + hk) << (p.c.shift - 4)) + (block_of(j) & ((1 << (p.c.shift - 4)) - 1));
+        ks_next = p.c.ks[at], vs_next = p.c.vs[at];
       }
+      ask_page(j + 1);
     };
-    if (my_n > 0) ask(0);
+    if (my_n > 0) ask_page(0), ask(0);
     float m = -CUDART_INF_F, l = 0.f;
     bool good = true;
-    float4(&sc)[KP_BLOCKS] = scales_s[warp];
-    for (int j = 0; j < my_n; ++j) {
-      __syncwarp();
+    auto scales = [&](int j) {  // of tile j, whose values have come, to shared memory; asks for the next tile's
       if (lane < KP_BLOCKS) {
         const float vs = fmaxf(vs_next, KP_LEAST_SCALE);
-        sc[lane] = make_float4(ks_next * scale, __log2f(vs), __fdividef(1.f, vs), 0.f);
+        scales_s[warp][j & 1][lane] = make_float2(ks_next * scale, __log2f(vs)), over_s[warp][j & 1][lane] = __fdividef(1.f, vs);
       }
+      ask(j + 1);
+    };
+    if (my_n > 0) scales(0);
+    for (int j = 0; j < my_n; ++j) {
+      const float2(&sc)[KP_BLOCKS] = scales_s[warp][j & 1];
+      const float(&over_vs)[KP_BLOCKS] = over_s[warp][j & 1];
       __syncwarp();
-      if (j + 1 < my_n) ask(j + 1);
       if (!__all_sync(0xffffffffu, kp_wait(bar, j & 1, &fail_s))) {
         good = false;
         break;
@@ -400,16 +412,16 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       // 64 keys of the row: their largest exponent, then P = 2^(x - m + 6)
       auto half = [&](int hb, auto all_keys) {
         constexpr bool ALL = decltype(all_keys)::value;
-        uint32_t s[64];
-        uint32_t(&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
-        uint32_t(&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
+        uint32_t s0[32] = {}, s1[32] = {};
+        auto s = [&](int i) { return __uint_as_float(i < 32 ? s0[i & 31] : s1[i & 31]); };
         const uint32_t at = hb ? t_other : t_first;
         ap_ld32(at, s0);
         ap_ld32(at + 32, s1);
+        if (hb == 1) scales(j + 1);
         float f[4], lv[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const float4 q = sc[4 * hb + b];
+          const float2 q = sc[4 * hb + b];
           f[b] = PARTS == 1 ? q.x : q.x * back, lv[b] = q.y;
         }
         const int mine = left - 64 * hb;
@@ -425,7 +437,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
           float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
           for (int i = 16 * b; i < 16 * b + 16; i += 2) {
-            const float u = ALL || i < mine ? __uint_as_float(s[i]) : -CUDART_INF_F, v = ALL || i + 1 < mine ? __uint_as_float(s[i + 1]) : -CUDART_INF_F;
+            const float u = ALL || i < mine ? s(i) : -CUDART_INF_F, v = ALL || i + 1 < mine ? s(i + 1) : -CUDART_INF_F;
             top[i >> 1 & 1] = fmaxf(top[i >> 1 & 1], fmaxf(u, v));
           }
           const float t = fmaxf(top[0], top[1]);
@@ -487,7 +499,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
 #pragma unroll
             for (int i = 8 * h; i < 8 * h + 8; ++i) {
               const int k = 32 * c + 2 * i;
-              KpPair v = kp_unpack(kp_fma2(kp_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, d2));
+              KpPair v = kp_unpack(kp_fma2(kp_pack(s(k), s(k + 1)), f2, d2));
               if constexpr (!ALL) v.a = k < mine ? v.a : -CUDART_INF_F, v.b = k + 1 < mine ? v.b : -CUDART_INF_F;
               float a, b2;
               if (PARTS == 1 && i % 4 == 3) {  // a quarter of them off the exponential unit
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
               }
             }
             const KpPair both = kp_unpack(sum);
-            l = fmaf(both.a + both.b, sc[4 * hb + b].z, l);
+            l = fmaf(both.a + both.b, over_vs[4 * hb + b], l);
           }
           ap_st16(p_at(2 * hb + c), hi);
           if constexpr (PARTS == 2) ap_st16(p_at(2 * hb + c) + 16, lo);
@@ -526,7 +538,10 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
           const uint32_t none[16] = {};
 #pragma unroll
           for (int c = 0; c < (PARTS == 1 ? 2 : 4); ++c) ap_st16((PARTS == 1 ? t_first + 32 * hb : ts + 64 * hb) + 16 * c, none);
-          if (PARTS == 1 && hb == 1) ap_arrive(bar_r);
+          if (hb == 1) {
+            scales(j + 1);
+            if (PARTS == 1) ap_arrive(bar_r);
+          }
         }
       }
       if (!good) break;
