@@ -785,30 +785,63 @@ static int decode_launch(DecodeParams p, const DecodePlan &d, cudaStream_t strea
   return AB200_OK;
 }
 
-// Sequences of up to KD_FEW packed rows go through the kernel above, longer ones through the prompt kernel.
+// Sequences of up to KD_FEW packed rows go through the kernel above, longer ones through the prompt kernel where rows of heads
+// times the positions that the pages hold are more than KD_PROMPT_WORK.  us, above / prompt kernel, rows of heads x positions:
+//   500 x 2600 (one kv head) 13.5 / 24.6     2240 x 570 14.1 / 18.3     4096 x 128 7.2 / 11.5     2048 x 64 12.2 / 10.3
+//   4800 x 650 28.6 / 23.4     2500 x 3000 (one kv head) 86 / 27     4000 x 2000 32 / 26     4096 x 4100 71 / 31     16384 x 4500 308 / 67
 constexpr int KD_FEW = 64;
+constexpr long KD_PROMPT_WORK = 2500000;
+struct AttendPlan {
+  bool prompts, few;  // which kernels run
+  DecodePlan d;
+  Kv8PrefillParams p;
+  size_t bytes;       // of workspace: the prompt kernel's, then the other's (they may run side by side)
+};
 struct NewRows {
   const void *k, *v;
   long k_stride, v_stride;
 };
-static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, int D, float scale, int dtype,
-                  const float *inv_freq, NewRows new_rows, int zero_rest, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
-  if (r.T == 0 || r.S == 0) return AB200_OK;
-  const DecodePlan d = decode_plan(r.S, r.T, r.cu ? max_rows : r.n, Hq, c.H, r.cu == nullptr, (long)r.max_pages << c.shift);
-  AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= d.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, d.bytes, workspace_bytes);
+static int attend_plan(const Kv8Cache &c, const Kv8Rows &r, int max_rows, int Hq, int dtype, bool rotate, AttendPlan *a) {
   const int group = Hq / c.H;
+  const long capacity = (long)r.max_pages << c.shift, most = r.cu ? max_rows : r.n;
+  a->prompts = most * group > KD_FEW && (long)r.T * Hq * capacity > KD_PROMPT_WORK && !rotate;
+  a->few = !a->prompts || r.cu != nullptr;
+  a->d = decode_plan(r.S, r.T, a->few && a->prompts ? KD_FEW / group : (int)most, Hq, c.H, r.cu == nullptr, capacity);
+  a->p = Kv8PrefillParams{};
+  a->p.c = c, a->p.r = r, a->p.group = group;
+  size_t prompt_bytes = 0;
+  if (a->prompts) {
+    const int rc = kv8_prefill_plan(&a->p, dtype, capacity, &prompt_bytes);
+    if (rc) return rc;
+  }
+  a->bytes = prompt_bytes + a->d.bytes;
+  return AB200_OK;
+}
+static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const void *q, long q_stride, void *out, int max_rows, int Hq, float scale, int dtype, const float *inv_freq,
+                  NewRows new_rows, int zero_rest, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (r.T == 0 || r.S == 0) return AB200_OK;
+  AttendPlan a;
+  int rc = attend_plan(c, r, max_rows, Hq, dtype, inv_freq != nullptr, &a);
+  if (rc) return rc;
+  AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= a.bytes, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, a.bytes, workspace_bytes);
   int *status = kernel_error_ptr();
   AB200_REQUIRE(status != nullptr, "%s: cannot resolve the status word", who);
+  const int group = Hq / c.H;
   const float scale2 = scale * 1.4426950408889634f;
-  const long most = r.cu ? max_rows : r.n;
-  const bool prompts = most * group > KD_FEW && inv_freq == nullptr;
-  if (prompts) {
-    const int rc = kv8_prefill(Kv8PrefillParams{c, r, q, q_stride, out, Hq, group, scale2, KD_FEW, nullptr, nullptr, status, 0, 0, 1}, dtype, stream);
-    if (rc || !r.cu) return rc;
+  if (a.prompts) {
+    a.p.q = q, a.p.q_stride = q_stride, a.p.out = out, a.p.Hq = Hq, a.p.scale = scale2, a.p.few = a.few ? KD_FEW : 0, a.p.status = status;
+    rc = kv8_prefill(a.p, dtype, workspace, stream);
+    if (rc) return rc;
   }
-  DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, new_rows.k, new_rows.v, new_rows.k_stride, new_rows.v_stride, zero_rest && r.cu, prompts ? KD_FEW : 0x7fffffff, 0, 0, prompts && pdl_enabled(), (float *)workspace, (int4 *)((char *)workspace + d.partial_bytes), status};
-  if (dtype == AB200_F32) return d.rows == 8 ? decode_launch<float, 8>(p, d, stream) : decode_launch<float, 16>(p, d, stream);
-  return d.rows == 8 ? decode_launch<__half, 8>(p, d, stream) : decode_launch<__half, 16>(p, d, stream);
+  if (a.few) {
+    char *ws = (char *)workspace + (a.bytes - a.d.bytes);
+    DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, new_rows.k, new_rows.v, new_rows.k_stride, new_rows.v_stride, zero_rest && r.cu,
+                   a.prompts ? KD_FEW : 0x7fffffff, 0, 0, a.prompts && pdl_enabled(), (float *)ws, (int4 *)(ws + a.d.partial_bytes), status};
+    if (dtype == AB200_F32) rc = a.d.rows == 8 ? decode_launch<float, 8>(p, a.d, stream) : decode_launch<float, 16>(p, a.d, stream);
+    else rc = a.d.rows == 8 ? decode_launch<__half, 8>(p, a.d, stream) : decode_launch<__half, 16>(p, a.d, stream);
+    if (rc) return rc;
+  }
+  return a.prompts ? kv8_prefill_join(a.p, dtype, workspace, stream) : AB200_OK;
 }
 
 static int attention_check(const char *who, const Kv8Cache &c, int T, const void *q, long q_stride, const void *out, int Hq, int D, int dtype) {
@@ -828,8 +861,21 @@ static int attention_check(const char *who, const Kv8Cache &c, int T, const void
 using namespace ab200;
 
 extern "C" size_t ab200_kv8_attention_workspace_bytes(int S, int T, int max_rows, int Hq, int Hkv) {
-  if (S <= 0 || T <= 0 || Hkv <= 0 || Hq < Hkv) return 0;
-  return decode_plan(S, T, max_rows, Hq, Hkv, false, 0).bytes;
+  if (S <= 0 || T <= 0 || Hkv <= 0 || Hq < Hkv || max_rows < 0) return 0;
+  // whichever kernels serve the call, however long the sequences, as many rows each or not
+  size_t most = 0;
+  for (int dtype = AB200_F16; dtype <= AB200_F32; ++dtype)
+    for (int ragged = 0; ragged < 2; ++ragged) {
+      Kv8Cache c = {};
+      Kv8Rows r = {};
+      c.H = Hkv, c.shift = 4;
+      r.S = S, r.T = T, r.n = T / S, r.max_pages = 1 << 26;
+      r.cu = ragged ? (const int32_t *)16 : nullptr;
+      AttendPlan a;
+      if ((!ragged && T % S) || attend_plan(c, r, max_rows, Hq, dtype, false, &a)) continue;
+      if (a.bytes > most) most = a.bytes;
+    }
+  return most;
 }
 
 extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages,
@@ -842,7 +888,7 @@ extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, cons
   int rc = kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_attention", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc) return rc;
-  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, D, scale, dtype, nullptr, NewRows{}, zero_rest, workspace, workspace_bytes, (cudaStream_t)stream);
+  return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, scale, dtype, nullptr, NewRows{}, zero_rest, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long q_stride, long k_stride, long v_stride, void *out, void *k_cache, void *v_cache,
@@ -858,18 +904,19 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   const long vec = dtype == AB200_F16 ? 8 : 4;
   AB200_REQUIRE(k && v && k_stride % vec == 0 && v_stride % vec == 0 && k_stride >= (long)Hkv * KV8_D && v_stride >= (long)Hkv * KV8_D && aligned16(k) && aligned16(v),
                 "kv8_step: k and v must be 16-byte aligned rows of at least %d values, a multiple of 16 bytes apart", Hkv * KV8_D);
-  const size_t need = decode_plan(S, T, T / S, Hq, Hkv, false, 0).bytes;
-  AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
+  AttendPlan a;
+  rc = attend_plan(c, r, T / S, Hq, dtype, inv_freq != nullptr, &a);
+  if (rc) return rc;
+  AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= a.bytes, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", a.bytes, workspace_bytes);
   // fp16 rows that fit into one tile are written by the attention kernel itself where an item is a cluster's; else by a launch
   // before it: us, together / apart: one request of 384 positions and 32 heads 11.0 / 12.9, 48 ragged ones in equal shares
   // 69 / 55 (each new block's 4 us then is one CTA's, and the others wait for it at the end)
-  const DecodePlan plan = decode_plan(S, T, T / S, Hq, Hkv, true, (long)max_pages * page_rows);
-  const bool together = dtype == AB200_F16 && plan.splits > 0 && plan.tiles == 1;
+  const bool together = dtype == AB200_F16 && !a.prompts && a.d.splits > 0 && a.d.tiles == 1;
   if (!together) {
     rc = ab200_kv8_append(k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, k, v, k_stride, v_stride,
                           nullptr, 0, nullptr, 0, 0, inv_freq, 0, dtype, stream);
     if (rc) return rc;
   }
-  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, D, scale, dtype, inv_freq, together ? NewRows{k, v, k_stride, v_stride} : NewRows{}, 0, workspace, workspace_bytes,
+  return attend("kv8_step", c, r, q, q_stride, out, T / S, Hq, scale, dtype, inv_freq, together ? NewRows{k, v, k_stride, v_stride} : NewRows{}, 0, workspace, workspace_bytes,
                 (cudaStream_t)stream);
 }

@@ -81,6 +81,32 @@ __device__ __forceinline__ uint32_t kp_half2(uint32_t flipped) {  // two codes (
   return h22u(__hsub2(u2h2(__byte_perm(flipped, 0x64646464u, SEL)), u2h2(0x64806480u)));
 }
 
+// The rows of a slot, ROWS packed rows of one sequence.  Sequence s owns the slots from begin(s) group / ROWS + s on: that
+// many lie before the next one's.  seq < 0: none.
+struct KpRows {
+  int seq, row0, rows, first;  // first row of the sequence in q, its packed rows, the slot's first of them
+};
+template <int ROWS, int THREADS>
+__device__ __forceinline__ KpRows kp_rows(const Kv8PrefillParams &p, int slot, int *seq_s) {
+  const Kv8Rows &r = p.r;
+  if (threadIdx.x == 0) *seq_s = r.cu ? -1 : slot / p.slots_per_seq;
+  __syncthreads();
+  if (r.cu) {
+    for (int s = threadIdx.x; s < r.S; s += THREADS) {
+      const long at = (long)r.begin(s) * p.group / ROWS + s, next = s + 1 < r.S ? (long)r.begin(s + 1) * p.group / ROWS + s + 1 : (long)p.slots;
+      if (slot >= at && slot < next) *seq_s = s;
+    }
+    __syncthreads();
+  }
+  KpRows o;
+  o.seq = *seq_s;
+  if (o.seq < 0 || o.seq >= r.S) return KpRows{-1, 0, 0, 0};
+  o.row0 = r.begin(o.seq), o.rows = max(0, r.end(o.seq) - o.row0) * p.group;
+  o.first = (int)(r.cu ? slot - ((long)o.row0 * p.group / ROWS + o.seq) : slot % p.slots_per_seq) * ROWS;
+  if (o.first >= o.rows || o.rows <= p.few) o.seq = -1;
+  return o;
+}
+
 // TILES: tiles of 128 packed query rows that share the CTA's keys.  PARTS: fp16 numbers that a query and a P are held in.
 template <typename T, int TILES, int PARTS>
 __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill_kernel(const __grid_constant__ Kv8PrefillParams p) {
@@ -97,23 +123,12 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   const Kv8Rows &r = p.r;
   pdl_wait();
 
-  // ---- which rows: pairs of tiles of one sequence and kv head.  Sequence s owns the slots from begin(s) group / 256 + s on.
+  // ---- which rows
   const int hk = blockIdx.x % p.c.H, slot = p.slots - 1 - (int)(blockIdx.x / p.c.H);  // the last rows have the most keys: they start first
-  constexpr int ROWS = TILES * KP_BM;
-  if (tid == 0) seq_s = r.cu ? -1 : slot / p.slots_per_seq, fail_s = 0;
-  __syncthreads();
-  if (r.cu) {
-    for (int s = tid; s < r.S; s += Z::THREADS) {
-      const long at = (long)r.begin(s) * p.group / ROWS + s, next = s + 1 < r.S ? (long)r.begin(s + 1) * p.group / ROWS + s + 1 : (long)p.slots;
-      if (slot >= at && slot < next) seq_s = s;
-    }
-    __syncthreads();
-  }
-  const int seq = seq_s;
-  if (seq < 0 || seq >= r.S) return;
-  const int row0 = r.begin(seq), rows = max(0, r.end(seq) - row0) * p.group;
-  const int first = (int)(r.cu ? slot - ((long)row0 * p.group / ROWS + seq) : slot % p.slots_per_seq) * ROWS;
-  if (first >= rows || rows <= p.few) return;
+  if (tid == 0) fail_s = 0;
+  const KpRows place = kp_rows<TILES * KP_BM, Z::THREADS>(p, slot, &seq_s);
+  const int seq = place.seq, row0 = place.row0, rows = place.rows, first = place.first;
+  if (seq < 0) return;
   if (PARTS == 1 && warp < Z::SOFT_WARPS) {
     // ---- the queries are on their way first: 16-byte chunk c of row i to half c / 8, chunk position (c % 8) ^ (i % 8)
     const int tile0 = first + (warp >> 2) * KP_BM, last = min(tile0 + KP_BM, rows) - 1, c = tid & 15, i0 = (tid & 127) >> 4;
@@ -557,7 +572,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       fail_s = 1;
     } else if (tile0 <= last) {
       if (p.splits > 1) {
-        const size_t at = ((((size_t)slot * p.c.H + hk) * p.splits + blockIdx.y) * TILES + t) * KP_BM + mine;
+        const size_t at = (((size_t)slot * p.c.H + hk) * p.splits + blockIdx.y) * (TILES * KP_BM) + t * KP_BM + mine;
         float *o_part = p.partial + at * KV8_D;
         if (my_n > 0) {
 #pragma unroll 1
@@ -621,23 +636,75 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   if (fail_s && tid == 0) atomicExch(p.status, 710);  // site 710: a wait of the 8-bit prompt attention ran out
 }
 
+// Joins the shares of the keys: a warp a packed row.
+constexpr int KP_JOIN_WARPS = 8;
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(KP_JOIN_WARPS * 32) kv8_prefill_join_kernel(const __grid_constant__ Kv8PrefillParams p) {
+  __shared__ int seq_s;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int hk = blockIdx.x % p.c.H, slot = (int)(blockIdx.x / p.c.H), lane = threadIdx.x & 31, row = blockIdx.y * KP_JOIN_WARPS + (threadIdx.x >> 5);
+  const KpRows place = kp_rows<ROWS, KP_JOIN_WARPS * 32>(p, slot, &seq_s);
+  const int packed = place.first + row;
+  if (place.seq < 0 || packed >= place.rows) return;
+  float m = -CUDART_INF_F, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int z = 0; z < p.splits; ++z) {
+    const size_t at = (((size_t)slot * p.c.H + hk) * p.splits + z) * ROWS + row;
+    const float2 ml = p.partial_ml[at];
+    if (ml.y == 0.f) continue;  // no keys there: nothing was written (a sum that is not a number is not 0)
+    const float4 v = reinterpret_cast<const float4 *>(p.partial + at * KV8_D)[lane];
+    const float up = fmaxf(m, ml.x), f = m == -CUDART_INF_F ? 0.f : ap_ex2(m - up), fc = ml.x == -CUDART_INF_F ? 1.f : ap_ex2(ml.x - up);
+    l = l * f + ml.y * fc;
+    acc.x = acc.x * f + v.x * fc, acc.y = acc.y * f + v.y * fc, acc.z = acc.z * f + v.z * fc, acc.w = acc.w * f + v.w * fc;
+    m = up;
+  }
+  const int token = packed / p.group, head = hk * p.group + packed - token * p.group;
+  T *out = (T *)p.out + ((size_t)(place.row0 + token) * p.Hq + head) * KV8_D + 4 * lane;
+  const float x[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.f ? 0.f : x[e] / l);
+}
+
 template <typename T, int TILES, int PARTS>
-static int prefill_launch(Kv8PrefillParams p, long slots, cudaStream_t stream) {
-  p.slots = (int)slots;
+static int prefill_launch(const Kv8PrefillParams &p, cudaStream_t stream) {
   using Z = KpShape<TILES, PARTS>;
   AB200_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<T, TILES, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM));
-  AB200_REQUIRE(slots * p.c.H < 1l << 31, "kv8_attention: %ld tiles of rows are beyond the built limits", slots * p.c.H);
-  AB200_CUDA(launch_pdl(kv8_prefill_kernel<T, TILES, PARTS>, dim3((unsigned)(slots * p.c.H), p.splits), dim3(Z::THREADS), Z::SMEM, stream, p));
+  AB200_CUDA(launch_pdl(kv8_prefill_kernel<T, TILES, PARTS>, dim3((unsigned)(p.slots * p.c.H), p.splits), dim3(Z::THREADS), Z::SMEM, stream, p));
   return AB200_OK;
 }
 
-int kv8_prefill(Kv8PrefillParams p, int dtype, cudaStream_t stream) {
+// Tiles of rows, and how the keys are shared out where those alone would leave most SMs idle.
+int kv8_prefill_plan(Kv8PrefillParams *p, int dtype, long capacity, size_t *bytes) {
   const int rows = dtype == AB200_F16 ? 256 : 128;
-  p.slots_per_seq = (int)(((long)p.r.n * p.group + rows - 1) / rows);
-  const long slots = p.r.cu ? (long)p.r.T * p.group / rows + p.r.S : (long)p.r.S * p.slots_per_seq;
-  p.splits = 1;
-  if (dtype == AB200_F16) return prefill_launch<__half, 2, 1>(p, slots, stream);
-  return prefill_launch<float, 1, 2>(p, slots, stream);
+  p->slots_per_seq = (int)(((long)p->r.n * p->group + rows - 1) / rows);
+  const long slots = p->r.cu ? (long)p->r.T * p->group / rows + p->r.S : (long)p->r.S * p->slots_per_seq, items = slots * p->c.H;
+  AB200_REQUIRE(items < 1l << 31, "kv8_attention: %ld tiles of rows are beyond the built limits", items);
+  p->slots = (int)slots;
+  // each share two tiles of keys at least; at most one CTA an SM, so that the parts stay within 20 MB
+  long splits = sm_count() / items;
+  if (splits > 8) splits = 8;
+  if (splits > capacity / (2 * KP_BN)) splits = capacity / (2 * KP_BN);
+  p->splits = splits > 1 ? (int)splits : 1;
+  *bytes = p->splits > 1 ? (size_t)items * p->splits * rows * (KV8_D + 2) * sizeof(float) : 0;
+  return AB200_OK;
+}
+
+int kv8_prefill(Kv8PrefillParams p, int dtype, void *workspace, cudaStream_t stream) {
+  p.partial = (float *)workspace;
+  p.partial_ml = (float2 *)(p.partial + (size_t)p.slots * p.c.H * p.splits * (dtype == AB200_F16 ? 256 : 128) * KV8_D);
+  return dtype == AB200_F16 ? prefill_launch<__half, 2, 1>(p, stream) : prefill_launch<float, 1, 2>(p, stream);
+}
+
+int kv8_prefill_join(Kv8PrefillParams p, int dtype, void *workspace, cudaStream_t stream) {
+  if (p.splits == 1) return AB200_OK;
+  p.partial = (float *)workspace;
+  p.partial_ml = (float2 *)(p.partial + (size_t)p.slots * p.c.H * p.splits * (dtype == AB200_F16 ? 256 : 128) * KV8_D);
+  if (dtype == AB200_F16)
+    AB200_CUDA(launch_pdl(kv8_prefill_join_kernel<__half, 256>, dim3((unsigned)(p.slots * p.c.H), 256 / KP_JOIN_WARPS), dim3(KP_JOIN_WARPS * 32), 0, stream, p));
+  else
+    AB200_CUDA(launch_pdl(kv8_prefill_join_kernel<float, 128>, dim3((unsigned)(p.slots * p.c.H), 128 / KP_JOIN_WARPS), dim3(KP_JOIN_WARPS * 32), 0, stream, p));
+  return AB200_OK;
 }
 
 }  // namespace ab200

@@ -13,11 +13,15 @@ struct Kv8PrefillParams {
   int Hq, group;
   float scale;        // times log2(e)
   int few;            // sequences of up to this many rows (times group) are another kernel's
-  float *partial;     // splits > 1: [slot][kv head][split][tile][128][128], and the rows' maximum and sum
-  float2 *partial_ml;
   int *status;
-  int slots, slots_per_seq, splits;  // set by kv8_prefill: tiles of rows, those of a sequence (cu == nullptr), shares of the keys
+  // set by kv8_prefill_plan: tiles of rows, those of a sequence (cu == nullptr), shares of the keys
+  int slots, slots_per_seq, splits;
+  // splits > 1: [slot][kv head][split][row of the slot][128], and the rows' maximum and sum
+  float *partial;
+  float2 *partial_ml;
 };
-int kv8_prefill(Kv8PrefillParams p, int dtype, cudaStream_t stream);
+int kv8_prefill_plan(Kv8PrefillParams *p, int dtype, long capacity, size_t *bytes);
+int kv8_prefill(Kv8PrefillParams p, int dtype, void *workspace, cudaStream_t stream);
+int kv8_prefill_join(Kv8PrefillParams p, int dtype, void *workspace, cudaStream_t stream);  // after every launch that may run beside the one above
 
 }  // namespace ab200

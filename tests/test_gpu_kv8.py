@@ -40,6 +40,12 @@ def _setup(seed, past, rows, heads, page, spare=3, filled=True):
     return [t.cuda() for t in cache], table.cuda()
 
 
+def _wide(table, page):
+    """The same table with room for 65536 positions: rows enough for the prompt kernel then go through it.  What it adds names
+    no page."""
+    return torch.cat([table, torch.full((table.shape[0], 65536 // page), 0x7FFFFFF0, dtype=torch.int32, device="cuda")], 1)
+
+
 def _ref(cache, table):
     return kv8_ref.Cache(cache, table)
 
@@ -72,6 +78,9 @@ CASES = [
     ([5, 200, 31], [4] * 3, 16, 4, 32), ([100, 3], [2] * 2, 5, 1, 128), ([2500], [1], 16, 1, 256), ([300] * 40, [1] * 40, 8, 8, 32), ([129, 300], [8, 8], 32, 2, 64),
     ([0], [17], 4, 4, 16), ([0], [130], 4, 2, 16), ([77], [64], 8, 2, 32), ([0, 40, 333, 0], [3, 200, 1, 129], 6, 2, 64), ([10, 20, 30], [0, 70, 0], 4, 4, 32),
     ([1200, 5, 64], [90, 1, 300], 8, 1, 128), ([0, 0], [256, 256], 2, 2, 16),
+    # prompts whose keys are one CTA's (many tiles of rows) or several, beside single rows
+    ([0], [150], 32, 4, 16), ([0, 3, 70], [140] * 3, 32, 32, 32), ([5, 40, 333, 0, 100], [130, 70, 1, 0, 65], 32, 4, 32), ([700], [257], 20, 4, 64), ([1100, 0], [60, 400], 12, 12, 128),
+    ([0], [129], 48, 16, 256), ([2000, 31], [3, 100], 63, 9, 64),
 ]
 
 
@@ -86,28 +95,29 @@ def test_attention(cuda, past, rows, hq, hkv, page, dtype):
     ref = _ref(cache, table)
     _check_attention(got, ref, q, past, cu, max(p + n for p, n in zip(past, rows)), dtype)
     # the same rows whatever the hint says and however the rows are named
-    for hint in (1, 7, T):
-        again = ops.kv8_attention(q, cache, table, _ints(past), cu_rows=_cu(rows), max_rows=hint)
+    for hint, t in ((1, table), (7, table), (T, table), (T, _wide(table, page)), (None, _wide(table, page))):
+        again = ops.kv8_attention(q, cache, t, _ints(past), cu_rows=None if hint is None and uniform else _cu(rows), max_rows=hint)
         _check_attention(again, ref, q, past, cu, max(p + n for p, n in zip(past, rows)), dtype)
     assert ops.kernel_status() == 0
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("mul", [0.0, 24.0])
-@pytest.mark.parametrize("past,rows,hq,hkv", [([333, 64], [1, 1], 8, 2), ([50], [140], 4, 1)])
+@pytest.mark.parametrize("past,rows,hq,hkv", [([333, 64], [1, 1], 8, 2), ([50], [140], 4, 1), ([50], [140], 32, 4), ([0, 60], [140, 140], 32, 32)])
 def test_flat_and_sharp_scores(cuda, past, rows, hq, hkv, mul, dtype):
     """All scores alike, and scores spread over hundreds: the running maximum moves often."""
     cache, table = _setup(3, past, rows, hkv, 32)
     q = _randn(2, sum(rows), hq, 128, dtype=dtype, mul=mul)
-    got = ops.kv8_attention(q, cache, table, _ints(past), max_rows=max(rows))
-    _check_attention(got, _ref(cache, table), q, past, None, max(p + n for p, n in zip(past, rows)), dtype)
+    for t in (table, _wide(table, 32)):
+        got = ops.kv8_attention(q, cache, t, _ints(past), max_rows=max(rows))
+        _check_attention(got, _ref(cache, table), q, past, None, max(p + n for p, n in zip(past, rows)), dtype)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("rows", [1, 40, 150])
 def test_block_scales_far_apart(cuda, rows, dtype):
     """Scales from 2^-40 to 2^12, and blocks of zeros, side by side."""
-    past, hq, hkv = 200, 8, 2
+    past, hq, hkv = 200, 32, 4
     cache, table = _setup(5, [past], [rows], hkv, 64)
     g = torch.Generator().manual_seed(8)
     for t in cache[2:]:
@@ -117,10 +127,12 @@ def test_block_scales_far_apart(cuda, rows, dtype):
     q = _randn(2, rows, hq, 128, dtype=dtype, mul=0.1)
     if dtype == F16:
         cache[3].clamp_(max=2.0 ** 5)
+    ref = _ref(cache, table)
+    table = _wide(table, 64)
     got = ops.kv8_attention(q, cache, table, _ints([past]))
-    _check_attention(got, _ref(cache, table), q, [past], None, past + rows, dtype, norm=False)
+    _check_attention(got, ref, q, [past], None, past + rows, dtype, norm=False)
     # a negative scale
-    _check_attention(ops.kv8_attention(q, cache, table, _ints([past]), scale=-0.05), _ref(cache, table), q, [past], None, past + rows, dtype, scale=-0.05, norm=False)
+    _check_attention(ops.kv8_attention(q, cache, table, _ints([past]), scale=-0.05), ref, q, [past], None, past + rows, dtype, scale=-0.05, norm=False)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
@@ -129,7 +141,7 @@ def test_rows_with_nothing_to_attend_to(cuda, rows, dtype):
     """Negative positions attend to nothing (zeros), positions behind the table to all of it."""
     cache, table = _setup(6, [400 - rows, 400 - rows], [rows] * 2, 2, 64)
     table = table[:, :6].contiguous()  # capacity 384
-    q = _randn(3, 2 * rows, 4, 128, dtype=dtype)
+    q = _randn(3, 2 * rows, 32, 128, dtype=dtype)
     for pos0 in ([-3, 384 - rows // 2], [-rows, -1000], [0, 383], [2 ** 31 - 1, -2 ** 31]):
         if max(pos0) > 10000 and rows > 1:
             continue
@@ -144,12 +156,13 @@ def test_rows_with_nothing_to_attend_to(cuda, rows, dtype):
 def test_queries_that_are_not_finite_stay_in_their_row(cuda, value, dtype):
     for past, rows in (([90], [3]), ([20], [150])):
         cache, table = _setup(7, past, rows, 2, 32)
-        q = _randn(4, rows[0], 6, 128, dtype=dtype)
+        q = _randn(4, rows[0], 30, 128, dtype=dtype)
+        table = _wide(table, 32)
         want = ops.kv8_attention(q, cache, table, _ints(past))
         q[1, 4, 7] = value
         got = ops.kv8_attention(q, cache, table, _ints(past))
         assert not got[1, 4].isfinite().any()
-        keep = torch.ones(rows[0], 6, dtype=torch.bool, device="cuda")
+        keep = torch.ones(rows[0], 30, dtype=torch.bool, device="cuda")
         keep[1, 4] = False
         assert torch.equal(got[keep], want[keep])
 
@@ -262,14 +275,15 @@ def test_rows_behind_the_last_sequence(cuda, rows):
     """A padded batch: rows that are nobody's keep what `out` held, and are zeros in a new result."""
     cache, table = _setup(11, [40, 3], [rows, 2], 2, 32)
     T = rows + 2 + 9
-    q = _randn(1, T, 4, 128)
+    q = _randn(1, T, 24, 128)
+    ref, table = _ref(cache, table), _wide(table, 32)
     cu = _ints([0, rows, rows + 2])
     out = torch.full_like(q, 5.0)
     ops.kv8_attention(q, cache, table, _ints([40, 3]), cu_rows=cu, out=out)
     assert (out[rows + 2:] == 5).all()
     new = ops.kv8_attention(q, cache, table, _ints([40, 3]), cu_rows=cu)
     assert torch.equal(new[:rows + 2], out[:rows + 2]) and not new[rows + 2:].any()
-    _check_attention(new[:rows + 2], _ref(cache, table), q[:rows + 2], [40, 3], np.array([0, rows, rows + 2]), 300, F16)
+    _check_attention(new[:rows + 2], ref, q[:rows + 2], [40, 3], np.array([0, rows, rows + 2]), 300, F16)
     qo = torch.full_like(q, 5.0)
     k = _randn(2, T, 2, 128)
     ops.kv8_append(cache, k, k, table, _ints([40, 3]), cu_rows=cu, q=q, inv_freq=torch.from_numpy(INV_FREQ).cuda(), q_out=qo)
@@ -307,9 +321,10 @@ def test_a_bad_page_is_reported(cuda):
     """Entries that name no page: nothing is written there, the status says so, and the next call is well."""
     for rows in (1, 150):
         cache, table = _setup(15, [70], [rows], 2, 32, filled=False)
+        table = _wide(table, 32)
         table[0, 2] = cache[0].shape[0]
         before = [t.clone() for t in cache]
-        x, q = _randn(1, rows, 2, 128), _randn(2, rows, 4, 128)
+        x, q = _randn(1, rows, 2, 128), _randn(2, rows, 32, 128)
         ops.kv8_append(cache, x, x, table, _ints([70]))
         with pytest.raises(_lib.Ab200Error, match="page table"):
             ops.kernel_status()
@@ -401,7 +416,7 @@ def test_captured_with_other_streams_alive(cuda, hq, hkv):
 
 
 def test_same_bits_every_time(cuda):
-    for past, rows, hq, hkv in (([3000, 1, 900], [1] * 3, 32, 8), ([500], [200], 8, 2)):
+    for past, rows, hq, hkv in (([3000, 1, 900], [1] * 3, 32, 8), ([500], [200], 8, 2), ([500], [200], 32, 2)):
         cache, table = _setup(30, past, rows, hkv, 64)
         q = _randn(1, sum(rows), hq, 128)
         first = ops.kv8_attention(q, cache, table, _ints(past))
