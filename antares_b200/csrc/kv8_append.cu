@@ -1,5 +1,11 @@
 // Writing rows into the 8-bit paged KV cache and reading them back (layout: kv8.cuh).  Both are streams: every element is
-// read once and written once.
+// read once and written once, so DRAM is what they cannot do without.
+//
+// Append.  s = max(the block's scale if it holds rows before the new ones, max |x| / 127), code = x / s rounded to the nearest.
+// 2000 rows of 32 heads, K, V and rotated queries: 82 MB in 23.3 us (3.5 TB/s; 17.2 us, 2.9 TB/s, without rotation and queries).
+// Bound by the chain of loads of a short-lived CTA (whose rows, which page, the rows) and the instructions between: 64 registers
+// and four CTAs an SM against 80 and three: 23.3 / 23.7 us; codes by a quotient of two bounds, repeated exactly where those differ: 31.
+// Read.  The same rows: 49 MB in 8.7 us (5.7 TB/s): bound by memory.
 #include <math_constants.h>
 
 #include "kv8_quant.cuh"
@@ -23,15 +29,23 @@ struct AppendParams {
   int *status;
 };
 
-// Whose the rows row0 .. row0 + n - 1 are (-1: nobody's), to shared memory.
+// Whose the rows row0 .. row0 + N - 1 are (-1: nobody's) and at which positions, to shared memory.  A thread asks for all it may
+// need of a sequence at once: one wait for memory, not three.
 template <int N, int THREADS>
-__device__ __forceinline__ void kv8_rows_of(const Kv8Rows &r, int row0, int (&row_seq)[N]) {
+__device__ __forceinline__ void kv8_rows_of(const Kv8Rows &r, int row0, int (&row_seq)[N], long (&row_pos)[N]) {
   const int tid = threadIdx.x;
-  if (tid < N) row_seq[tid] = r.cu || row0 + tid >= r.T ? -1 : (row0 + tid) / r.n;
+  if (tid < N) {
+    const int row = row0 + tid;
+    row_seq[tid] = -1;
+    if (!r.cu && row < r.T) row_seq[tid] = row / r.n, row_pos[tid] = (long)r.pos0[row / r.n] + row % r.n;
+  }
   __syncthreads();
   if (r.cu) {
-    for (int s = tid; s < r.S; s += THREADS)
-      for (int i = max(r.begin(s) - row0, 0), e = min(r.end(s) - row0, N); i < e; ++i) row_seq[i] = s;
+    for (int s = tid; s < r.S; s += THREADS) {
+      const int begin = r.begin(s), end = r.end(s);
+      const long pos0 = r.pos0[s];
+      for (int i = max(begin - row0, 0), e = min(end - row0, N); i < e; ++i) row_seq[i] = s, row_pos[i] = pos0 + row0 + i - begin;
+    }
     __syncthreads();
   }
 }
@@ -44,10 +58,11 @@ __device__ __forceinline__ void kv8_rows_of(const Kv8Rows &r, int row0, int (&ro
 // q: a slot is 16 consecutive rows.
 // Rows are asked for before the sines are made.
 template <typename T>
-__global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 3 : 1) kv8_append_kernel(const __grid_constant__ AppendParams<T> p) {
+__global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 4 : 1) kv8_append_kernel(const __grid_constant__ AppendParams<T> p) {
   typedef typename KaAngle<T>::type A;
   __shared__ __align__(16) A sn[KV8_BLOCK][KV8_D / 2], cs[KV8_BLOCK][KV8_D / 2];
-  __shared__ int seq_s, row_seq[KV8_BLOCK];
+  __shared__ int seq_s, begin_s, end_s, row_seq[KV8_BLOCK];
+  __shared__ long pos_s, row_pos[KV8_BLOCK];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane & 15, hw = lane >> 4;
   const Kv8Rows &r = p.r;
   pdl_launch_dependents();
@@ -56,18 +71,18 @@ __global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 3 : 1) kv8_append
   if ((int)blockIdx.y >= p.kv_groups) {  // ---- rotate query rows
     const int row0 = blockIdx.x * KV8_BLOCK;
     if (row0 >= r.T) return;
-    kv8_rows_of<KV8_BLOCK, KA_THREADS>(r, row0, row_seq);
+    kv8_rows_of<KV8_BLOCK, KA_THREADS>(r, row0, row_seq, row_pos);
     const int h0 = ((int)blockIdx.y - p.kv_groups) * KA_Q_HEADS;
     constexpr int EACH = KV8_BLOCK * KA_Q_HEADS / (KA_THREADS / 16);  // rows of heads that a half-warp has
-    float f[EACH][8];
+    KaRaw<T> raw[EACH];
 #pragma unroll
     for (int n = 0; n < EACH; ++n) {
       const int i = (tid >> 4) + n * (KA_THREADS / 16), row = i / KA_Q_HEADS, h = h0 + i % KA_Q_HEADS;
-      if (row0 + row < r.T && row_seq[row] >= 0 && h < p.Hq) ka_load(p.q + (size_t)(row0 + row) * p.q_stride + (size_t)h * KV8_D, sub, f[n]);
+      if (row0 + row < r.T && row_seq[row] >= 0 && h < p.Hq) ka_ask(p.q + (size_t)(row0 + row) * p.q_stride + (size_t)h * KV8_D, sub, raw[n]);
     }
     for (int i = tid; i < KV8_BLOCK * KV8_D / 2; i += KA_THREADS) {
-      const int row = i >> 6, s = row_seq[row];
-      if (s >= 0) ka_sincos((float)(r.pos0[s] + row0 + row - r.begin(s)) * p.inv_freq[i & 63], &sn[row][i & 63], &cs[row][i & 63]);
+      const int row = i >> 6;
+      if (row_seq[row] >= 0) ka_sincos((float)(int)row_pos[row] * p.inv_freq[i & 63], &sn[row][i & 63], &cs[row][i & 63]);
     }
     __syncthreads();
 #pragma unroll
@@ -76,8 +91,10 @@ __global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 3 : 1) kv8_append
       if (row0 + row >= r.T || h >= p.Hq) continue;
       T *out = p.q_out + (size_t)(row0 + row) * p.q_out_stride + (size_t)h * KV8_D;
       if (row_seq[row] >= 0) {
-        ka_turn(f[n], sn[row], cs[row], sub);
-        ka_store(out, sub, f[n]);
+        float f[8];
+        ka_widen(raw[n], f);
+        ka_turn(f, sn[row], cs[row], sub);
+        ka_store(out, sub, f);
       } else if (p.zero_rest) {
         const float none[8] = {};
         ka_store(out, sub, none);
@@ -87,46 +104,44 @@ __global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 3 : 1) kv8_append
   }
 
   // ---- a block of K and V
-  int s, slot;
+  int s, slot, row0, n;
+  long pos0;
   if (r.cu) {
     if (tid == 0) seq_s = -1;
     __syncthreads();
-    for (int i = tid; i < r.S; i += KA_THREADS)
-      if ((int)blockIdx.x >= (r.begin(i) >> 4) + 2 * i && (i + 1 == r.S || (int)blockIdx.x < (r.begin(i + 1) >> 4) + 2 * (i + 1))) seq_s = i;
+    for (int i = tid; i < r.S; i += KA_THREADS) {
+      const int begin = r.begin(i), end = r.end(i), next = i + 1 < r.S ? r.begin(i + 1) : 0;
+      const long pos = r.pos0[i];
+      if ((int)blockIdx.x >= (begin >> 4) + 2 * i && (i + 1 == r.S || (int)blockIdx.x < (next >> 4) + 2 * (i + 1))) seq_s = i, begin_s = begin, end_s = end, pos_s = pos;
+    }
     __syncthreads();
     s = seq_s;
     if (s < 0) return;
-    slot = (int)blockIdx.x - (r.begin(s) >> 4) - 2 * s;
+    row0 = begin_s, n = end_s - begin_s, pos0 = pos_s;
+    slot = (int)blockIdx.x - (row0 >> 4) - 2 * s;
   } else {
     s = blockIdx.x / p.slots_per_seq;
     if (s >= r.S) return;
     slot = blockIdx.x % p.slots_per_seq;
+    row0 = s * r.n, n = r.n, pos0 = r.pos0[s];
   }
-  const int row0 = r.begin(s), n = r.end(s) - row0;
-  const long pos0 = r.pos0[s], first = max(pos0, 0l), last = min(pos0 + n, (long)r.max_pages << p.c.shift) - 1;  // positions that are stored
+  const long first = max(pos0, 0l), last = min(pos0 + n, (long)r.max_pages << p.c.shift) - 1;  // positions that are stored
   const long block = (first >> 4) + slot;
   if (first > last || block > (last >> 4)) return;
   const int at = (int)(block << 4);  // the block's first position
   const int lo = (int)(max(first, (long)at) - at), hi = (int)(min(last, (long)at + 15) - at);  // its rows lo .. hi are new
   const int h = blockIdx.y * KA_HEADS + (warp >> 1);
   const bool is_v = warp & 1, turn = !is_v && p.inv_freq != nullptr;
-  float f[8][8];
+  KaRaw<T> raw[8];  // as they came: widened and rotated twice, for the largest value and for the codes, which costs less than
+                    // the registers that 64 values a thread would take
   const bool whole = lo == 0 && hi == 15;
   if (h < p.c.H) {
-    const T *src = (is_v ? p.v : p.k) + (size_t)h * KV8_D + (size_t)(row0 + (at - pos0)) * (is_v ? p.v_stride : p.k_stride);
     const long stride = is_v ? p.v_stride : p.k_stride;
-    if (whole) {
+    const T *src = (is_v ? p.v : p.k) + (size_t)h * KV8_D + (row0 + (at - pos0)) * stride;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ka_load(src + (2 * j + hw) * stride, sub, f[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = 2 * j + hw;
-        if (i >= lo && i <= hi) ka_load(src + i * stride, sub, f[j]);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[j][e] = 0.f;  // counts for nothing
-      }
+    for (int j = 0; j < 8; ++j) {
+      const int i = 2 * j + hw;
+      if (whole || (i >= lo && i <= hi)) ka_ask(src + i * stride, sub, raw[j]);
     }
   }
   const long page = kv8_page(p.c, r, s, at, tid == 0 ? p.status : nullptr);
@@ -142,55 +157,58 @@ __global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 3 : 1) kv8_append
   int8_t *dst = (is_v ? p.c.v : p.c.k) + ((at_head << p.c.shift) + in_page) * KV8_D;
   float *scale = (is_v ? p.c.vs : p.c.ks) + (at_head << (p.c.shift - 4)) + (in_page >> 4);
   const float was = older ? *scale : 0.f;
-  if (turn) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (whole || (2 * j + hw >= lo && 2 * j + hw <= hi)) ka_turn(f[j], sn[2 * j + hw], cs[2 * j + hw], sub);
-  }
+  auto row = [&](int j, float(&f)[8]) {
+    ka_widen(raw[j], f);
+    if (turn) ka_turn(f, sn[2 * j + hw], cs[2 * j + hw], sub);
+  };
   float most = 0.f, odd = 0.f;  // the largest; not 0 if a value is not finite
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 8; ++j) {
+    const int i = 2 * j + hw;
+    if (!whole && (i < lo || i > hi)) continue;
+    float f[8];
+    row(j, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e])), odd = fmaf(f[j][e], 0.f, odd);
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e])), odd = fmaf(f[e], 0.f, odd);
+  }
   const bool finite = odd == 0.f;
   if (!finite) {
     most = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+      const int i = 2 * j + hw;
+      if (i < lo || i > hi) continue;
+      float f[8];
+      ka_load((is_v ? p.v : p.k) + (size_t)h * KV8_D + (row0 + (at + i - pos0)) * (is_v ? p.v_stride : p.k_stride), sub, f);
+      if (turn) ka_turn(f, sn[i], cs[i], sub);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[j][e]) < CUDART_INF_F ? fabsf(f[j][e]) : 0.f);
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) < CUDART_INF_F ? fabsf(f[e]) : 0.f);
+    }
   }
   most = warp_max(most);
   float now = most * (1.f / 127.f);
   now = now < KA_LEAST_SCALE ? 0.f : now;
   now = fmaxf(was, now);
-  const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f, less = inv * (1.f - 0x1p-20f), more = inv * (1.f + 0x1p-20f);
+  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
   const bool slow = !finite || now == 0.f;
   __syncwarp();  // every lane has read the scale
   if (lane == 0) *scale = now;
-  if (whole) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t *d = reinterpret_cast<uint32_t *>(dst + (2 * j + hw) * KV8_D) + sub;
-      const uint2 w = kv8_codes(f[j], now, less, more, slow);
-      d[0] = w.x, d[16] = w.y;
-    }
-    return;
-  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int i = 2 * j + hw;
     uint32_t *d = reinterpret_cast<uint32_t *>(dst + i * KV8_D) + sub;
-    const bool again = i < lo && older && now > was;
-    if (again) {  // the values they stood for, at the new scale
+    float f[8];
+    if (whole || (i >= lo && i <= hi)) {
+      row(j, f);
+    } else if (i < lo && older && now > was) {  // the values they stood for, at the new scale
       const uint32_t a = d[0], b = d[16];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[j][e] = (float)(int8_t)(a >> (8 * e)) * was, f[j][4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
+      for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(a >> (8 * e)) * was, f[4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
+    } else {
+      continue;
     }
-    if (again || (i >= lo && i <= hi)) {
-      const uint2 w = kv8_codes(f[j], now, less, more, slow);
-      d[0] = w.x, d[16] = w.y;
-    }
+    const uint2 w = kv8_codes(f, now, inv, slow);
+    d[0] = w.x, d[16] = w.y;
   }
 }
 
@@ -201,17 +219,17 @@ template <typename T>
 __global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(const __grid_constant__ Kv8Cache c, const __grid_constant__ Kv8Rows r, T *k_out, T *v_out, int zero_rest, int *status) {
   constexpr int EACH = 16 / sizeof(T);  // codes that a thread has of a row
   __shared__ int row_seq[KR_ROWS];
-  __shared__ long row_at[KR_ROWS];  // page * H, or -1
+  __shared__ long row_pos[KR_ROWS], row_at[KR_ROWS];  // position; page * H, or -1
   __shared__ int row_in[KR_ROWS];
   const int tid = threadIdx.x, row0 = blockIdx.x * KR_ROWS;
   pdl_launch_dependents();
   pdl_wait();
-  kv8_rows_of<KR_ROWS, KR_THREADS>(r, row0, row_seq);
+  kv8_rows_of<KR_ROWS, KR_THREADS>(r, row0, row_seq, row_pos);
   if (tid < KR_ROWS) {
     const int s = row_seq[tid];
     long at = -1;
     if (s >= 0) {
-      const long pos = (long)r.pos0[s] + row0 + tid - r.begin(s);
+      const long pos = row_pos[tid];
       if (pos >= 0 && pos < (long)r.max_pages << c.shift) {
         const long page = kv8_page(c, r, s, (int)pos, blockIdx.y == 0 ? status : nullptr);
         at = page < 0 ? -1 : page * c.H;

@@ -173,7 +173,7 @@ __device__ __noinline__ void kd_append(int8_t *dst, float *scale, const __half *
   float now = most * (1.f / 127.f);
   now = now < KA_LEAST_SCALE ? 0.f : now;
   now = fmaxf(was, now);
-  const float inv = now > 0.f ? __fdividef(1.f, now) : 0.f, less = inv * (1.f - 0x1p-20f), more = inv * (1.f + 0x1p-20f);
+  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
   __syncwarp();  // every lane has read the scale
   if (lane == 0) *scale = now;
 #pragma unroll
@@ -187,7 +187,7 @@ __device__ __noinline__ void kd_append(int8_t *dst, float *scale, const __half *
       for (int e = 0; e < 4; ++e) f[j][e] = (float)(int8_t)(a >> (8 * e)) * was, f[j][4 + e] = (float)(int8_t)(b >> (8 * e)) * was;
     }
     if (again || (i >= lo && i <= hi)) {
-      const uint2 w = kv8_codes(f[j], now, less, more, !finite || now == 0.f);
+      const uint2 w = kv8_codes(f[j], now, inv, !finite || now == 0.f);
       d[0] = w.x, d[16] = w.y;
     }
   }

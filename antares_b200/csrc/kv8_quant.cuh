@@ -2,6 +2,8 @@
 #pragma once
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace ab200 {
@@ -9,75 +11,70 @@ namespace ab200 {
 constexpr float KA_LEAST_SCALE = 0x1p-100f;  // below it a block is held as zeros: quotients stay clear of subnormal arithmetic
 constexpr float KA_MAGIC = 12582912.f;       // 1.5 * 2^23: a number of less than 2^22 added to it is rounded to an integer, in the low bits
 
-// The code of x at scale s: the quotient x / s rounded to the nearest, ties to even, as if it had all its digits.  `inv` is
-// about 1 / s, so k is off by one at most; the two sums (each one rounding, so their signs are exact) say which side of the
-// middle between two codes x lies on.
-static __device__ __noinline__ int kv8_code(float x, float s, float inv) {
-  if (s == 0.f) return 0;
-  if (!(fabsf(x) < CUDART_INF_F)) return x > 0.f ? 127 : x < 0.f ? -127 : 0;
-  float k = rintf(x * inv);
-  const float up = fmaf(-(k + 0.5f), s, x), down = fmaf(-(k - 0.5f), s, x);
-  const bool odd = ((int)k & 1) != 0;
-  if (up > 0.f || (up == 0.f && odd)) k += 1.f;
-  else if (down < 0.f || (down == 0.f && odd)) k -= 1.f;
-  return (int)fminf(fmaxf(k, -127.f), 127.f);
-}
-// Eight of them, as two words.  Where the quotients by a scale 2^-20 smaller and larger round alike, so does the exact one;
-// elsewhere, about once in 10000 values, the slow way decides.  (It was most of the kernel's instructions for every value.)
+// The codes of eight values at scale s: the quotients x / s rounded to the nearest, ties to even, as if they had all their
+// digits.  k = x * inv rounded is off by one at most, and e = x - k s is exact: k is a small integer, x and s are fp32, and
+// what is left has the digits of the coarser of the two and is no larger than s.  So k is right where |e| is below half of s;
+// next to it, which is seldom, |e| and the last bit of k decide.  Two values an instruction.
 __device__ __forceinline__ uint64_t ka_pair(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ void ka_round(const uint64_t (&x)[4], float inv, uint32_t (&w)[2]) {
-  const uint64_t f = ka_pair(inv, inv), magic = ka_pair(KA_MAGIC, KA_MAGIC);
+__device__ __forceinline__ uint2 kv8_codes(const float (&x)[8], float s, float inv, bool odd_values) {
+  const uint64_t f = ka_pair(inv, inv), magic = ka_pair(KA_MAGIC, KA_MAGIC), less = ka_pair(-KA_MAGIC, -KA_MAGIC), minus = ka_pair(-s, -s);
+  const float half = 0.5f * s, below = __uint_as_float(__float_as_uint(half) - 1u);
+  uint32_t t[8];
+  float e[8];
+  bool near = odd_values;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t t[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint64_t r;
-      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x[2 * h + i]), "l"(f), "l"(magic));
-      asm("mov.b64 {%0, %1}, %2;" : "=r"(t[2 * i]), "=r"(t[2 * i + 1]) : "l"(r));
-    }
-    w[h] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t v = ka_pair(x[2 * i], x[2 * i + 1]);
+    uint64_t k, left;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(k) : "l"(v), "l"(f), "l"(magic));
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(t[2 * i]), "=r"(t[2 * i + 1]) : "l"(k));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(k) : "l"(k), "l"(less));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(left) : "l"(k), "l"(minus), "l"(v));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(e[2 * i]), "=f"(e[2 * i + 1]) : "l"(left));
+    near = near || fabsf(e[2 * i]) > below || fabsf(e[2 * i + 1]) > below;
   }
-}
-__device__ __forceinline__ uint2 kv8_codes(const float (&x)[8], float s, float inv_less, float inv_more, bool slow) {
-  const uint64_t v[4] = {ka_pair(x[0], x[1]), ka_pair(x[2], x[3]), ka_pair(x[4], x[5]), ka_pair(x[6], x[7])};
-  uint32_t w[2], u[2];
-  ka_round(v, inv_less, w);
-  ka_round(v, inv_more, u);
-  if (slow || w[0] != u[0] || w[1] != u[1]) {
-    const float inv = s > 0.f ? __fdividef(1.f, s) : 0.f;
+  if (near) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      w[h] = 0;
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        const float y = i == 0 ? x[4 * h] : i == 1 ? x[4 * h + 1] : i == 2 ? x[4 * h + 2] : x[4 * h + 3];
-        w[h] |= (uint32_t)(kv8_code(y, s, inv) & 255) << (8 * i);
-      }
+    for (int i = 0; i < 8; ++i) {
+      if (fabsf(e[i]) > (t[i] & 1u ? below : half)) t[i] += e[i] < 0.f ? -1 : 1;
+      if (odd_values) t[i] = s == 0.f || x[i] != x[i] ? 0u : x[i] == CUDART_INF_F ? 127u : x[i] == -CUDART_INF_F ? -127u : t[i];
     }
   }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) w[h] = __byte_perm(__byte_perm(t[4 * h], t[4 * h + 1], 0x0040), __byte_perm(t[4 * h + 2], t[4 * h + 3], 0x0040), 0x5410);
   return make_uint2(w[0], w[1]);
 }
 
-// dims 4 sub .. 4 sub + 3 and 64 + the same of a row: a rotated pair is one thread's
-__device__ __forceinline__ void ka_load(const __half *p, int sub, float (&f)[8]) {
+// A thread's part of a row, as it lies in memory: dims 4 sub .. 4 sub + 3 and 64 + the same, so a rotated pair is one thread's.
+template <typename T> struct KaRaw;
+template <> struct KaRaw<__half> { uint2 v[2]; };
+template <> struct KaRaw<float> { float4 v[2]; };
+template <typename T>
+__device__ __forceinline__ void ka_ask(const T *p, int sub, KaRaw<T> &r) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) r.v[half] = *reinterpret_cast<const std::remove_reference_t<decltype(r.v[0])> *>(p + 64 * half + 4 * sub);
+}
+__device__ __forceinline__ void ka_widen(const KaRaw<__half> &r, float (&f)[8]) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p + 64 * half + 4 * sub);
-    const float2 a = __half22float2(u2h2(v.x)), b = __half22float2(u2h2(v.y));
+    const float2 a = __half22float2(u2h2(r.v[half].x)), b = __half22float2(u2h2(r.v[half].y));
     f[4 * half] = a.x, f[4 * half + 1] = a.y, f[4 * half + 2] = b.x, f[4 * half + 3] = b.y;
   }
 }
-__device__ __forceinline__ void ka_load(const float *p, int sub, float (&f)[8]) {
+__device__ __forceinline__ void ka_widen(const KaRaw<float> &r, float (&f)[8]) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const float4 v = *reinterpret_cast<const float4 *>(p + 64 * half + 4 * sub);
-    f[4 * half] = v.x, f[4 * half + 1] = v.y, f[4 * half + 2] = v.z, f[4 * half + 3] = v.w;
-  }
+  for (int half = 0; half < 2; ++half) f[4 * half] = r.v[half].x, f[4 * half + 1] = r.v[half].y, f[4 * half + 2] = r.v[half].z, f[4 * half + 3] = r.v[half].w;
+}
+template <typename T>
+__device__ __forceinline__ void ka_load(const T *p, int sub, float (&f)[8]) {
+  KaRaw<T> r;
+  ka_ask(p, sub, r);
+  ka_widen(r, f);
 }
 __device__ __forceinline__ void ka_store(__half *p, int sub, const float (&f)[8]) {
 #pragma unroll
