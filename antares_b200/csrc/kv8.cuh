@@ -43,6 +43,10 @@ __device__ __forceinline__ long kv8_page(const Kv8Cache &c, const Kv8Rows &r, in
   return page;
 }
 
+// Rows of k and v into the cache, by a kernel that lets the one behind it start once what came before has ended: that one
+// waits for it before it reads a block from pos0 / 16 on (kv8_append.cu).
+int kv8_append_beside(const Kv8Cache &c, const Kv8Rows &r, const void *k, const void *v, long k_stride, long v_stride, const float *inv_freq, int dtype, cudaStream_t stream);
+
 // Host: checks what every entry point checks of a cache and its rows.
 inline int kv8_check(const char *who, const void *k, const void *v, const void *ks, const void *vs, int pages, int page_rows, int Hkv, const void *table,
                      long table_stride, int max_pages, const void *pos0, const void *cu, int S, int T, Kv8Cache *c, Kv8Rows *r) {

@@ -26,6 +26,7 @@ struct AppendParams {
   int zero_rest;
   int slots_per_seq;  // cu == nullptr
   int kv_groups;
+  int beside;                // the kernel behind this one starts before it ends: what came before it has ended by then
   int *status;
 };
 
@@ -65,8 +66,9 @@ __global__ void __launch_bounds__(KA_THREADS, sizeof(T) == 2 ? 4 : 1) kv8_append
   __shared__ long pos_s, row_pos[KV8_BLOCK];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane & 15, hw = lane >> 4;
   const Kv8Rows &r = p.r;
-  pdl_launch_dependents();
+  if (!p.beside) pdl_launch_dependents();
   pdl_wait();
+  if (p.beside) pdl_launch_dependents();
 
   if ((int)blockIdx.y >= p.kv_groups) {  // ---- rotate query rows
     const int row0 = blockIdx.x * KV8_BLOCK;
@@ -278,14 +280,19 @@ __global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(const __grid_const
 
 template <typename T>
 static int append_launch(const Kv8Cache &c, const Kv8Rows &r, const void *k, const void *v, long k_stride, long v_stride, const void *q, long q_stride, void *q_out,
-                         long q_out_stride, int Hq, const float *inv_freq, int zero_rest, cudaStream_t stream) {
+                         long q_out_stride, int Hq, const float *inv_freq, int zero_rest, int beside, cudaStream_t stream) {
   AppendParams<T> p{c, r, (const T *)k, (const T *)v, (const T *)q, (T *)q_out, k_stride, v_stride, q_stride, q_out_stride, Hq, inv_freq, zero_rest, (r.n + 14) / 16 + 1,
-                    (c.H + KA_HEADS - 1) / KA_HEADS, kernel_error_ptr()};
+                    (c.H + KA_HEADS - 1) / KA_HEADS, beside, kernel_error_ptr()};
   const long slots = r.cu ? (long)r.T / 16 + 2l * r.S : (long)r.S * p.slots_per_seq;
   const int q_groups = q ? (Hq + KA_Q_HEADS - 1) / KA_Q_HEADS : 0;
   const long x = q && (r.T + 15) / 16 > slots ? (r.T + 15) / 16 : slots;
   AB200_CUDA(launch_pdl(kv8_append_kernel<T>, dim3((unsigned)x, p.kv_groups + q_groups), dim3(KA_THREADS), 0, stream, p));
   return AB200_OK;
+}
+
+int kv8_append_beside(const Kv8Cache &c, const Kv8Rows &r, const void *k, const void *v, long k_stride, long v_stride, const float *inv_freq, int dtype, cudaStream_t stream) {
+  if (dtype == AB200_F16) return append_launch<__half>(c, r, k, v, k_stride, v_stride, nullptr, 0, nullptr, 0, 0, inv_freq, 0, 1, stream);
+  return append_launch<float>(c, r, k, v, k_stride, v_stride, nullptr, 0, nullptr, 0, 0, inv_freq, 0, 1, stream);
 }
 
 template <typename T>
@@ -321,8 +328,8 @@ extern "C" int ab200_kv8_append(void *k_cache, void *v_cache, float *k_scale, fl
     AB200_REQUIRE(Hq > 0 && Hq <= 65535 && q_stride % vec == 0 && q_out_stride % vec == 0 && q_stride >= (long)Hq * KV8_D && q_out_stride >= (long)Hq * KV8_D && aligned16(q) &&
                       aligned16(q_out), "kv8_append: q and q_out must be 16-byte aligned rows of at least %d values, a multiple of 16 bytes apart", Hq * KV8_D);
   }
-  if (dtype == AB200_F16) return append_launch<__half>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, zero_rest, (cudaStream_t)stream);
-  return append_launch<float>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, zero_rest, (cudaStream_t)stream);
+  if (dtype == AB200_F16) return append_launch<__half>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, zero_rest, 0, (cudaStream_t)stream);
+  return append_launch<float>(c, r, k, v, k_stride, v_stride, q, q_stride, q_out, q_out_stride, Hq, inv_freq, zero_rest, 0, (cudaStream_t)stream);
 }
 
 extern "C" int ab200_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int pages, int page_rows, int Hkv,

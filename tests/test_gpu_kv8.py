@@ -317,6 +317,36 @@ def test_step(cuda, past, n, hq, hkv, page, rope, dtype):
     assert ops.kernel_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_in_a_row(cuda, captured, dtype):
+    """A step's rows are written beside its attention's start and read by it: the bits of one call after the other, step by step,
+    over the ends of blocks, with scales that grow (older rows of the block change too)."""
+    past, hq, hkv, steps = [int(n) for n in np.random.RandomState(3).randint(0, 900, 30)], 16, 8, 24
+    past[0] = 899
+    cache, table = _setup(33, past, [steps] * len(past), hkv, 32)
+    apart = [t.clone() for t in cache]
+    q, k, v = (_randn(i, steps, len(past), h, 128, dtype=dtype) for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    k, v = (t * (1 + 0.2 * torch.arange(steps, device="cuda")).to(dtype)[:, None, None, None] for t in (k, v))
+    pos0 = [_ints([n + i for n in past]) for i in range(steps)]
+    run = lambda: [ops.kv8_step(q[i], k[i], v[i], cache, table, pos0[i]) for i in range(steps)]  # noqa: E731
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run()
+        graph.replay()
+    else:
+        outs = run()
+    torch.cuda.synchronize()
+    for i in range(steps):
+        ops.kv8_append(apart, k[i], v[i], table, pos0[i])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], ops.kv8_attention(q[i], apart, table, pos0[i])), i
+    for a, b in zip(cache, apart):
+        assert torch.equal(a.view(torch.int8), b.view(torch.int8))
+    assert ops.kernel_status() == 0
+
+
 def test_a_bad_page_is_reported(cuda):
     """Entries that name no page: nothing is written there, the status says so, and the next call is well."""
     for rows in (1, 150):

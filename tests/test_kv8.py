@@ -1,5 +1,6 @@
 """The 8-bit paged cache on the CPU: what its calls refuse before any kernel runs."""
 import ctypes
+import re
 
 import numpy as np
 import pytest
@@ -101,3 +102,28 @@ def test_the_reference_keeps_half_a_step():
     k, _ = c.values(0, 41)
     step = np.repeat(np.concatenate([c.ks[2], c.ks[0]], 1), 16, 1).T[:41, :, None]
     assert (np.abs(k[:40] - x) <= step[:40] * 1.0001).all() and (np.abs(k[40:] - y) <= step[40:] * 0.5000001).all()
+
+
+def test_workspace_sizes_are_enough_for_every_call():
+    """A call without a workspace says how much it needs, which the functions that size one must cover: whichever kernels serve it."""
+    import random
+    L = _lib.load()
+    rng, fake = random.Random(1), 4096
+    for _ in range(4000):
+        hkv = rng.choice([1, 1, 2, 3, 8, 32])
+        hq = hkv * rng.choice([1, 2, 5, 8, 33, 64, 65, 128])
+        S, n = rng.choice([1, 2, 3, 16, 500]), rng.choice([1, 2, 3, 17, 64, 300, 2000])
+        T, shift, dtype = S * n, rng.randrange(4, 9), rng.randrange(2)
+        if T * hq > 1 << 30:
+            continue
+        cu = fake if rng.random() < 0.5 else None
+        most = rng.choice([0, 1, n, T]) if cu else n
+        max_pages = max(1, 2 ** rng.randrange(4, 22) >> shift)
+        stride = (hq + 2) * 128
+        cache = (fake, fake, fake, fake, 64, 1 << shift, hkv, fake, max_pages, max_pages, fake)
+        assert L.ab200_kv8_attention(fake, stride, fake, *cache, cu, S, T, most, hq, 128, 0.1, 1, dtype, None, 0, None) != 0
+        need = int(re.search(r"workspace of (\d+) bytes, got 0", L.ab200_last_error().decode()).group(1))
+        assert need <= L.ab200_kv8_attention_workspace_bytes(S, T, most, hq, hkv), (hkv, hq, S, n, cu, most, max_pages, shift, dtype)
+        assert L.ab200_kv8_step(fake, fake, fake, stride, stride, stride, fake, *cache, S, T, hq, 128, rng.choice([None, fake]), 0.1, dtype, None, 0, None) != 0
+        need = int(re.search(r"workspace of (\d+) bytes, got 0", L.ab200_last_error().decode()).group(1))
+        assert need <= L.ab200_kv8_attention_workspace_bytes(S, T, n, hq, hkv), (hkv, hq, S, n, max_pages, shift, dtype)
