@@ -102,6 +102,19 @@ def test_attention(cuda, past, rows, hq, hkv, page, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("past,rows,hq,hkv", [([5000], [1], 64, 64), ([int(n) for n in np.random.RandomState(1).randint(-1, 700, 150)], [1] * 150, 4, 2),
+                                              ([int(n) for n in np.random.RandomState(2).randint(-3, 400, 40)], [0, 1, 2, 7] * 10, 8, 2), ([3], [1], 64, 64)])
+def test_shares_of_two_sizes(cuda, past, rows, hq, hkv, dtype):
+    """Room for so many positions that the work is cut into large shares and small ones: items in one, two or a hundred of them."""
+    cache, table = _setup(41, past, rows, hkv, 64)
+    table, q = _wide(table, 64), _randn(1, sum(rows), hq, 128, dtype=dtype, mul=2)
+    cu = None if len(set(rows)) == 1 else np.cumsum([0] + rows)
+    got = ops.kv8_attention(q, cache, table, _ints(past), cu_rows=None if cu is None else _cu(rows), max_rows=max(rows))
+    _check_attention(got, _ref(cache, table), q, past, cu, max(p + n for p, n in zip(past, rows)), dtype)
+    assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("mul", [0.0, 24.0])
 @pytest.mark.parametrize("past,rows,hq,hkv", [([333, 64], [1, 1], 8, 2), ([50], [140], 4, 1), ([50], [140], 32, 4), ([0, 60], [140, 140], 32, 32)])
 def test_flat_and_sharp_scores(cuda, past, rows, hq, hkv, mul, dtype):
@@ -318,13 +331,14 @@ def test_step(cuda, past, n, hq, hkv, page, rope, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
-@pytest.mark.parametrize("captured", [False, True])
-def test_steps_in_a_row(cuda, captured, dtype):
+@pytest.mark.parametrize("captured,wide", [(False, False), (True, False), (False, True)])
+def test_steps_in_a_row(cuda, captured, wide, dtype):
     """A step's rows are written beside its attention's start and read by it: the bits of one call after the other, step by step,
     over the ends of blocks, with scales that grow (older rows of the block change too)."""
     past, hq, hkv, steps = [int(n) for n in np.random.RandomState(3).randint(0, 900, 30)], 16, 8, 24
     past[0] = 899
     cache, table = _setup(33, past, [steps] * len(past), hkv, 32)
+    table = _wide(table, 32) if wide else table
     apart = [t.clone() for t in cache]
     q, k, v = (_randn(i, steps, len(past), h, 128, dtype=dtype) for i, h in ((1, hq), (2, hkv), (3, hkv)))
     k, v = (t * (1 + 0.2 * torch.arange(steps, device="cuda")).to(dtype)[:, None, None, None] for t in (k, v))
