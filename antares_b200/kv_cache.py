@@ -77,8 +77,8 @@ class PagePool:
         self.rows[seq] = rows
 
     def reserve(self, need):
-        """Makes room for need[seq] more rows of each sequence: new pages, and an own copy of a last page that is shared and
-        partly filled.  Returns the (source, destination) pages to copy before anything is written."""
+        """Makes room for need[seq] more rows of each sequence: new pages, and own ones in place of those that are shared and will
+        be written.  Returns the (source, destination) pages to copy before anything is written: those partly filled."""
         fresh, own = {}, {}
         users = {}
         for seq, n in need.items():
@@ -90,20 +90,20 @@ class PagePool:
             if want > self.max_pages:
                 raise CacheFull("sequence %d: %d rows are more than its %d pages hold" % (seq, end, self.max_pages))
             fresh[seq] = max(0, want - have)
-            at = self.rows[seq] // self.page_rows
-            if n > 0 and self.rows[seq] % self.page_rows:
+            for at in range(self.rows[seq] // self.page_rows, min(have, want) if n else 0):
                 page = self.held[seq][at]
                 left = users.setdefault(page, self.users[page])
                 if left > 1:   # the last one of those that write keeps the page
-                    own[seq] = at
+                    own[seq, at] = self.rows[seq] > at * self.page_rows
                     users[page] = left - 1
         total = sum(fresh.values()) + len(own)
         if total > len(self._free):
             raise CacheFull("%d pages are needed, %d are free" % (total, len(self._free)))
         copies = []
-        for seq, at in own.items():
+        for (seq, at), filled in own.items():
             new, old = heapq.heappop(self._free), self.held[seq][at]
-            copies.append((old, new))
+            if filled:
+                copies.append((old, new))
             self.users[new] = 1
             self.held[seq][at] = new
             self._drop(old)
@@ -137,7 +137,8 @@ class PagePool:
 
 class PagedKV8Cache:
     """The 8-bit cache of a model's layers.  layer(l) is what the ops.kv8_* calls take, batch(seqs) their page table and
-    positions.  A serving step: reserve({seq: rows}), then per layer kv8_step or kv8_append + kv8_attention, then advance()."""
+    positions (columns without a page hold -1: rows that were not reserved are not written, and kernel_status says so).  A
+    serving step: reserve({seq: rows}), then per layer kv8_step or kv8_append + kv8_attention, then advance()."""
 
     def __init__(self, layers, pages, kv_heads, page_rows=64, max_seqs=64, max_seq=None, device="cuda"):
         if page_rows < 16 or page_rows & (page_rows - 1):
@@ -184,7 +185,9 @@ class PagedKV8Cache:
 
     def batch(self, seqs):
         """(page_table int32 [len(seqs), max_pages], pos0 int32 [len(seqs)]) on the device: where the sequences' next rows go."""
-        table = torch.zeros(len(seqs), self.pool.max_pages, dtype=torch.int32)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is in a batch once, got %r" % (list(seqs),))
+        table = torch.full((len(seqs), self.pool.max_pages), -1, dtype=torch.int32)
         for i, s in enumerate(seqs):
             pages = self.pool.held[s]
             table[i, :len(pages)] = torch.tensor(pages, dtype=torch.int32)

@@ -436,11 +436,12 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
  * ab200_kernel_status.
  * The call's rows: T rows of S sequences, sequence s has rows cu_rows_dev[s] .. cu_rows_dev[s + 1] - 1 (int32 [S + 1];
  * NULL: T / S each) at the positions pos0_dev[s], pos0_dev[s] + 1, ... (int32 [S]).  Rows behind the last sequence's are
- * left as they were (zero_rest: become zeros).  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the results; rows may be
- * strided (in elements, a multiple of 16 bytes), the heads of a row lie together. */
+ * left as they were (zero_rest: become zeros).  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the
+ * results; rows may be strided (in elements, a multiple of 16 bytes), the heads of a row lie together.  Sequences may share pages
+ * that a call reads; the blocks of 16 rows that it writes belong to one sequence of the call. */
 
 /* Writes the rows of k and v [T][Hkv][128] into the cache.  inv_freq (fp32, 64 values used; NULL: none) rotates k by halves
- * at the rows' positions first, and q [T][Hq][128] into q_out (both NULL: no queries; q_out may be q).  For each block that
+ * at the rows' positions first, and q [T][Hq][128] into q_out (both NULL: no queries; q_out may be q, not k or v).  For each block that
  * new rows lie in and each head: scale = max(scale of the block if it holds rows before pos0, else 0; largest |value| of
  * the new rows times 1/127, all fp32), codes = value / scale rounded to the nearest, ties to even; rows before the new ones are rounded again
  * if their scale grew; codes behind the new rows stay as they are.  8 bits hold no infinities or NaN: +-inf becomes the

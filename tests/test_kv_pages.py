@@ -49,7 +49,7 @@ def test_any_order_of_calls(seed):
     m = Model(40, rng.choice([1, 4, 16]))
     for t in range(400):
         seqs = sorted(m.want)
-        what = rng.choice(["add", "write", "write", "write", "fork", "free", "truncate", "compact"])
+        what = rng.choice(["add", "write", "write", "write", "fork", "free", "truncate", "compact", "reserve"])
         try:
             if what == "add":
                 m.want[m.pool.add()] = []
@@ -61,6 +61,8 @@ def test_any_order_of_calls(seed):
                 s = rng.choice(seqs)
                 if what == "write":
                     m.write(rng.sample(seqs, rng.randrange(1, len(seqs) + 1)), rng.randrange(0, 9), t)
+                elif what == "reserve":   # room that is not used before something else happens
+                    m.copy(m.pool.reserve({s: rng.randrange(20)}))
                 elif what == "fork":
                     m.want[m.pool.fork(s)] = list(m.want[s])
                 elif what == "free":
@@ -91,6 +93,24 @@ def test_the_last_writer_keeps_the_page():
     d = m.pool.fork(a)
     m.want[d] = list(m.want[a])
     assert m.pool.reserve({d: 1}) == [] and m.pool.users[m.pool.held[d][0]] == 2
+
+
+def test_forks_of_room_that_is_reserved_but_not_written():
+    """Pages of rows to come are shared by a fork like any other; whoever writes first gets pages of its own, nothing to copy."""
+    for rows in (0, 16, 20):
+        m = Model(12, 16)
+        a = m.pool.add()
+        m.want[a] = []
+        m.write([a], rows, 0)
+        m.copy(m.pool.reserve({a: 36}))
+        b = m.pool.fork(a)
+        m.want[b] = list(m.want[a])
+        copies = m.pool.reserve({a: 36})
+        assert len(copies) == (rows % 16 > 0)
+        m.copy(copies)
+        m.write([a], 36, 1)
+        m.write([b], 36, 2)
+        m.check()
 
 
 def test_what_does_not_fit_changes_nothing():
@@ -129,4 +149,7 @@ def test_batches_on_the_host():
     c.advance(a, 20)
     table, pos0 = c.batch([b, a])
     assert table.shape == (2, 3) and pos0.tolist() == [0, 20] and table[1, :2].tolist() == c.pool.held[a]
+    assert table[0, 1:].tolist() == [-1, -1] and table[1, 2] == -1
+    with pytest.raises(ValueError, match="once"):
+        c.batch([a, a])
     assert len(c.layer(1)) == 4 and c.layer(1)[2].shape == (6, 2, 1)
