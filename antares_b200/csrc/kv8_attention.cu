@@ -371,10 +371,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
                     is_v ? nullptr : p.inv_freq);
         }
       }
-      if (here) {
-        __threadfence();
-        __syncthreads();
-      }
+      if (here) __syncthreads();  // who reads the block is of this CTA
     }
     if (p.beside == KD_BESIDE_APPEND) fresh = (int)(max(it.pos0, 0l) >> 4);
     live = min(it.b1, (limit_of(it.last) + 15) >> 4);  // blocks that hold a key some row attends to
@@ -943,9 +940,10 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   if (rc) return rc;
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= a.bytes, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", a.bytes, workspace_bytes);
   // fp16 rows that fit into one tile are written by the attention kernel itself where an item is a cluster's (us, together /
-  // apart: one request of 384 positions and 32 heads 11.0 / 12.9; 48 ragged ones in equal shares 69 / 55: each new block's 4 us
-  // then is one CTA's, and the others wait for it at the end).  Else by a launch that the attention kernel starts beside, and only
-  // waits for where it reads those rows: 51.3 for the 48, against 54.5 one after the other.
+  // apart: one request of 384 positions and 32 heads 9.7 / 9.7 step behind step, 13.5 / 15.2 with a read of the rows behind each; 48
+  // ragged ones in equal shares 69 / 55: each new block's 4 us then is one CTA's, and the others wait for it at the end).  Else by
+  // a launch that the attention kernel starts beside, and only waits for where it reads those rows: 51.3 for the 48, against 54.5 one
+  // after the other.
   const bool together = dtype == AB200_F16 && !a.prompts && a.d.splits > 0 && a.d.tiles == 1;
   const bool beside = !together && !a.prompts;
   if (beside) rc = kv8_append_beside(c, r, k, v, k_stride, v_stride, inv_freq, dtype, (cudaStream_t)stream);
