@@ -704,8 +704,11 @@ struct Joined {
     m = up;
   }
 };
+// BATCH parts are loaded at once.  With 8 a thread has 79 registers and an SM three CTAs, with 4 64 and four; us, 8 / 4, the whole call
+// among others: one sequence of 131072 positions 57 / 62, 48 ragged requests 58.7 / 61; tiles of 16 rows, 16 sequences of four 24.1 / 22.5.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_constant__ DecodeParams p, int ctas) {
+  constexpr int BATCH = ROWS == 8 ? 8 : 4;
   __shared__ float4 acc_s[KJ_WARPS][32];
   __shared__ float2 ml_s[KJ_WARPS];
   pdl_launch_dependents();
@@ -721,22 +724,29 @@ __global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_const
     const bool none = row < sp.z >> 20;
     kd_store4(out, a.acc, none ? 0.f : 1.f / a.l);
   };
+  // the parts of an item that two CTAs share, before it is known whether there is one
+  float2 s0[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float4 v0[2] = {};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (c0 + warp + i < ctas) s0[i] = ml[part(c0 + warp, i)], v0[i] = acc[part(c0 + warp, i) * (KV8_D / 4)];
   for (int k = 0; k < KJ_WARPS; ++k) {
     const int4 sp = make_int4(__shfl_sync(0xffffffffu, my.x, k), __shfl_sync(0xffffffffu, my.y, k), __shfl_sync(0xffffffffu, my.z, k), __shfl_sync(0xffffffffu, my.w, k));
     if (sp.x == 0 || row > (sp.z >> 16 & 15) || (sp.x <= KJ_WARPS && k != warp)) continue;
     const int step = sp.x <= KJ_WARPS ? 1 : KJ_WARPS;
     Joined a;
-    for (int i0 = step == 1 ? 0 : warp; i0 < sp.x; i0 += 8 * step) {
-      float2 s[8];
-      float4 v[8];
+    if (step == 1) a.add(s0[0], v0[0]), a.add(s0[1], v0[1]);  // two at least
+    for (int i0 = step == 1 ? 2 : warp; i0 < sp.x; i0 += BATCH * step) {
+      float2 s[BATCH];
+      float4 v[BATCH];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < BATCH; ++j) {
         const int i = i0 + j * step;
         s[j] = i < sp.x ? ml[part(c0 + k, i)] : make_float2(-CUDART_INF_F, 0.f);
         v[j] = i < sp.x ? acc[part(c0 + k, i) * (KV8_D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.add(s[j], v[j]);
+      for (int j = 0; j < BATCH; ++j) a.add(s[j], v[j]);
     }
     if (step > 1) {  // every warp is here
       __syncthreads();
