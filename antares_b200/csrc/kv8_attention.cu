@@ -14,8 +14,8 @@
 // Bound by memory: 257 bytes for a position and kv head.  Few rows read all of it, so the warp's own matrix instructions serve:
 // their 16 rows are filled by 8 packed rows and their second parts, codes go in as they are, and what a warp keeps of a block
 // stays in its registers (the 5th-generation tensor cores would want 64 rows and codes widened to 16 bits in shared memory).
-// us (TB/s): 64 sequences, all of 16000 positions, 8 kv heads of 4 query heads 334 (6.3, 96 % of a copy's rate); one of 131072 and
-// 32 kv heads 177 (6.1); one of 131072 and 8 kv heads 59 (4.6); 64 ragged ones of up to 8000, 8 heads of 8 108.6 (5.1).  Where a share is
+// us (TB/s): 64 sequences, all of 16000 positions, 8 kv heads of 4 query heads 323 (6.5, 99 % of a copy's rate); one of 131072 and
+// 32 kv heads 170 (6.3); one of 131072 and 8 kv heads 54 (5.0); 64 ragged ones of up to 8000, 8 heads of 8 107 (5.2).  Where a share is
 // small, starting an item (7800 cycles) and the second launch weigh: 48 ragged ones of up to 4000 45 us (4.4), of one request of
 // 384 positions 7.0 us only a tenth is the stream.  16 rows a tile: products and exponentials bound it, twice a block's instructions.
 #include <math_constants.h>
@@ -34,7 +34,6 @@ constexpr int KD_WARPS = 4, KD_THREADS = KD_WARPS * 32, KD_STAGES = 4;
 constexpr int KD_STAGE_BYTES = 2 * KV8_BLOCK * KV8_D;  // a block of K, a block of V
 constexpr int KD_LEAST = 8;                            // blocks a CTA takes at least, two a warp
 constexpr int KD_ITEM = 16;                            // what an item costs besides its blocks, in blocks: 7800 cycles against 470 a block
-constexpr int KD_LATE = 8;                             // one part in this many of the work is small shares (5: 109.8 us, 8: 108.5, 12: 110.2)
 constexpr float KD_RAISE = 8.f, KD_P_EXP = 6.f;        // P is scaled by 2^6: its second half stays out of fp16's subnormals
 constexpr float KD_LEAST_SCALE = 0x1p-100f;            // a V scale below it (a block of zeros) counts as this
 
@@ -52,7 +51,6 @@ struct DecodeParams {
   long k_stride, v_stride;
   int zero_rest;             // rows behind the last sequence's become zeros
   int few;                   // sequences with more rows than this (rows x group) are another kernel's
-  int late;                  // the grid is twice the CTAs that fit: those of its second half have small shares
   int splits, tiles;         // FIXED: CTAs of an item; tiles of a sequence's rows
   int beside;                // KD_BESIDE_*: the kernel before in the stream runs beside this one, which only ends after it
   float *partial;            // [CTAs][2][rows][128], then [CTAs][2][rows][2]: maximum, sum
@@ -236,23 +234,17 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       reinterpret_cast<uint4 *>(p.out)[i] = make_uint4(0, 0, 0, 0);
   }
 
-  // The CTAs of the grid's second half start where one of the first has ended: SMs do not get the same bandwidth, and those
-  // that are done early take more of them.
-  const int first_half = gridDim.x >> 1;
-  const int share = FIXED || !p.late ? blockIdx.x : blockIdx.x < first_half ? 2 * blockIdx.x : 2 * (blockIdx.x - first_half) + 1;
   // ---- this CTA's share: w0 .. w1 - 1 of all work, ordered by sequence, kv head, tile, block
-  long total = 0, start = 0, weight = 0, per = 1, big = 0, w0 = 0, w1 = 0;
+  long total = 0, start = 0, weight = 0, per = 1, w0 = 0, w1 = 0;
   if constexpr (!FIXED) {
     for (int base = 0; base < r.S; base += KD_THREADS) {
       weight = base + tid < r.S ? kd_weight<ROWS>(p, base + tid) * p.c.H : 0;
       const long before = total;
       start = before + kd_scan(weight, scan_s, &total);
     }
-    const int halves = gridDim.x >> p.late;
-    per = max((long)kd_div(total + halves - 1, halves), (long)KD_LEAST);
-    big = per - (p.late ? per / KD_LATE : 0);
-    w0 = (share >> p.late) * per + (share & p.late ? big : 0), w1 = min((share >> p.late) * per + (share & p.late || !p.late ? per : big), total);
-    if (tid == 0) p.split[share] = make_int4(0, 0, 0, 0);
+    per = max((long)kd_div(total + gridDim.x - 1, gridDim.x), (long)KD_LEAST);
+    w0 = blockIdx.x * per, w1 = min(w0 + per, total);
+    if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (w0 >= w1) {
       if (p.beside) pdl_wait();
       return;
@@ -644,7 +636,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       const int packed = done.first + row, token = packed / p.group, head = done.hk * p.group + packed - token * p.group;
       T *out = (T *)p.out + ((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + col;
       // a part to be joined: FIXED into the ring's other half, else to memory
-      float *part = FIXED ? reinterpret_cast<float *>(smem) + row * KV8_D + col : p.partial + (((size_t)share * 2 + slot) * ROWS + row) * KV8_D + col;
+      float *part = FIXED ? reinterpret_cast<float *>(smem) + row * KV8_D + col : p.partial + (((size_t)blockIdx.x * 2 + slot) * ROWS + row) * KV8_D + col;
       const float over = row < empty ? 0.f : 1.f / sum;
 #pragma unroll
       for (int c = 0; c < PIECES; ++c) {
@@ -660,7 +652,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       if (FIXED) {
         if (col == 0) q_max_s[0][row] = mx, q_max_s[1][row] = sum;
       } else if (!whole && col == 0)
-        reinterpret_cast<float2 *>(p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D)[((size_t)share * 2 + slot) * ROWS + row] = make_float2(mx, sum);
+        reinterpret_cast<float2 *>(p.partial + (size_t)gridDim.x * 2 * ROWS * KV8_D)[((size_t)blockIdx.x * 2 + slot) * ROWS + row] = make_float2(mx, sum);
     }
     if constexpr (FIXED) {
       if (p.splits > 1) {
@@ -681,11 +673,9 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
         }
         cluster.sync();  // nobody leaves while its memory is read
       }
-    } else if (!whole && slot == 1 && tid == 0) {  // begun here: the shares up to the one with the item's last block have the rest
-      const long end = done.item + KD_ITEM + done.blocks - 1, whose = kd_div(end, per);
-      const int last = p.late ? (int)(2 * whose + (end - whose * per >= big)) : (int)whose;
-      p.split[share] = make_int4(last - share + 1, done.row0, done.hk | (done.last - done.first) << 16 | empty << 20, done.first);
-    }
+    } else if (!whole && slot == 1 && tid == 0)  // begun here: the CTAs up to the one with the item's last block have the rest
+      p.split[blockIdx.x] = make_int4((int)kd_div(done.item + KD_ITEM + done.blocks - 1, per) - (int)blockIdx.x + 1, done.row0,
+                                      done.hk | (done.last - done.first) << 16 | empty << 20, done.first);
   }
   if (p.beside) pdl_wait();
 }
@@ -704,8 +694,10 @@ struct Joined {
     m = up;
   }
 };
-// BATCH parts are loaded at once.  With 8 a thread has 79 registers and an SM three CTAs, with 4 64 and four; us, 8 / 4, the whole call
-// among others: one sequence of 131072 positions 57 / 62, 48 ragged requests 58.7 / 61; tiles of 16 rows, 16 sequences of four 24.1 / 22.5.
+// BATCH parts are loaded at once, the first two before it is known whether there are any.  With 8 a thread has 79 registers and an
+// SM three CTAs, with 4 64 and four; us, 8 / 4, the whole call among others (which start while the kernel before still runs): one
+// sequence of 131072 positions 57 / 62, 48 ragged requests 58.7 / 61; tiles of 16 rows, 16 sequences of four 24.1 / 22.5.  Before, with 64
+// registers and parts asked for when known: 64.8, 63.3, 23.0, and 377 for 64 sequences of 16000 positions (323 now).
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_constant__ DecodeParams p, int ctas) {
   constexpr int BATCH = ROWS == 8 ? 8 : 4;
@@ -764,7 +756,7 @@ __global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_const
 
 // ---- host --------------------------------------------------------------------------------------------------------
 struct DecodePlan {
-  int rows, ctas, late;
+  int rows, ctas;
   int splits;  // > 0: an item to a cluster of this many CTAs; 0: equal shares and a second launch that joins them
   int tiles;
   size_t partial_bytes, bytes;
@@ -774,8 +766,8 @@ static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool 
   const long group = Hq / Hkv;
   d.rows = (long)max_rows * group <= 8 ? 8 : 16;
   d.ctas = sm_count() * (d.rows == 8 ? 3 : 2);
-  d.partial_bytes = (size_t)2 * d.ctas * 2 * d.rows * (KV8_D + 2) * sizeof(float);
-  d.bytes = d.partial_bytes + (size_t)2 * d.ctas * sizeof(int4);
+  d.partial_bytes = (size_t)d.ctas * 2 * d.rows * (KV8_D + 2) * sizeof(float);
+  d.bytes = d.partial_bytes + (size_t)d.ctas * sizeof(int4);
   // One launch where no CTA then has 24 blocks more to do than its equal share (what the lookups and the second launch take):
   // one sequence as long as its pages allow, of several the longest so long and half as much in the mean.
   // us, clusters / equal shares: one request of 384 positions and 32 heads 6.7 / 10.8; five of up to 1000 12.8 / 16.1;
@@ -783,10 +775,6 @@ static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool 
   const long tiles = ((long)(T / S) * group + d.rows - 1) / d.rows, items = S * Hkv * tiles, blocks = (capacity + 15) / 16;
   d.tiles = (int)tiles;
   d.splits = 0;
-  // Small shares behind the others where those may have 400 blocks, so that it pays to begin once more.  us, without / with, blocks a share
-  // (half of it in the mean where ragged): 64 ragged sequences of up to 4000 and 8 heads 288: 63.2 / 65.5; of 6000 432: 86.6 / 88.2; 32 of
-  // 12000 432: 102 / 90; 64 of 8000 577: 116 / 108.5; one of 131072 and 32 heads 590: 209 / 177; 64 all of 16000 1153: 377 / 334.
-  d.late = items * blocks / d.ctas >= 400;
   if (uniform && items <= d.ctas) {
     int c = 1;
     while (c < 8 && items * c * 2 <= d.ctas) c *= 2;
@@ -818,10 +806,8 @@ static int decode_launch(DecodeParams p, const DecodePlan &d, cudaStream_t strea
     return AB200_OK;
   }
   AB200_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<T, ROWS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int grid = d.ctas << d.late;
-  p.late = d.late;
-  AB200_CUDA(launch_pdl(kv8_decode_kernel<T, ROWS, false>, dim3(grid), dim3(KD_THREADS), smem, stream, p));
-  AB200_CUDA(launch_pdl(kv8_join_kernel<T, ROWS>, dim3((grid + KJ_WARPS - 1) / KJ_WARPS, ROWS), dim3(KJ_THREADS), 0, stream, p, grid));
+  AB200_CUDA(launch_pdl(kv8_decode_kernel<T, ROWS, false>, dim3(d.ctas), dim3(KD_THREADS), smem, stream, p));
+  AB200_CUDA(launch_pdl(kv8_join_kernel<T, ROWS>, dim3((d.ctas + KJ_WARPS - 1) / KJ_WARPS, ROWS), dim3(KJ_THREADS), 0, stream, p, d.ctas));
   return AB200_OK;
 }
 
@@ -847,7 +833,6 @@ static int attend_plan(const Kv8Cache &c, const Kv8Rows &r, int max_rows, int Hq
   a->prompts = most * group > KD_FEW && (long)r.T * Hq * capacity > KD_PROMPT_WORK && !rotate;
   a->few = !a->prompts || r.cu != nullptr;
   a->d = decode_plan(r.S, r.T, a->few && a->prompts ? std::max(KD_FEW / group, 1) : (int)most, Hq, c.H, r.cu == nullptr, capacity);
-  if (a->prompts) a->d.late = 0;  // how many rows are left for it is not known here
   a->p = Kv8PrefillParams{};
   a->p.c = c, a->p.r = r, a->p.group = group;
   size_t prompt_bytes = 0;
@@ -877,7 +862,7 @@ static int attend(const char *who, const Kv8Cache &c, const Kv8Rows &r, const vo
   if (a.few) {
     char *ws = (char *)workspace + (a.bytes - a.d.bytes);
     DecodeParams p{c, r, q, q_stride, out, Hq, group, scale2, inv_freq, new_rows.k, new_rows.v, new_rows.k_stride, new_rows.v_stride, zero_rest && r.cu,
-                   a.prompts ? KD_FEW : 0x7fffffff, 0, 0, 0, a.prompts && pdl_enabled() ? KD_BESIDE_PROMPTS : appending && pdl_enabled() ? KD_BESIDE_APPEND : KD_BESIDE_NONE, (float *)ws, (int4 *)(ws + a.d.partial_bytes), status};
+                   a.prompts ? KD_FEW : 0x7fffffff, 0, 0, a.prompts && pdl_enabled() ? KD_BESIDE_PROMPTS : appending && pdl_enabled() ? KD_BESIDE_APPEND : KD_BESIDE_NONE, (float *)ws, (int4 *)(ws + a.d.partial_bytes), status};
     if (dtype == AB200_F32) rc = a.d.rows == 8 ? decode_launch<float, 8>(p, a.d, stream) : decode_launch<float, 16>(p, a.d, stream);
     else rc = a.d.rows == 8 ? decode_launch<__half, 8>(p, a.d, stream) : decode_launch<__half, 16>(p, a.d, stream);
     if (rc) return rc;

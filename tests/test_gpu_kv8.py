@@ -104,8 +104,8 @@ def test_attention(cuda, past, rows, hq, hkv, page, dtype):
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("past,rows,hq,hkv", [([5000], [1], 64, 64), ([int(n) for n in np.random.RandomState(1).randint(-1, 700, 150)], [1] * 150, 4, 2),
                                               ([int(n) for n in np.random.RandomState(2).randint(-3, 400, 40)], [0, 1, 2, 7] * 10, 8, 2), ([3], [1], 64, 64)])
-def test_shares_of_two_sizes(cuda, past, rows, hq, hkv, dtype):
-    """Room for so many positions that the work is cut into large shares and small ones: items in one, two or a hundred of them."""
+def test_shares_of_long_and_short_items(cuda, past, rows, hq, hkv, dtype):
+    """Equal shares of all work whatever room the tables have: items in one share, in two and in many, shares of many items."""
     cache, table = _setup(41, past, rows, hkv, 64)
     table, q = _wide(table, 64), _randn(1, sum(rows), hq, 128, dtype=dtype, mul=2)
     cu = None if len(set(rows)) == 1 else np.cumsum([0] + rows)
