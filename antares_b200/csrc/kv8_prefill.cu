@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       ap_arrive(bar_p);
     }
     // ---- O / l: a thread's row through its own idle query memory, then stored as whole rows; or its part, to be joined
-    if (good && my_n > 1) good = __all_sync(0xffffffffu, kp_wait(bar_o, (my_n - 2) & 1, &fail_s));
+    // The product before the last is complete: the last scores' second half was only issued after it.  A wait for it here could
+    // come after the last one has ended too, whose phase looks like the one before it.
     if (good && my_n > 0) good = __all_sync(0xffffffffu, kp_wait(bar_o, (my_n - 1) & 1, &fail_s));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (!good) {
