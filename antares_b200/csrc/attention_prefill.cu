@@ -393,12 +393,16 @@ __global__ void __launch_bounds__(AP_THREADS, 2) attention_prefill_kernel(AttnPr
       put(r1, 16);
       l += l0 + l1;
       ap_wait_st();
+      // Before the last arrival: the last tile's MMAs are only issued after it, so the phase before theirs cannot be hidden by their
+      // own (it would look like the one before it), nor pass for it in the wait behind the loop.  Costs nothing: they wait for it too.
+      if (j > 0 && j + 1 == tiles && !__all_sync(0xffffffffu, ap_wait(b_odone, (tiles - 2) & 1))) {
+        good = false;
+        break;
+      }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       ap_arrive(b_pfull + 8 * (j & 1));
     }
     // ---- O / l, rounded, parked row by row in the idle Q and ring memory, then stored as whole 256-byte rows
-    // the last tile but one first: its MMAs need not be complete yet, and a barrier two phases behind looks complete
-    if (good && tiles > 1) good = __all_sync(0xffffffffu, ap_wait(b_odone, (tiles - 2) & 1));
     if (good && tiles > 0) good = __all_sync(0xffffffffu, ap_wait(b_odone, (tiles - 1) & 1));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (!good) {

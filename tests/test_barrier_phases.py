@@ -111,3 +111,39 @@ def test_the_model_finds_both_faults():
         explore(mma, [w + [("wait", "o", 1), ("wait", "o", 0)] + last for w in bare], dict(s0=1, s1=1, p=2, o=1, read=2))
     with pytest.raises(Stuck, match="before it is complete"):
         explore(mma, [w + last for w in bare], dict(s0=1, s1=1, p=2, o=1, read=2))
+
+
+def _fp16_waits():
+    """What the softmax warps of attention_prefill.cu wait for of O: before their arrival with the last tile's P, and behind it; offsets
+    from the number of tiles."""
+    text = _source("attention_prefill.cu")
+    loop, tail = text.split("// ---- softmax: thread = query row")[1].split("// ---- O / l, rounded")
+    find = lambda t: [int(n) for n in re.findall(r"ap_wait\(b_odone, \(tiles - (\d)\) & 1", t)]  # noqa: E731
+    return find(loop.split("ap_arrive(b_pfull")[0]), find(tail.split("if (!good)")[0])
+
+
+def _fp16(n, raises):
+    mma = [("issue", ("s", 0)), ("commit", "s0")]
+    for j in range(n):
+        if j > 0:
+            mma += [("wait", "o", (j - 1) & 1)]
+        if j + 1 < n:
+            mma += [("issue", ("s", j + 1)), ("commit", "s%d" % (j + 1 & 1))]
+        mma += [("wait", "p%d" % (j & 1), j >> 1 & 1), ("issue", ("o", j)), ("commit", "o")]
+    early, late = _fp16_waits()
+    warp = []
+    for j in range(n):
+        warp += [("wait", "s%d" % (j & 1), j >> 1 & 1), ("needs", ("s", j))]
+        if raises and j > 0:
+            warp += [("wait", "o", (j - 1) & 1), ("needs", ("o", j - 1))]
+        if j == n - 1:
+            warp += [("wait", "o", (n - k) & 1) for k in early if n >= k]
+        warp += [("arrive", "p%d" % (j & 1))]
+    warp += [("wait", "o", (n - k) & 1) for k in late if n >= k]
+    return mma, [warp + [("needs", ("o", n - 1))] for _ in range(2)]
+
+
+@pytest.mark.parametrize("raises", [False, True])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5])
+def test_the_prompt_kernel_over_the_fp16_cache(n, raises):
+    explore(*_fp16(n, raises), dict(s0=1, s1=1, p0=2, p1=2, o=1))
