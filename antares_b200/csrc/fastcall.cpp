@@ -398,8 +398,8 @@ struct Kv8Call {
   long table_stride;
   const void *table, *pos0, *cu;
 };
-// the cache (a tuple or list of four), page table, positions and offsets (or None) of a call
-bool kv8_call(PyObject *cache, PyObject *table, PyObject *pos0, PyObject *cu, int device, Kv8Call *c) {
+// the cache (a tuple or list of four), page table, positions and offsets (or None) of a call; `writes`: no two sequences have one table row
+bool kv8_call(PyObject *cache, PyObject *table, PyObject *pos0, PyObject *cu, bool writes, int device, Kv8Call *c) {
   if (!PyTuple_Check(cache) && !PyList_Check(cache)) return false;
   if (PySequence_Fast_GET_SIZE(cache) != 4) return false;
   const Tensor *t[4], *tab, *pos, *off = nullptr;
@@ -413,11 +413,12 @@ bool kv8_call(PyObject *cache, PyObject *table, PyObject *pos0, PyObject *cu, in
     return false;
   if (!(tab = plain_strided(table, device)) || tab->dim() != 2 || tab->scalar_type() != at::kInt || (tab->size(1) > 1 && tab->stride(1) != 1)) return false;
   const int64_t S = tab->size(0);
+  if (S > 1 && tab->stride(0) < tab->size(1) && (writes || tab->stride(0) != 0)) return false;
   if (S <= 0 || !(pos = plain_strided(pos0, device)) || !pos->is_contiguous() || pos->scalar_type() != at::kInt || pos->numel() != S) return false;
   if (cu != Py_None && (!(off = plain_strided(cu, device)) || !off->is_contiguous() || off->scalar_type() != at::kInt || off->numel() != S + 1)) return false;
   if (k.size(0) > INT32_MAX || k.size(1) > INT32_MAX || rows > INT32_MAX || tab->size(1) > INT32_MAX || S > INT32_MAX) return false;
   *c = Kv8Call{k.data_ptr(), t[1]->data_ptr(), s.data_ptr(), t[3]->data_ptr(), (int)k.size(0), (int)rows, (int)k.size(1), (int)tab->size(1), (int)S,
-               std::max<long>(tab->stride(0), tab->size(1)), tab->data_ptr(), pos->data_ptr(), off ? off->data_ptr() : nullptr};
+               S > 1 ? (long)tab->stride(0) : (long)tab->size(1), tab->data_ptr(), pos->data_ptr(), off ? off->data_ptr() : nullptr};
   return true;
 }
 inline int current_device() { return c10::cuda::current_device(); }
@@ -441,7 +442,7 @@ PyObject *py_kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Kv8Call c;
     long stride, most;
     float scale;
-    if (n != 7 || !(q = plain_strided(a[0], device)) || q->dim() != 3 || !kv8_call(a[1], a[2], a[3], a[4], device, &c)) NOT_HERE;
+    if (n != 7 || !(q = plain_strided(a[0], device)) || q->dim() != 3 || !kv8_call(a[1], a[2], a[3], a[4], false, device, &c)) NOT_HERE;
     const int code = code_of(*q);
     const int64_t T = q->size(0), hq = q->size(1);
     if (code < 0 || !rows3(*q, q->scalar_type(), T, -1, &stride) || hq % c.heads || T > INT32_MAX || hq > INT32_MAX || (!c.cu && T % c.S)) NOT_HERE;
@@ -476,7 +477,7 @@ PyObject *py_kv8_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
     long qs, ks, vs;
     float scale;
     if (n != 8 || !(q = plain_strided(a[0], device)) || !(k = plain_strided(a[1], device)) || !(v = plain_strided(a[2], device)) || q->dim() != 3) NOT_HERE;
-    if (!kv8_call(a[3], a[4], a[5], Py_None, device, &c) || (a[6] != Py_None && !(f = inv_freq_arg(a[6], device)))) NOT_HERE;
+    if (!kv8_call(a[3], a[4], a[5], Py_None, true, device, &c) || (a[6] != Py_None && !(f = inv_freq_arg(a[6], device)))) NOT_HERE;
     const int code = code_of(*q);
     const int64_t T = q->size(0), hq = q->size(1);
     if (code < 0 || !rows3(*q, q->scalar_type(), T, -1, &qs) || !rows3(*k, q->scalar_type(), T, c.heads, &ks) || !rows3(*v, q->scalar_type(), T, c.heads, &vs)) NOT_HERE;
@@ -502,7 +503,7 @@ PyObject *py_kv8_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor *k, *v, *q = nullptr, *f = nullptr;
     Kv8Call c;
     long ks, vs, qs = 0;
-    if (n != 8 || !(k = plain_strided(a[1], device)) || !(v = plain_strided(a[2], device)) || k->dim() != 3 || !kv8_call(a[0], a[3], a[4], a[5], device, &c)) NOT_HERE;
+    if (n != 8 || !(k = plain_strided(a[1], device)) || !(v = plain_strided(a[2], device)) || k->dim() != 3 || !kv8_call(a[0], a[3], a[4], a[5], true, device, &c)) NOT_HERE;
     if ((a[6] != Py_None && !(q = plain_strided(a[6], device))) || (a[7] != Py_None && !(f = inv_freq_arg(a[7], device))) || (q && !f)) NOT_HERE;
     const int code = code_of(*k);
     const int64_t T = k->size(0);
@@ -528,7 +529,7 @@ PyObject *py_kv8_read(PyObject *, PyObject *const *a, Py_ssize_t n) {
   GUARDED({
     const int device = current_device();
     Kv8Call c;
-    if (n != 6 || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[5]) || !kv8_call(a[0], a[1], a[2], a[4], device, &c)) NOT_HERE;
+    if (n != 6 || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[5]) || !kv8_call(a[0], a[1], a[2], a[4], false, device, &c)) NOT_HERE;
     const long T = PyLong_AsLong(a[3]), code = PyLong_AsLong(a[5]);
     if (PyErr_Occurred() || T <= 0 || T > INT32_MAX || code < 0 || code > 1 || (!c.cu && T % c.S)) {
       PyErr_Clear();

@@ -2,7 +2,8 @@
 //
 //   k, v      int8 [pages][Hkv][page_rows][128]         value = code * scale, codes -127 .. 127
 //   ks, vs    fp32 [pages][Hkv][page_rows / 16]         one scale for each 16 rows (a block) and head
-//   table     int32 [S][table_stride], max_pages in use; position p of sequence s is row p % page_rows of page table[s][p / page_rows]
+//   table     int32 [S][table_stride], max_pages in use; position p of sequence s is row p % page_rows of page table[s][p / page_rows];
+//             table_stride 0: one row for all of them, where nothing is written
 //
 // A head's rows of a page lie together: a block is 2 KiB of consecutive memory and shares its scale, so a reader takes
 // 16 keys and two scales at a time whatever the page size (a power of two from 16).
@@ -47,15 +48,15 @@ __device__ __forceinline__ long kv8_page(const Kv8Cache &c, const Kv8Rows &r, in
 // waits for it before it reads a block from pos0 / 16 on (kv8_append.cu).
 int kv8_append_beside(const Kv8Cache &c, const Kv8Rows &r, const void *k, const void *v, long k_stride, long v_stride, const float *inv_freq, int dtype, cudaStream_t stream);
 
-// Host: checks what every entry point checks of a cache and its rows.
-inline int kv8_check(const char *who, const void *k, const void *v, const void *ks, const void *vs, int pages, int page_rows, int Hkv, const void *table,
+// Host: checks what every entry point checks of a cache and its rows.  `writes`: a table row is one sequence's alone.
+inline int kv8_check(const char *who, bool writes, const void *k, const void *v, const void *ks, const void *vs, int pages, int page_rows, int Hkv, const void *table,
                      long table_stride, int max_pages, const void *pos0, const void *cu, int S, int T, Kv8Cache *c, Kv8Rows *r) {
   int shift = 0;
   while (shift < 30 && (1 << shift) < page_rows) ++shift;
   AB200_REQUIRE(page_rows >= KV8_BLOCK && (1 << shift) == page_rows, "%s: page_rows=%d must be a power of two from %d", who, page_rows, KV8_BLOCK);
   AB200_REQUIRE(pages > 0 && Hkv > 0 && Hkv <= 65535, "%s: bad cache, pages=%d heads=%d", who, pages, Hkv);
   AB200_REQUIRE((long)pages * Hkv << (shift - 4) < 1l << 31, "%s: %d pages of %d heads and %d rows are more blocks than the built 2^31", who, pages, Hkv, page_rows);
-  AB200_REQUIRE(S >= 0 && T >= 0 && max_pages > 0 && table_stride >= max_pages, "%s: bad shape S=%d T=%d max_pages=%d table_stride=%ld", who, S, T, max_pages, table_stride);
+  AB200_REQUIRE(S >= 0 && T >= 0 && max_pages > 0 && (table_stride >= max_pages || (table_stride == 0 && !writes)), "%s: bad shape S=%d T=%d max_pages=%d table_stride=%ld", who, S, T, max_pages, table_stride);
   AB200_REQUIRE((long)max_pages << shift <= 1l << 30, "%s: %d pages of %d rows are more positions than the built 2^30", who, max_pages, page_rows);
   AB200_REQUIRE(T <= 1 << 28 && S <= 1 << 20, "%s: T=%d rows of S=%d sequences are beyond the built limits", who, T, S);
   AB200_REQUIRE(cu != nullptr || S == 0 || T % S == 0, "%s: %d rows do not divide into %d sequences (cu_rows says how many each has)", who, T, S);

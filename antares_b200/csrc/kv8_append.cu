@@ -315,7 +315,7 @@ extern "C" int ab200_kv8_append(void *k_cache, void *v_cache, float *k_scale, fl
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
-  const int rc = kv8_check("kv8_append", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
+  const int rc = kv8_check("kv8_append", true, k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (rc) return rc;
   AB200_REQUIRE(dtype == AB200_F16 || dtype == AB200_F32, "kv8_append: unknown dtype %d", dtype);
   if (S == 0 || T == 0) return AB200_OK;
@@ -338,7 +338,7 @@ extern "C" int ab200_kv8_read(const void *k_cache, const void *v_cache, const fl
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
-  const int rc = kv8_check("kv8_read", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
+  const int rc = kv8_check("kv8_read", false, k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (rc) return rc;
   AB200_REQUIRE(dtype == AB200_F16 || dtype == AB200_F32, "kv8_read: unknown dtype %d", dtype);
   if (S == 0 || T == 0) return AB200_OK;

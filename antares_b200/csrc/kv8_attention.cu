@@ -911,7 +911,7 @@ extern "C" int ab200_kv8_attention(const void *q, long q_stride, void *out, cons
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
-  int rc = kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
+  int rc = kv8_check("kv8_attention", false, k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, cu_rows_dev, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_attention", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc) return rc;
   return attend("kv8_attention", c, r, q, q_stride, out, max_rows, Hq, scale, dtype, nullptr, NewRows{}, false, zero_rest, workspace, workspace_bytes, (cudaStream_t)stream);
@@ -924,7 +924,7 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   clear_error();
   Kv8Cache c;
   Kv8Rows r;
-  int rc = kv8_check("kv8_step", k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, &c, &r);
+  int rc = kv8_check("kv8_step", true, k_cache, v_cache, k_scale, v_scale, pages, page_rows, Hkv, page_table, table_stride, max_pages, pos0_dev, nullptr, S, T, &c, &r);
   if (!rc) rc = attention_check("kv8_step", c, T, q, q_stride, out, Hq, D, dtype);
   if (rc || S == 0 || T == 0) return rc;
   const long vec = dtype == AB200_F16 ? 8 : 4;

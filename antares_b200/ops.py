@@ -323,11 +323,12 @@ def row_program(rp, mats, cols, out=None, out_dtype=None):
 # ---- a paged KV cache held in 8 bits ---------------------------------------------------------------------------
 # A layer's cache is four tensors (k, v, k_scale, v_scale): int8 [pages, kv heads, page rows, 128] twice, fp32 [pages, kv
 # heads, page rows / 16] twice; a value is code * scale.  kv_cache.PagedKV8Cache keeps the pages of many sequences.
-# `page_table` int32 [S, max_pages]: position p of sequence s is row p % page_rows of page table[s, p // page_rows].
+# `page_table` int32 [S, max_pages]: position p of sequence s is row p % page_rows of page table[s, p // page_rows].  A table that
+# is only read may be one row expanded over the sequences.
 # `pos0` int32 [S]: the position of each sequence's first row of the call.  `cu_rows` int32 [S + 1]: which rows are whose
 # (None: as many for each).  The tensors' device is the one that works, whichever is current.
 
-def _kv8_args(cache, page_table, pos0, cu_rows, T, q=None):
+def _kv8_args(cache, page_table, pos0, cu_rows, T, q=None, writes=False):
     """The cache and row arguments of a kv8 entry point; checks what only tensors can say."""
     k, v, ks, vs = cache
     if k.dim() != 4 or k.shape[3] != 128 or v.shape != k.shape:
@@ -340,13 +341,16 @@ def _kv8_args(cache, page_table, pos0, cu_rows, T, q=None):
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_cuda or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError("page_table must be a CUDA int32 tensor [sequences, pages] with consecutive columns")
     S = page_table.shape[0]
+    stride = page_table.stride(0) if S > 1 else page_table.shape[1]
+    if stride < page_table.shape[1] and (writes or stride):
+        raise ValueError("the rows of page_table may not overlap%s" % (" where pages are written" if stride == 0 else ""))
     if pos0.numel() != S or (cu_rows is not None and cu_rows.numel() != S + 1):
         raise ValueError("%d sequences need %d positions in pos0 and %d offsets in cu_rows" % (S, S, S + 1))
     for t in (v, ks, vs, page_table, pos0, cu_rows, q):
         if t is not None and t.device != k.device:
             raise ValueError("the tensors of a kv8 call lie on one device (%s and %s)" % (k.device, t.device))
     return (_chk(k, "k cache", torch.int8), _chk(v, "v cache", torch.int8), _chk(ks, "k_scale", torch.float32), _chk(vs, "v_scale", torch.float32),
-            pages, rows, heads, page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), page_table.shape[1], _chk(pos0, "pos0", torch.int32),
+            pages, rows, heads, page_table.data_ptr(), stride, page_table.shape[1], _chk(pos0, "pos0", torch.int32),
             0 if cu_rows is None else _chk(cu_rows, "cu_rows", torch.int32), S, T)
 
 
@@ -383,7 +387,7 @@ def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=Non
         raise ValueError("q_out without q")
     if q is not None and inv_freq is None:
         raise ValueError("q is only rotated: it needs inv_freq")
-    args = _kv8_args(cache, page_table, pos0, cu_rows, T, k)
+    args = _kv8_args(cache, page_table, pos0, cu_rows, T, k, writes=True)
     kp, k_stride = _rows3(k, "k", k.dtype, heads=args[6])
     vp, v_stride = _rows3(v, "v", k.dtype, T, args[6])
     fp = 0
@@ -486,7 +490,7 @@ def kv8_step(q, k, v, cache, page_table, pos0, inv_freq=None, scale=None, out=No
         if y is not None:
             return y
     T, hq = q.shape[0], q.shape[1]
-    args = _kv8_args(cache, page_table, pos0, None, T, q)
+    args = _kv8_args(cache, page_table, pos0, None, T, q, writes=True)
     qp, q_stride = _rows3(q, "q", q.dtype)
     kp, k_stride = _rows3(k, "k", q.dtype, T, args[6])
     vp, v_stride = _rows3(v, "v", q.dtype, T, args[6])

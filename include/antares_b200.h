@@ -431,9 +431,9 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
  *   k_cache, v_cache  int8 [pages][Hkv][page_rows][128], 16-byte aligned; value = code * scale, codes -127 .. 127
  *   k_scale, v_scale  fp32 [pages][Hkv][page_rows / 16], one for each block of 16 rows and head
  * page_rows is a power of two from 16.  page_table int32 [S][table_stride], its first max_pages columns in use: position p
- * of sequence s is row p % page_rows of page table[s][p / page_rows].  Entries of positions that a call does not touch are
- * not read.  An entry outside 0 .. pages - 1 that it does touch writes nothing, reads as zeros or as page 0, and shows in
- * ab200_kernel_status.
+ * of sequence s is row p % page_rows of page table[s][p / page_rows]; ab200_kv8_read and ab200_kv8_attention also take a
+ * table_stride of 0: one row for all sequences.  Entries of positions that a call does not touch are not read.  An entry
+ * outside 0 .. pages - 1 that it does touch writes nothing, reads as zeros or as page 0, and shows in ab200_kernel_status.
  * The call's rows: T rows of S sequences, sequence s has rows cu_rows_dev[s] .. cu_rows_dev[s + 1] - 1 (int32 [S + 1];
  * NULL: T / S each) at the positions pos0_dev[s], pos0_dev[s] + 1, ... (int32 [S]).  Rows behind the last sequence's are
  * left as they were (zero_rest: become zeros).  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the

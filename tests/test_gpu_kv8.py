@@ -555,3 +555,25 @@ def test_pages_of_many_sequences(cuda):
     write({b: 30, d: 1, e: 1})
     check()
     assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rows,hq", [(1, 8), (3, 8), (100, 32)])
+def test_a_page_table_row_that_sequences_share(cuda, rows, hq, dtype):
+    """An expanded table: as many sequences over one prompt, each with its own queries."""
+    S, past = 5, 300
+    cache, table = _setup(51, [past], [rows], 2, 32)
+    table = _wide(table, 32)
+    q, pos0 = _randn(1, S * rows, hq, 128, dtype=dtype), _ints([past, 0, past - 7, 40, 299])
+    shared = table.expand(S, -1)
+    assert torch.equal(ops.kv8_attention(q, cache, shared, pos0), ops.kv8_attention(q, cache, shared.contiguous(), pos0))
+    for a, b in zip(ops.kv8_read(cache, shared, pos0, S * rows), ops.kv8_read(cache, shared.contiguous(), pos0, S * rows)):
+        assert torch.equal(a, b)
+    before = [t.clone() for t in cache]
+    k = q[:, :2]
+    for f in (lambda: ops.kv8_append(cache, k, k, shared, pos0), lambda: ops.kv8_step(q, k, k, cache, shared, pos0),
+              lambda: ops.kv8_attention(q, cache, table[0].as_strided((S, 8), (1, 1)), pos0)):
+        with pytest.raises(ValueError, match="overlap|written"):
+            f()
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, before))
+    assert ops.kernel_status() == 0

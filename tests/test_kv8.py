@@ -127,3 +127,44 @@ def test_workspace_sizes_are_enough_for_every_call():
         assert L.ab200_kv8_step(fake, fake, fake, stride, stride, stride, fake, *cache, S, T, hq, 128, rng.choice([None, fake]), 0.1, dtype, None, 0, None) != 0
         need = int(re.search(r"workspace of (\d+) bytes, got 0", L.ab200_last_error().decode()).group(1))
         assert need <= L.ab200_kv8_attention_workspace_bytes(S, T, n, hq, hkv), (hkv, hq, S, n, max_pages, shift, dtype)
+
+
+class OnGpu(torch.Tensor):
+    """A tensor that says it lies on a GPU: for the host's checks of arguments, which look no further."""
+    is_cuda = property(lambda self: True)
+
+
+def _gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+def _host_cache(pages=4, heads=2, rows=16):
+    return tuple(_gpu(t) for t in (torch.zeros(pages, heads, rows, 128, dtype=torch.int8), torch.zeros(pages, heads, rows, 128, dtype=torch.int8),
+                                   torch.zeros(pages, heads, rows // 16), torch.zeros(pages, heads, rows // 16)))
+
+
+def test_page_tables_whose_rows_overlap():
+    """Sequences may share one row of a table that is only read; the kernels step through a table by its own stride."""
+    cache, pos0 = _host_cache(), _gpu(torch.zeros(3, dtype=torch.int32))
+    one = torch.tensor([[2, 1, 3]], dtype=torch.int32)
+    table = _gpu(one.expand(3, -1))
+    args = ops._kv8_args(cache, table, pos0, None, 3)
+    assert args[8] == 0 and args[9] == 3 and args[12] == 3
+    with pytest.raises(ValueError, match="written"):
+        ops._kv8_args(cache, table, pos0, None, 3, writes=True)
+    windows = _gpu(torch.arange(6, dtype=torch.int32).as_strided((3, 3), (1, 1)))
+    for writes in (False, True):
+        with pytest.raises(ValueError, match="overlap"):
+            ops._kv8_args(cache, windows, pos0, None, 3, writes=writes)
+        # one row has no stride to speak of
+        assert ops._kv8_args(cache, _gpu(one.expand(1, -1)), pos0[:1], None, 1, writes=writes)[8] >= 3
+        assert ops._kv8_args(cache, _gpu(torch.zeros(3, 8, dtype=torch.int32)[:, :3]), pos0, None, 3, writes=writes)[8] == 8
+    # the C entry points: readers take it (and ask for a workspace next), writers do not
+    rc, text = _attention(stride=0)
+    assert rc == _lib.EINVAL and "workspace" in text
+    rc, text = _append(stride=0)
+    assert rc == _lib.EINVAL and "table_stride=0" in text
+    L = _lib.load()
+    assert L.ab200_kv8_step(4096, 4096, 4096, 512, 256, 256, 4096, 4096, 4096, 4096, 4096, 8, 32, 2, 4096, 0, 4, 4096, 2, 2, 4, 128, None, 0.1, 0, None, 0, None) == _lib.EINVAL
+    assert "table_stride=0" in L.ab200_last_error().decode()
+    assert _append(stride=-4)[0] == _lib.EINVAL and _attention(stride=-4)[0] == _lib.EINVAL
