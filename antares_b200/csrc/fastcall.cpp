@@ -406,7 +406,8 @@ bool kv8_call(PyObject *cache, PyObject *table, PyObject *pos0, PyObject *cu, bo
   for (int i = 0; i < 4; ++i)
     if (!(t[i] = plain_strided(PySequence_Fast_GET_ITEM(cache, i), device)) || !t[i]->is_contiguous()) return false;
   const Tensor &k = *t[0], &s = *t[2];
-  if (k.dim() != 4 || k.scalar_type() != at::kChar || t[1]->scalar_type() != at::kChar || t[1]->sizes() != k.sizes() || k.size(3) != KV8_D) return false;
+  if (k.dim() != 4 || k.scalar_type() != at::kChar || t[1]->scalar_type() != at::kChar || t[1]->sizes() != k.sizes() || k.size(3) != KV8_D || k.size(0) == 0 || k.size(1) == 0)
+    return false;
   const int64_t rows = k.size(2);
   if (rows < 16 || (rows & (rows - 1)) || s.dim() != 3 || s.scalar_type() != at::kFloat || t[3]->scalar_type() != at::kFloat || t[3]->sizes() != s.sizes() ||
       s.size(0) != k.size(0) || s.size(1) != k.size(1) || s.size(2) != rows / 16)

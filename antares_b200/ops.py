@@ -334,6 +334,8 @@ def _kv8_args(cache, page_table, pos0, cu_rows, T, q=None, writes=False):
     if k.dim() != 4 or k.shape[3] != 128 or v.shape != k.shape:
         raise ValueError("a kv8 cache holds k and v int8 [pages, kv heads, page rows, 128], got %s and %s" % (tuple(k.shape), tuple(v.shape)))
     pages, heads, rows, _ = k.shape
+    if pages == 0 or heads == 0:
+        raise ValueError("a kv8 cache with no heads or no pages holds nothing, got %s" % (tuple(k.shape),))
     if rows < 16 or rows & (rows - 1):
         raise ValueError("a kv8 cache's pages hold a power of two of rows, 16 or more; got %d" % rows)
     if ks.shape != (pages, heads, rows // 16) or vs.shape != ks.shape:

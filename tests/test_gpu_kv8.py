@@ -577,3 +577,15 @@ def test_a_page_table_row_that_sequences_share(cuda, rows, hq, dtype):
             f()
     assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, before))
     assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("pages,heads", [(4, 0), (0, 2)])
+def test_a_cache_without_heads_or_pages(cuda, pages, heads):
+    """Refused by both front ends (the native one divides by the heads)."""
+    i8, f32 = dict(dtype=torch.int8, device="cuda"), dict(dtype=F32, device="cuda")
+    cache = (torch.zeros(pages, heads, 16, 128, **i8), torch.zeros(pages, heads, 16, 128, **i8), torch.zeros(pages, heads, 1, **f32), torch.zeros(pages, heads, 1, **f32))
+    table, q, k = torch.zeros(1, 2, dtype=torch.int32, device="cuda"), _randn(1, 1, 4, 128), torch.zeros(1, heads, 128, dtype=F16, device="cuda")
+    for f in (lambda: ops.kv8_attention(q, cache, table, _ints([0])), lambda: ops.kv8_step(q, k, k, cache, table, _ints([0])), lambda: ops.kv8_append(cache, k, k, table, _ints([0])),
+              lambda: ops.kv8_read(cache, table, _ints([0]), 1)):
+        with pytest.raises(ValueError, match="no heads or no pages"):
+            f()

@@ -168,3 +168,14 @@ def test_page_tables_whose_rows_overlap():
     assert L.ab200_kv8_step(4096, 4096, 4096, 512, 256, 256, 4096, 4096, 4096, 4096, 4096, 8, 32, 2, 4096, 0, 4, 4096, 2, 2, 4, 128, None, 0.1, 0, None, 0, None) == _lib.EINVAL
     assert "table_stride=0" in L.ab200_last_error().decode()
     assert _append(stride=-4)[0] == _lib.EINVAL and _attention(stride=-4)[0] == _lib.EINVAL
+
+
+@pytest.mark.parametrize("pages,heads", [(4, 0), (0, 2)])
+def test_a_cache_without_heads_or_pages_is_refused(pages, heads):
+    cache, x = _host_cache(pages, heads), _gpu(torch.zeros(1, 4, 128).half())
+    table, pos0 = _gpu(torch.zeros(1, 2, dtype=torch.int32)), _gpu(torch.zeros(1, dtype=torch.int32))
+    k = _gpu(torch.zeros(1, heads, 128).half())
+    for f in (lambda: ops.kv8_attention(x, cache, table, pos0), lambda: ops.kv8_step(x, k, k, cache, table, pos0), lambda: ops.kv8_append(cache, k, k, table, pos0),
+              lambda: ops.kv8_read(cache, table, pos0, 1)):
+        with pytest.raises(ValueError, match="no heads or no pages"):
+            f()
