@@ -254,8 +254,9 @@ __global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(const __grid_const
       w[i][which] = make_uint2(0, 0), f[i][which] = 0.f;
       if (at >= 0) {
         const int8_t *src = (which ? c.v : c.k) + (((at + h) << c.shift) + row_in[i]) * KV8_D + in_head;
-        if constexpr (EACH == 8) w[i][which] = ldg_nc_v2(src);
-        else w[i][which].x = __ldg(reinterpret_cast<const uint32_t *>(src));
+        // not as read-only data: the append before may still run when this kernel starts
+        if constexpr (EACH == 8) w[i][which] = __ldcg(reinterpret_cast<const uint2 *>(src));
+        else w[i][which].x = __ldcg(reinterpret_cast<const uint32_t *>(src));
         f[i][which] = (which ? c.vs : c.ks)[((at + h) << (c.shift - 4)) + (row_in[i] >> 4)];
       }
     }

@@ -589,3 +589,44 @@ def test_a_cache_without_heads_or_pages(cuda, pages, heads):
               lambda: ops.kv8_read(cache, table, _ints([0]), 1)):
         with pytest.raises(ValueError, match="no heads or no pages"):
             f()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_other_rows_over_the_same_pages_call_behind_call(cuda, dtype, captured):
+    """Append and read in turn with nothing between them, other values each time at the same positions: every read has the rows of
+    the append right before it."""
+    past, rows, heads, turns = [0, 32, 5], [48, 1, 20], 8, 12
+    cache, table = _setup(61, past, rows, heads, 32, filled=False)
+    # the positions before: held already, so that every block that is read has been written
+    first = _randn(7, sum(past), heads, 128, dtype=dtype)
+    ops.kv8_append(cache, first, first, table, _ints([0, 0, 0]), cu_rows=_cu(past))
+    start = [t.clone() for t in cache]
+    T, cu, pos0 = sum(rows), _cu(rows), _ints(past)
+    k, v = (_randn(i, turns, T, heads, 128, dtype=dtype) for i in (8, 9))
+    k, v = (t * (1 + torch.arange(turns, device="cuda")).to(dtype)[:, None, None, None] for t in (k, v))
+    freq = torch.from_numpy(INV_FREQ).cuda()
+
+    def run():
+        out = []
+        for i in range(turns):
+            ops.kv8_append(cache, k[i], v[i], table, pos0, cu_rows=cu, inv_freq=freq)
+            out.append(ops.kv8_read(cache, table, pos0, T, cu_rows=cu, dtype=dtype))
+        return out
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run()
+        graph.replay()
+    else:
+        outs = run()
+    torch.cuda.synchronize()
+    for t, s in zip(cache, start):
+        t.copy_(s)
+    for i in range(turns):
+        torch.cuda.synchronize()
+        ops.kv8_append(cache, k[i], v[i], table, pos0, cu_rows=cu, inv_freq=freq)
+        torch.cuda.synchronize()
+        for got, want in zip(outs[i], ops.kv8_read(cache, table, pos0, T, cu_rows=cu, dtype=dtype)):
+            assert torch.equal(got, want), i
+    assert ops.kernel_status() == 0

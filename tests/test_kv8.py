@@ -179,3 +179,16 @@ def test_a_cache_without_heads_or_pages_is_refused(pages, heads):
               lambda: ops.kv8_read(cache, table, pos0, 1)):
         with pytest.raises(ValueError, match="no heads or no pages"):
             f()
+
+
+def test_the_cache_is_not_read_by_read_only_loads():
+    """Its kernels start while the one before them may still write (programmatic launches): loads of memory that is read-only for a
+    kernel's whole life (ld.global.nc, __ldg) are not for it."""
+    import glob
+    import os
+    from conftest import ROOT
+    files = glob.glob(os.path.join(ROOT, "antares_b200", "csrc", "kv8*.cu*")) + [os.path.join(ROOT, "antares_b200", "csrc", "kv_pages.cu")]
+    assert len(files) >= 6
+    for name in files:
+        with open(name) as f:
+            assert not re.search(r"\bld\.global\.nc|\b__ldg\(|\bldg_nc", f.read()), name
