@@ -70,18 +70,31 @@ __device__ __forceinline__ bool kp_wait(uint32_t bar, unsigned parity, const vol
   }
   return false;
 }
-// 2^y for two y of -126 .. 126 on the fused multiply-add pipes: y = n + r with r in -1/2 .. 1/2, a polynomial for 2^r fitted for the
-// least relative error (2.7e-6, a hundredth of a step of the fp16 it becomes), n added to its exponent.
-__device__ __forceinline__ uint64_t kp_exp2(uint64_t y) {
-  const uint64_t magic = kp_pack(12582912.f, 12582912.f), minus = kp_pack(-12582912.f, -12582912.f), neg = kp_pack(-1.f, -1.f);
+__device__ __forceinline__ uint64_t kp_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float kp_max_nan(float a, float b) {  // fmaxf would drop a NaN
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^a and 2^b, both below 2^127, on the fused multiply-add pipes: y = n + r with r in -1/2 .. 1/2, a polynomial for 2^r fitted for the
+// least relative error (2.7e-6, a hundredth of a step of the fp16 it becomes), times 2^n.  n + 127 is what the low bits of the sum
+// with `magic` hold, so a shift makes it an exponent: 0, the number 0, for y = -127, which stands for all below.  So a key that is
+// masked or far below the others adds nothing, and a NaN stays one.
+__device__ __forceinline__ uint64_t kp_exp2(float a, float b) {
+  const uint64_t y = kp_pack(kp_max_nan(a, -127.f), kp_max_nan(b, -127.f));
+  const uint64_t magic = kp_pack(12583039.f, 12583039.f), minus = kp_pack(-12583039.f, -12583039.f), neg = kp_pack(-1.f, -1.f);  // 1.5 * 2^23 + 127
   auto both = [](float c) { return kp_pack(c, c); };
   const uint64_t n = kp_add2(y, magic), r = kp_fma2(kp_add2(n, minus), neg, y);
   uint64_t e = kp_fma2(both(0.00957010195f), r, both(0.0559178616f));
   e = kp_fma2(e, r, both(0.240247448f));
   e = kp_fma2(e, r, both(0.693121815f));
   e = kp_fma2(e, r, both(0.999999261f));
-  const KpPair nn = kp_unpack(n), ee = kp_unpack(e);
-  return kp_pack(__int_as_float((__float_as_int(nn.a) << 23) + __float_as_int(ee.a)), __int_as_float((__float_as_int(nn.b) << 23) + __float_as_int(ee.b)));
+  const KpPair nn = kp_unpack(n);
+  return kp_mul2(e, kp_pack(__int_as_float(__float_as_int(nn.a) << 23), __int_as_float(__float_as_int(nn.b) << 23)));
 }
 // Nothing uses the loaded registers before this.
 __device__ __forceinline__ void kp_wait_ld(uint32_t (&r)[32]) {
@@ -532,7 +545,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
               if constexpr (!ALL) v.a = k < mine ? v.a : -CUDART_INF_F, v.b = k + 1 < mine ? v.b : -CUDART_INF_F;
               float a, b2;
               if (PARTS == 1 && i % 4 == 3) {  // a quarter of them off the exponential unit
-                const KpPair e = kp_unpack(kp_exp2(kp_pack(fmaxf(v.a, -126.f), fmaxf(v.b, -126.f))));
+                const KpPair e = kp_unpack(kp_exp2(v.a, v.b));
                 a = e.a, b2 = e.b;
               } else {
                 a = ap_ex2(v.a), b2 = ap_ex2(v.b);

@@ -630,3 +630,56 @@ def test_other_rows_over_the_same_pages_call_behind_call(cuda, dtype, captured):
         for got, want in zip(outs[i], ops.kv8_read(cache, table, pos0, T, cu_rows=cu, dtype=dtype)):
             assert torch.equal(got, want), i
     assert ops.kernel_status() == 0
+
+
+# many tiles of rows (keys are one CTA's), and few (keys in shares, joined)
+WHOLE_OR_SHARED = [([0, 0, 0], [140] * 3, 32, 32), ([0], [150], 8, 2)]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("past,rows,hq,hkv", WHOLE_OR_SHARED[:1])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_every_prompt_row_with_an_infinite_query_is_nan(cuda, past, rows, hq, hkv, value, dtype):
+    """Scores that are infinite have no softmax, whichever keys they are of and whatever their signs: a code of either sign or of
+    zero, the only score that is not -inf at any place of a block."""
+    cache, table = _setup(71, past, rows, hkv, 32)
+    table = _wide(table, 32)
+    sign = 1 if value != float("-inf") else -1
+    for d, high in ((7, ()), (8, (6, 7)), (9, (15,)), (10, (3,)), (11, tuple(range(16)))):
+        codes = torch.full((32,), -5 * sign, dtype=torch.int8, device="cuda")
+        for i in high:
+            codes[i], codes[16 + i] = 5 * sign, 5 * sign
+        cache[0][..., d] = codes
+    cache[0][..., 12] = 0
+    q = _randn(4, sum(rows), hq, 128, dtype=dtype)
+    want = ops.kv8_attention(q, cache, table, _ints(past))
+    assert want.isfinite().all()
+    for d in (7, 8, 9, 10, 11, 12):
+        for every in (1, 5):
+            x = q.clone()
+            x[::every, 1, d] = value
+            got = ops.kv8_attention(x, cache, table, _ints(past))
+            bad = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+            bad[::every, 1] = True
+            assert got[bad].isnan().all(), (d, every, got[bad].isnan().all(1).logical_not().nonzero()[:5])
+            assert torch.equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq,hkv,rows", [(80, 80, 66), (4, 1, 66), (8, 2, 1)])
+def test_keys_of_no_weight_add_nothing(cuda, hq, hkv, rows, dtype):
+    """One key with large values has all the weight; 2000 others far below it hold values of scale 0, whose part of the sum counts
+    2^100 times what their part of the product does."""
+    past = 2000
+    cache, table = _setup(72, [past], [rows], hkv, 64)
+    page, rest = int(table[0, 0]), table[0, :-(-(past + rows) // 64)].long()
+    for t, fill in ((cache[0], -100), (cache[1], 0), (cache[2], 0.02), (cache[3], 0.0)):
+        t[rest] = fill
+    g = torch.Generator().manual_seed(5)
+    cache[0][page, :, :1] = 100
+    cache[1][page, :, :1] = torch.randint(-1, 2, (hkv, 1, 128), generator=g).to(torch.int8).cuda()
+    cache[3][page, :, 0] = 2.0 ** 15
+    q = torch.ones(rows, hq, 128, dtype=dtype, device="cuda")
+    q[:, :, ::3] = 0.5
+    got = ops.kv8_attention(q, cache, _wide(table, 64), _ints([past]))
+    _check_attention(got, _ref(cache, table), q, [past], None, past + rows, dtype, norm=False)
