@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(KP_JOIN_WARPS * 32) kv8_prefill_join_kernel(co
   for (int z = 0; z < p.splits; ++z) {
     const size_t at = (((size_t)slot * p.c.H + hk) * p.splits + z) * ROWS + row;
     const float2 ml = p.partial_ml[at];
-    if (ml.y == 0.f) continue;  // no keys there: nothing was written (a sum that is not a number is not 0)
+    if (ml.y == 0.f) continue;  // no key of any weight there, perhaps nothing written (a sum that is not a number is not 0)
     const float4 v = reinterpret_cast<const float4 *>(p.partial + at * KV8_D)[lane];
     const float up = fmaxf(m, ml.x), f = m == -CUDART_INF_F ? 0.f : ap_ex2(m - up), fc = ml.x == -CUDART_INF_F ? 1.f : ap_ex2(ml.x - up);
     l = l * f + ml.y * fc;
@@ -690,8 +690,9 @@ __global__ void __launch_bounds__(KP_JOIN_WARPS * 32) kv8_prefill_join_kernel(co
   const int token = packed / p.group, head = hk * p.group + packed - token * p.group;
   T *out = (T *)p.out + ((size_t)(place.row0 + token) * p.Hq + head) * KV8_D + 4 * lane;
   const float x[4] = {acc.x, acc.y, acc.z, acc.w};
+  const bool none = p.r.pos0[place.seq] + (long)(packed / p.group) < 0;  // nothing to attend to; keys whose scores are all -inf have no softmax: 0 / 0
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.f ? 0.f : x[e] / l);
+  for (int e = 0; e < 4; ++e) out[e] = (T)(none ? 0.f : x[e] / l);
 }
 
 template <typename T, int TILES, int PARTS>

@@ -637,7 +637,7 @@ WHOLE_OR_SHARED = [([0, 0, 0], [140] * 3, 32, 32), ([0], [150], 8, 2)]
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
-@pytest.mark.parametrize("past,rows,hq,hkv", WHOLE_OR_SHARED[:1])
+@pytest.mark.parametrize("past,rows,hq,hkv", WHOLE_OR_SHARED)
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 def test_every_prompt_row_with_an_infinite_query_is_nan(cuda, past, rows, hq, hkv, value, dtype):
     """Scores that are infinite have no softmax, whichever keys they are of and whatever their signs: a code of either sign or of
