@@ -34,6 +34,10 @@ struct Kv8Rows {
   __device__ __forceinline__ int end(int s) const { return cu ? min(max(cu[s + 1], 0), T) : s * n + n; }
 };
 
+// 2^e, exact: -149 <= e <= 127.  A query's largest value can lie at either end of fp32, and 2^e that brings it to a fixed size beyond
+// both: that one goes in two steps.
+__device__ __forceinline__ float kv8_pow2(int e) { return __int_as_float(e >= -126 ? (127 + e) << 23 : 1 << (149 + e)); }
+
 // First element of head h in the page that holds position p of sequence s; -1 where the table names no page of the cache.
 __device__ __forceinline__ long kv8_page(const Kv8Cache &c, const Kv8Rows &r, int s, int p, int *status) {
   const int page = r.table[(size_t)s * r.table_stride + (p >> c.shift)];

@@ -435,15 +435,15 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < KD_WARPS; ++i) most = max(most, __float_as_uint(q_max_s[i][8 * n + g]));
-      const int e = max(-100, min(100, 21 - (int)(most >> 23) + 127));
-      const float up = __int_as_float((127 + e) << 23);
-      back[n] = most >= 0x7f800000u ? CUDART_NAN_F : __int_as_float((127 - e) << 23);
+      const int e = 21 - (int)(most >> 23) + 127;  // -107 .. 148
+      const float up = kv8_pow2(e >> 1), up2 = kv8_pow2(e - (e >> 1));
+      back[n] = most >= 0x7f800000u ? CUDART_NAN_F : kv8_pow2(-e);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t part[BYTES] = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          int v = __float2int_rn(f[n][c][i] * up);
+          int v = __float2int_rn(f[n][c][i] * up * up2);
 #pragma unroll
           for (int k = BYTES - 1; k > 0; --k) {
             const int low = (int)(int8_t)v;

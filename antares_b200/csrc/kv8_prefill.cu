@@ -225,16 +225,16 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
           const float4 v = q[c];
           most = max(max(most, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
         }
-        const int e = max(-100, min(100, 13 - (int)(most >> 23) + 127));
-        const float up = __int_as_float((127 + e) << 23) * (flip ? -1.f : 1.f);
-        back = most >= 0x7f800000u ? CUDART_NAN_F : __int_as_float((127 - e) << 23);
+        const int e = 13 - (int)(most >> 23) + 127;  // -115 .. 140
+        const float up = kv8_pow2(e >> 1) * (flip ? -1.f : 1.f), up2 = kv8_pow2(e - (e >> 1));
+        back = most >= 0x7f800000u ? CUDART_NAN_F : kv8_pow2(-e);
 #pragma unroll 4
         for (int c = 0; c < KV8_D / 8; ++c) {
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 v = q[2 * c + h];
-            const float x[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
+            const float x[4] = {v.x * up * up2, v.y * up * up2, v.z * up * up2, v.w * up * up2};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);

@@ -683,3 +683,17 @@ def test_keys_of_no_weight_add_nothing(cuda, hq, hkv, rows, dtype):
     q[:, :, ::3] = 0.5
     got = ops.kv8_attention(q, cache, _wide(table, 64), _ints([past]))
     _check_attention(got, _ref(cache, table), q, [past], None, past + rows, dtype, norm=False)
+
+
+@pytest.mark.parametrize("rows,hq,hkv", [(1, 4, 4), (3, 16, 2), (150, 8, 2), (140, 80, 80)])
+@pytest.mark.parametrize("e", [124, 118, 80, -80, -95, -118])
+def test_queries_of_any_size(cuda, rows, hq, hkv, e):
+    """fp32 queries up to the type's largest and down to its smallest, over keys that bring their scores back to ordinary ones."""
+    past = 77
+    cache, table = _setup(81, [past], [rows], hkv, 32)
+    cache[2].mul_(2.0 ** min(-e, 118))
+    q = _randn(3, rows, hq, 128, dtype=F32).clamp_(-6, 6) * 2.0 ** e
+    got = ops.kv8_attention(q, cache, _wide(table, 32), _ints([past]))
+    _check_attention(got, _ref(cache, table), q, [past], None, past + rows, F32)
+    step = ops.kv8_attention(q[:1], cache, table, _ints([past]))
+    _check_attention(step, _ref(cache, table), q[:1], [past], None, past + rows, F32)
