@@ -49,7 +49,7 @@ struct DecodeParams {
   const float *inv_freq;     // rotate the queries, or nullptr
   const void *k_new, *v_new;  // this step's rows of keys and values, written first; nullptr: the cache holds them
   long k_stride, v_stride;
-  int zero_rest;             // rows behind the last sequence's become zeros
+  int zero_rest;             // rows that are no sequence's become zeros
   int few;                   // sequences with more rows than this (rows x group) are another kernel's
   int splits, tiles;         // FIXED: CTAs of an item; tiles of a sequence's rows
   int beside;                // KD_BESIDE_*: the kernel before in the stream runs beside this one, which only ends after it
@@ -228,10 +228,10 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
   // comes after this kernel waits for it alone, so it waits for the one beside it before it ends.
   if (!p.beside) pdl_wait();
 
-  if (p.zero_rest) {
-    const long row16 = (long)p.Hq * KV8_D * sizeof(T) / 16;
-    for (long i = r.end(r.S - 1) * row16 + (long)blockIdx.x * KD_THREADS + tid; i < r.T * row16; i += (long)gridDim.x * KD_THREADS)
-      reinterpret_cast<uint4 *>(p.out)[i] = make_uint4(0, 0, 0, 0);
+  if (p.zero_rest) {  // rows in front of the first sequence's, then those behind the last one's
+    const long row16 = (long)p.Hq * KV8_D * sizeof(T) / 16, front = r.begin(0) * row16, own = (r.end(r.S - 1) - r.begin(0)) * row16;
+    for (long i = (long)blockIdx.x * KD_THREADS + tid; i < r.T * row16 - own; i += (long)gridDim.x * KD_THREADS)
+      reinterpret_cast<uint4 *>(p.out)[i < front ? i : i + own] = make_uint4(0, 0, 0, 0);
   }
 
   // ---- this CTA's share: w0 .. w1 - 1 of all work, ordered by sequence, kv head, tile, block

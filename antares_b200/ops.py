@@ -414,7 +414,7 @@ def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=Non
 
 def kv8_read(cache, page_table, pos0, rows, cu_rows=None, dtype=torch.float16, out=None):
     """The values held at the rows' positions, (k, v) [rows, kv heads, 128] each; zeros outside the table.  out: a pair of
-    tensors to write to, whose rows behind the last sequence's stay as they are (new tensors: zeros)."""
+    tensors to write to, whose rows that are no sequence's stay as they are (new tensors: zeros)."""
     if out is None:
         y = fast().kv8_read(cache, page_table, pos0, rows, cu_rows, _DT.get(dtype, -1))
         if y is not None:
@@ -454,7 +454,7 @@ def _kv8_workspace(workspace, S, T, max_rows, Hq, Hkv, device):
 def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale=None, out=None, workspace=None):
     """Row r of sequence s, q [T, query heads, 128], over the positions 0 .. pos0[s] + r of the cache, which holds them already
     (kv8_append); kv head = query head // (query heads / kv heads).  Rows with no position to attend to are zeros, and so are
-    rows behind the last sequence's in a new result (in `out` they stay as they are).  max_rows: the most rows of a sequence,
+    rows that are no sequence's in a new result (in `out` they stay as they are).  max_rows: the most rows of a sequence,
     a hint.  out may be q where q is contiguous."""
     if out is None and workspace is None:
         y = fast().kv8_attention(q, cache, page_table, pos0, cu_rows, max_rows, scale)

@@ -435,8 +435,9 @@ int ab200_greedy_next_tp_emulated(const float *const *logits_host, const int *n_
  * table_stride of 0: one row for all sequences.  Entries of positions that a call does not touch are not read.  An entry
  * outside 0 .. pages - 1 that it does touch writes nothing, reads as zeros or as page 0, and shows in ab200_kernel_status.
  * The call's rows: T rows of S sequences, sequence s has rows cu_rows_dev[s] .. cu_rows_dev[s + 1] - 1 (int32 [S + 1];
- * NULL: T / S each) at the positions pos0_dev[s], pos0_dev[s] + 1, ... (int32 [S]).  Rows behind the last sequence's are
- * left as they were (zero_rest: become zeros).  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the
+ * NULL: T / S each) at the positions pos0_dev[s], pos0_dev[s] + 1, ... (int32 [S]).  Offsets do not fall.
+ * Rows that are no sequence's (in front of the first one's, behind the last one's) are left as they were (zero_rest: become
+ * zeros).  S = 0 and T = 0 are calls that do nothing.  `dtype` is that of q, k, v and the
  * results; rows may be strided (in elements, a multiple of 16 bytes), the heads of a row lie together.  Sequences may share pages
  * that a call reads; the blocks of 16 rows that it writes belong to one sequence of the call. */
 

@@ -697,3 +697,25 @@ def test_queries_of_any_size(cuda, rows, hq, hkv, e):
     _check_attention(got, _ref(cache, table), q, [past], None, past + rows, F32)
     step = ops.kv8_attention(q[:1], cache, table, _ints([past]))
     _check_attention(step, _ref(cache, table), q[:1], [past], None, past + rows, F32)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rows", [1, 30, 200])
+def test_rows_in_front_of_the_first_sequence(cuda, rows, dtype):
+    """A batch whose offsets do not begin at 0: the rows before are nobody's either."""
+    cache, table = _setup(12, [40, 3], [rows, 2], 2, 32)
+    table, freq = _wide(table, 32), torch.from_numpy(INV_FREQ).cuda()
+    front, T = 5, rows + 2 + 5 + 4
+    own = slice(front, front + rows + 2)
+    q, k = _randn(1, T, 24, 128, dtype=dtype), _randn(2, T, 2, 128, dtype=dtype)
+    cu, pos0 = _ints([front, front + rows, front + rows + 2]), _ints([40, 3])
+    want = ops.kv8_attention(q[own], cache, table, pos0, cu_rows=_ints([0, rows, rows + 2]))
+    out = torch.full_like(q, 5.0)
+    ops.kv8_attention(q, cache, table, pos0, cu_rows=cu, out=out)
+    torch.full_like(q, 7.0)  # memory that a new result may be given
+    new = ops.kv8_attention(q, cache, table, pos0, cu_rows=cu)
+    turned = ops.kv8_append(cache, k, k, table, pos0, cu_rows=cu, q=q, inv_freq=freq)
+    back = ops.kv8_read(cache, table, pos0, T, cu_rows=cu, dtype=dtype)
+    for t in (new, turned) + back:
+        assert not t[:front].any() and not t[own.stop:].any() and t[own].any()
+    assert torch.equal(new[own], want) and torch.equal(out[own], want) and (out[:front] == 5).all() and (out[own.stop:] == 5).all()
