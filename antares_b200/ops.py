@@ -402,7 +402,7 @@ def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=Non
         qp, q_stride = _rows3(q, "q", k.dtype, T)
         hq = q.shape[1]
         if q_out is None:
-            zero, q_out = 1, torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            zero, q_out = 1, (torch.empty if args[12] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
         qo, qo_stride = _rows3(q_out, "q_out", k.dtype, T, hq)
     for t in (v, q, q_out, inv_freq):
         if t is not None and t.device != k.device:

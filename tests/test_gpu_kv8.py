@@ -719,3 +719,20 @@ def test_rows_in_front_of_the_first_sequence(cuda, rows, dtype):
     for t in (new, turned) + back:
         assert not t[:front].any() and not t[own.stop:].any() and t[own].any()
     assert torch.equal(new[own], want) and torch.equal(out[own], want) and (out[:front] == 5).all() and (out[own.stop:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_rows_of_no_sequences_at_all(cuda, dtype):
+    """S = 0 with rows: new results are zeros, a given one stays as it was."""
+    cache, _ = _setup(1, [10], [1], 2, 32)
+    table, pos0 = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    q, k, cu = _randn(1, 6, 4, 128, dtype=dtype), _randn(2, 6, 2, 128, dtype=dtype), torch.zeros(1, dtype=torch.int32, device="cuda")
+    freq = torch.from_numpy(INV_FREQ).cuda()
+    for _ in range(3):
+        torch.full_like(q, 7.0), torch.full_like(k, 7.0)  # memory that a new result is given
+        turned = ops.kv8_append(cache, k, k, table, pos0, cu_rows=cu, q=q, inv_freq=freq)
+        assert not turned.any() and not ops.kv8_attention(q, cache, table, pos0, cu_rows=cu).any()
+        assert not any(t.any() for t in ops.kv8_read(cache, table, pos0, 6, cu_rows=cu, dtype=dtype))
+    out = torch.full_like(q, 5.0)
+    ops.kv8_append(cache, k, k, table, pos0, cu_rows=cu, q=q, inv_freq=freq, q_out=out)
+    assert (out == 5).all()
