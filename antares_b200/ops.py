@@ -374,12 +374,27 @@ def _disjoint(out, name, *others):
     a, b = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
     for t in others:
         if t is not None and t.numel() and t.data_ptr() < b and a < t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size():
-            raise ValueError("%s may not lie over an input" % name)
+            raise ValueError("%s may not lie over an input or another result" % name)
+
+
+def _rows_meet(a, b):
+    """Whether two tensors of as many rows, as _rows3 takes them, have a byte in common: rows may lie between one another's, as
+    slices of one projection's result do."""
+    T, e = a.shape[0], a.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, wa, sa), (b0, wb, sb) = ((t.data_ptr(), t.shape[1] * 128 * t.element_size(), t.stride(0) * t.element_size()) for t in (a, b))
+    if T == 1 or a0 + (T - 1) * sa + wa <= b0 or b0 + (T - 1) * sb + wb <= a0:
+        return a0 < b0 + (T - 1) * sb + wb and b0 < a0 + (T - 1) * sa + wa
+    import numpy as np
+    at = np.arange(T, dtype=np.int64) * sa + (a0 - b0)     # a's rows, counted from b's first
+    j = np.clip(at // max(sb, e), 0, T - 1)                # the last of b's rows that begins at or before each, and the next
+    return any(bool(((at < n * sb + wb) & (n * sb < at + wa)).any()) for n in (j, np.minimum(j + 1, T - 1)))
 
 
 def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=None, q_out=None):
     """Writes rows k, v [T, kv heads, 128] into the cache; with inv_freq, k rotated by halves at its positions, and q [T, query
-    heads, 128] too: returns the rotated queries (q_out, which may be q), else None."""
+    heads, 128] too: returns the rotated queries (q_out, which may be q but not lie over k, v or other rows of q), else None."""
     if q_out is None:
         y = fast().kv8_append(cache, k, v, page_table, pos0, cu_rows, q, inv_freq)
         if y is not None:
@@ -404,6 +419,9 @@ def kv8_append(cache, k, v, page_table, pos0, cu_rows=None, q=None, inv_freq=Non
         if q_out is None:
             zero, q_out = 1, (torch.empty if args[12] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
         qo, qo_stride = _rows3(q_out, "q_out", k.dtype, T, hq)
+        for t, name in ((k, "k"), (v, "v"), (q, "q")):
+            if _rows_meet(q_out, t) and not (name == "q" and qo == qp and (qo_stride == q_stride or T == 1)):
+                raise ValueError("q_out may not lie over %s%s" % (name, " unless it is q" if name == "q" else ""))
     for t in (v, q, q_out, inv_freq):
         if t is not None and t.device != k.device:
             raise ValueError("the tensors of a kv8 call lie on one device")
@@ -429,6 +447,8 @@ def kv8_read(cache, page_table, pos0, rows, cu_rows=None, dtype=torch.float16, o
         _rows3(t, "out", dtype, rows, args[6])
         if not t.is_contiguous() or t.device != cache[0].device:
             raise ValueError("out must be contiguous and on the cache's device")
+        _disjoint(t, "out", *cache)
+    _disjoint(out[0], "out", out[1])
     with torch.cuda.device(cache[0].device):
         call("ab200_kv8_read", *args, out[0].data_ptr(), out[1].data_ptr(), int(zero), _code(dtype), _stream())
     return out[0], out[1]
@@ -477,6 +497,7 @@ def kv8_attention(q, cache, page_table, pos0, cu_rows=None, max_rows=None, scale
         _chk(out, "out", q.dtype)
         if not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
             _disjoint(out, "out", q)
+        _disjoint(out, "out", *cache)
     scale = 128 ** -0.5 if scale is None else scale
     with torch.cuda.device(q.device):
         ws, ws_bytes, held = _kv8_workspace(workspace, S, T, max_rows, hq, args[6], q.device)
@@ -512,7 +533,7 @@ def kv8_step(q, k, v, cache, page_table, pos0, inv_freq=None, scale=None, out=No
         if out.shape != q.shape:
             raise ValueError("out must be %s" % (tuple(q.shape),))
         _chk(out, "out", q.dtype)
-        _disjoint(out, "out", q, k, v)
+        _disjoint(out, "out", q, k, v, *cache)
     S = args[12]
     scale = 128 ** -0.5 if scale is None else scale
     with torch.cuda.device(q.device):

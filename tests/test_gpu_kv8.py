@@ -736,3 +736,21 @@ def test_rows_of_no_sequences_at_all(cuda, dtype):
     out = torch.full_like(q, 5.0)
     ops.kv8_append(cache, k, k, table, pos0, cu_rows=cu, q=q, inv_freq=freq, q_out=out)
     assert (out == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_rotated_queries_may_be_the_queries(cuda, dtype):
+    """q_out over q itself, slices of one projection's result: the same rows, k and v untouched."""
+    cache, table = _setup(91, [7], [40], 2, 32, filled=False)
+    both, freq = _randn(1, 40, 10, 128, dtype=dtype), torch.from_numpy(INV_FREQ).cuda()
+    q, k, v = both[:, :6], both[:, 6:8], both[:, 8:]
+    before = both.clone()
+    want = ops.kv8_append([t.clone() for t in cache], k, v, table, _ints([7]), q=q, inv_freq=freq)
+    assert ops.kv8_append(cache, k, v, table, _ints([7]), q=q, inv_freq=freq, q_out=q) is q
+    assert torch.equal(q, want) and torch.equal(both[:, 6:], before[:, 6:])
+    for bad in (both[:, 4:], both[:, 1:7]):
+        with pytest.raises(ValueError, match="may not lie over"):
+            ops.kv8_append(cache, k, v, table, _ints([7]), q=q, inv_freq=freq, q_out=bad)
+    out = torch.zeros(4, 2, 128, dtype=dtype, device="cuda")
+    with pytest.raises(ValueError, match="may not lie over"):
+        ops.kv8_read(cache, table, _ints([0]), 4, out=(out, out))

@@ -192,3 +192,45 @@ def test_the_cache_is_not_read_by_read_only_loads():
     for name in files:
         with open(name) as f:
             assert not re.search(r"\bld\.global\.nc|\b__ldg\(|\bldg_nc", f.read()), name
+
+
+def test_whether_rows_meet():
+    """Against every byte of both, for layouts of any stride."""
+    import random
+    rng, pool = random.Random(2), torch.zeros(40000, dtype=torch.float16)
+    met = 0
+    for _ in range(3000):
+        T = rng.randrange(1, 6)
+        sets = []
+        for _ in range(2):
+            heads = rng.randrange(1, 4)
+            stride = heads * 128 + 64 * rng.choice([0, 0, 1, 2, 6, 8])
+            sets.append(pool.as_strided((T, heads, 128), (stride, 128, 1), 64 * rng.randrange(0, 40)))
+        mine, other = ({t.storage_offset() + i * t.stride(0) + j for i in range(T) for j in range(t.shape[1] * 128)} for t in sets)
+        assert ops._rows_meet(*sets) == bool(mine & other), [(t.shape, t.stride(), t.storage_offset()) for t in sets]
+        met += bool(mine & other)
+    assert 500 < met < 2500
+    assert not ops._rows_meet(pool[:0].view(0, 1, 128), pool[:128].view(1, 1, 128))
+
+
+def test_results_over_inputs_are_refused():
+    cache, table, pos0 = _host_cache(), _gpu(torch.zeros(1, 2, dtype=torch.int32)), _gpu(torch.zeros(1, dtype=torch.int32))
+    freq, both = _gpu(torch.ones(64)), _gpu(torch.zeros(4, 8, 128).half())
+    q, k, v = both[:, :4], both[:, 4:6], both[:, 6:]
+    append = lambda q_out, q=q, k=k, v=v: ops.kv8_append(cache, k, v, table, pos0, q=q, inv_freq=freq, q_out=q_out)  # noqa: E731
+    flat = _gpu(torch.zeros(6, 4, 128).half())
+    for f in (lambda: append(both[:, 3:7]), lambda: append(both[:, 4:]), lambda: append(both[:, 2:6]), lambda: append(both[:, 1:5]), lambda: append(flat[1:5], q=flat[:4]),
+              lambda: append(q.as_strided((4, 4, 128), (512, 128, 1)))):
+        with pytest.raises(ValueError, match="may not lie over"):
+            f()
+    out = _gpu(torch.zeros(4, 2, 128).half())
+    over_codes = cache[0].view(-1).view(torch.float16)[:2 * 2 * 128].view(2, 2, 128)
+    # the kernels never see these: what refuses them is the host (a call that is taken ends at the missing GPU instead)
+    for f in (lambda: ops.kv8_read(cache, table, pos0, 4, out=(out, out)), lambda: ops.kv8_read(cache, table, pos0, 3, out=(out[:3], out[1:])),
+              lambda: ops.kv8_read(cache, table, pos0, 2, out=(out[:2], over_codes)), lambda: ops.kv8_attention(_gpu(torch.zeros(2, 2, 128).half()), cache, table, pos0, out=over_codes)):
+        with pytest.raises(ValueError, match="may not lie over"):
+            f()
+    for good in (q, _gpu(torch.zeros(4, 4, 128).half()), None):
+        with pytest.raises(Exception) as e:
+            append(good)
+        assert "may not lie over" not in str(e.value)
