@@ -187,9 +187,13 @@ class PagedKV8Cache:
         """(page_table int32 [len(seqs), max_pages], pos0 int32 [len(seqs)]) on the device: where the sequences' next rows go."""
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence is in a batch once, got %r" % (list(seqs),))
-        table = torch.full((len(seqs), self.pool.max_pages), -1, dtype=torch.int32)
+        n, width, device = len(seqs), self.pool.max_pages, self.k.device
+        # one upload, from pinned memory that torch keeps until the copy has run: nothing waits for the GPU
+        host = torch.full((n * (width + 1),), -1, dtype=torch.int32, pin_memory=device.type == "cuda")
+        table = host[:n * width].view(n, width)
         for i, s in enumerate(seqs):
             pages = self.pool.held[s]
             table[i, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
-        pos0 = torch.tensor([self.pool.rows[s] for s in seqs], dtype=torch.int32)
-        return table.to(self.k.device), pos0.to(self.k.device)
+        host[n * width:] = torch.tensor([self.pool.rows[s] for s in seqs], dtype=torch.int32)
+        both = host.to(device, non_blocking=True)
+        return both[:n * width].view(n, width), both[n * width:]

@@ -754,3 +754,48 @@ def test_rotated_queries_may_be_the_queries(cuda, dtype):
     out = torch.zeros(4, 2, 128, dtype=dtype, device="cuda")
     with pytest.raises(ValueError, match="may not lie over"):
         ops.kv8_read(cache, table, _ints([0]), 4, out=(out, out))
+
+
+def test_a_serving_step_does_not_wait_for_the_gpu(cuda):
+    """reserve, batch, append, attention, step, fork, compact and advance queue their work and return; what batch() uploads is what
+    it was called for, however late the copy runs."""
+    from antares_b200.kv_cache import PagedKV8Cache
+    c = PagedKV8Cache(1, 40, 2, page_rows=16, max_seqs=8, max_seq=256)
+    k, q = _randn(1, 40, 2, 128), _randn(2, 40, 4, 128)
+    cu = _ints([0, 20, 40])
+    for f in (ops.kv8_append, lambda *a, **kw: ops.kv8_attention(q, c.layer(0), *a[3:], **kw)):   # first calls load kernels
+        f(c.layer(0), k, k, *(t.cuda() for t in (torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))), cu_rows=cu)
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    busy, idle = torch.cuda.Event(), []
+    try:
+        torch.cuda._sleep(800_000_000)   # some 400 ms
+        busy.record()
+        a, b = c.add(), c.add()
+        c.reserve({a: 20, b: 20})
+        table, pos0 = c.batch([a, b])
+        ops.kv8_append(c.layer(0), k, k, table, pos0, cu_rows=cu)
+        ops.kv8_attention(q, c.layer(0), table, pos0, cu_rows=cu)
+        c.advance(a, 20), c.advance(b, 20)
+        seen = []
+        d = c.fork(a)
+        for _ in range(12):
+            seqs = [b, a, d]
+            c.reserve({s: 1 for s in seqs})
+            table, pos0 = c.batch(seqs)
+            seen.append((table, pos0, [list(c.pool.held[s]) for s in seqs], [c.rows(s) for s in seqs]))
+            ops.kv8_step(q[:3], k[:3], k[:3], c.layer(0), table, pos0)
+            for s in seqs:
+                c.advance(s, 1)
+        c.free(b)
+        c.compact()
+        idle.append(busy.query())
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert idle == [False]
+    torch.cuda.synchronize()
+    for table, pos0, held, rows in seen:
+        assert table.shape == (3, 16) and table.is_cuda and pos0.tolist() == rows
+        for row, pages in zip(table.tolist(), held):
+            assert row == pages + [-1] * (16 - len(pages))
+    assert ops.kernel_status() == 0
