@@ -29,7 +29,7 @@ constexpr int KP_HALF_BYTES = KP_BN * 128;          // 64 dims of 128 rows, fp16
 constexpr int KP_STAGE_BYTES = 2 * KP_HALF_BYTES;   // a tile of K or of V
 constexpr int KP_RAW_BYTES = KP_BN * KV8_D;         // its codes
 constexpr int KP_BLOCKS = KP_BN / KV8_BLOCK;
-constexpr float KP_RAISE = 8.f, KP_P_EXP = 6.f, KP_LEAST_SCALE = 0x1p-100f;
+constexpr float KP_RAISE = 8.f, KP_P_EXP = 7.f, KP_LEAST_SCALE = 0x1p-100f;  // P: its largest 2^6 at least, since m is a whole number, and 2^15 at most
 
 template <int TILES, int PARTS>
 struct KpShape {
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
       const bool all = __all_sync(0xffffffffu, left >= KP_BN || packed > last);
       const uint32_t t_first = ts + (PARTS == 1 ? 64 * (j & 1) : 0), t_other = ts + (PARTS == 1 ? 64 * (j & 1 ^ 1) : 64);
       auto p_at = [&](int c) { return PARTS == 1 ? t_first + 16 * c : ts + 32 * c; };  // P of 32 keys
-      // 64 keys of the row: their largest exponent, then P = 2^(x - m + 6)
+      // 64 keys of the row: their largest exponent, then P = 2^(x - m + 7)
       auto half = [&](int hb, auto all_keys) {
         constexpr bool ALL = decltype(all_keys)::value;
         uint32_t s0[32] = {}, s1[32] = {};
@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
         }
         const bool raise = mx > m + KP_RAISE;
         if (__any_sync(0xffffffffu, raise)) {
-          const float up = raise ? mx : m, by = up == m ? 1.f : m == -CUDART_INF_F ? 0.f : ap_ex2(m - up);
+          // to a whole number: O, l and what is held of P are scaled by a power of two, which rounds nothing
+          const float up = raise ? ceilf(mx) : m, d = m - up, by = up == m ? 1.f : d < -126.f ? 0.f : kv8_pow2((int)d);
           m = up;
           l *= by;
           ap_wait_st();

@@ -799,3 +799,23 @@ def test_a_serving_step_does_not_wait_for_the_gpu(cuda):
         for row, pages in zip(table.tolist(), held):
             assert row == pages + [-1] * (16 - len(pages))
     assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("rows,hq,hkv", [(300, 80, 80), (300, 8, 1)])
+def test_a_maximum_that_rises_inside_a_tile_rounds_nothing_twice(cuda, rows, hq, hkv):
+    """fp16 prompts: one key with values 6.4 to 8 octaves above the first 128, behind it another that makes the maximum rise: what is
+    held of the first is scaled, not rounded a second time."""
+    past = 260
+    cache, table = _setup(95, [past], [rows], hkv, 32)
+    for t, fill in zip(cache, (0, 0, 0.02, 0.25)):
+        t.fill_(fill)
+    g = torch.Generator().manual_seed(3)
+    place = lambda p: (int(table[0, p // 32]), slice(None), p % 32)  # noqa: E731
+    cache[0][place(130)], cache[0][place(250)] = 0, 0
+    cache[0][place(130) + (5,)], cache[0][place(250) + (5,)] = 100, 127
+    cache[1][place(130)] = torch.randint(-127, 128, (hkv, 128), generator=g).to(torch.int8).cuda()
+    # 128 ** -0.5 * log2(e) * 0.02 * 100 octaves for a query of 1
+    q = torch.zeros(rows, hq, 128, dtype=F16, device="cuda")
+    q[..., 5] = ((6.4 + 1.55 * torch.rand(rows, hq, generator=g)) / (128 ** -0.5 * 1.4426950408889634 * 2)).half().cuda()
+    got = ops.kv8_attention(q, cache, _wide(table, 32), _ints([past]))
+    _check_attention(got, _ref(cache, table), q, [past], None, past + rows, F16, norm=False)
