@@ -819,3 +819,75 @@ def test_a_maximum_that_rises_inside_a_tile_rounds_nothing_twice(cuda, rows, hq,
     q[..., 5] = ((6.4 + 1.55 * torch.rand(rows, hq, generator=g)) / (128 ** -0.5 * 1.4426950408889634 * 2)).half().cuda()
     got = ops.kv8_attention(q, cache, _wide(table, 32), _ints([past]))
     _check_attention(got, _ref(cache, table), q, [past], None, past + rows, F16, norm=False)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("past,hq,hkv,rope", [([367], 32, 32, True), ([367], 32, 32, False), ([0], 8, 1, True), ([30, 600, 0, 15, 250], 16, 4, True), ([30, 600, 0, 15, 250], 16, 4, False)])
+def test_steps_in_a_row_of_few_requests(cuda, past, hq, hkv, rope, captured, dtype):
+    """A decoder's form of the step: tables no wider than its requests need, an item to a cluster of CTAs, which in fp16 write the new
+    rows themselves.  Steps of growing values behind one another, over the ends of blocks and pages, have the bits of the same steps
+    one at a time, and of append and attention apart."""
+    steps, S = 40, len(past)
+    cache, table = _setup(34, past, [steps] * S, hkv, 32, filled=False)
+    filled = sum(past)
+    if filled:  # rows that are there before, as a prompt's append leaves them
+        x = _randn(9, filled, hkv, 128, dtype=dtype)
+        ops.kv8_append(cache, x, x, table, _ints([0] * S), cu_rows=_cu(past))
+    ahead, apart = ([t.clone() for t in cache] for _ in range(2))
+    q, k, v = (_randn(i, steps, S, h, 128, dtype=dtype) for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    k, v = (t * (1 + 0.2 * torch.arange(steps, device="cuda")).to(dtype)[:, None, None, None] for t in (k, v))
+    freq = torch.from_numpy(INV_FREQ).cuda() if rope else None
+    pos0 = [_ints([n + i for n in past]) for i in range(steps)]
+    run = lambda: [ops.kv8_step(q[i], k[i], v[i], cache, table, pos0[i], inv_freq=freq) for i in range(steps)]  # noqa: E731
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run()
+        graph.replay()
+    else:
+        outs = run()
+    torch.cuda.synchronize()
+    for i in range(steps):
+        one = ops.kv8_step(q[i], k[i], v[i], ahead, table, pos0[i], inv_freq=freq)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], one), i
+        ops.kv8_append(apart, k[i], v[i], table, pos0[i], inv_freq=freq)
+        torch.cuda.synchronize()
+        if not rope:
+            assert torch.equal(one, ops.kv8_attention(q[i], apart, table, pos0[i])), i
+    for a, b, c in zip(cache, ahead, apart):
+        assert torch.equal(a.view(torch.int8), b.view(torch.int8)) and torch.equal(a.view(torch.int8), c.view(torch.int8))
+    want, spread, score, tiny = kv8_ref.attention(_ref(cache, table), q[-1].double().cpu().numpy(), [n + steps - 1 for n in past], None, None, INV_FREQ if rope else None)
+    if rope:  # a rotated query may be kept in its type: half a step of it moves every score
+        score = score + 1.5 * kv8_ref.attention(_ref(cache, table), q[-1].double().cpu().numpy(), [n + steps - 1 for n in past], None)[2] * 2.0 ** 19 * (torch.finfo(dtype).eps / 2 + 2.0 ** -21)
+    off = np.abs(outs[-1].double().cpu().numpy() - want) / kv8_ref.bound(want, spread, score, tiny, max(past) + steps, dtype)
+    assert off.max() <= 1, off.max()
+    assert ops.kernel_status() == 0
+
+
+def _prompt_kernel_serves(q, cache, table, cu, most):
+    """The library's rule: rows of a sequence (times group) beyond 64 in a call of more than 2.5 million rows of heads x positions."""
+    group = q.shape[1] // cache[0].shape[1]
+    return most * group > 64 and q.shape[0] * q.shape[1] * table.shape[1] * cache[0].shape[2] > 2500000
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("past,rows,hq,hkv,page", [c for c in CASES if max(c[1]) > 1])
+def test_fp16_rows_of_the_few_row_kernel_hold_p_in_22_bits(cuda, past, rows, hq, hkv, page, wide):
+    """The bound of a P held as a pair of fp16 numbers, 2^-20, for every row that the few-row kernel serves: all rows of calls that it
+    serves alone, and short sequences beside prompts."""
+    cache, table = _setup(len(past) + sum(rows), past, rows, hkv, page)
+    ref = _ref(cache, table)
+    table = _wide(table, page) if wide else table
+    q, cu = _randn(1, sum(rows), hq, 128, mul=2), np.cumsum([0] + rows)
+    got = ops.kv8_attention(q, cache, table, _ints(past), cu_rows=_cu(rows), max_rows=max(rows)).double().cpu().numpy()
+    want, spread, score, tiny = kv8_ref.attention(ref, q.double().cpu().numpy(), past, cu)
+    single = np.zeros(got.shape, bool)
+    if _prompt_kernel_serves(q, cache, table, cu, max(rows)):
+        for s, n in enumerate(rows):
+            single[cu[s]:cu[s + 1]] = n * (hq // hkv) > 64
+    keys = max(p + n for p, n in zip(past, rows))
+    tight, loose = (kv8_ref.bound(want, spread, score, tiny, keys, F16, one) for one in (False, True))
+    off = np.abs(got - want) / np.where(single, loose, tight)
+    assert off.max() <= 1, (off.max(), np.unravel_index(off.argmax(), off.shape))
