@@ -29,7 +29,7 @@ constexpr int KP_HALF_BYTES = KP_BN * 128;          // 64 dims of 128 rows, fp16
 constexpr int KP_STAGE_BYTES = 2 * KP_HALF_BYTES;   // a tile of K or of V
 constexpr int KP_RAW_BYTES = KP_BN * KV8_D;         // its codes
 constexpr int KP_BLOCKS = KP_BN / KV8_BLOCK;
-constexpr float KP_RAISE = 8.f, KP_P_EXP = 7.f, KP_LEAST_SCALE = 0x1p-100f;  // P: its largest 2^6 at least, since m is a whole number, and 2^15 at most
+constexpr float KP_RAISE = 8.f, KP_P_EXP = 7.f, KP_LEAST_SCALE = 0x1p-100f;  // P: a row's largest 2^6 at least, since m is raised by whole numbers, and 2^15 at most
 
 template <int TILES, int PARTS>
 struct KpShape {
@@ -487,8 +487,9 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
         }
         const bool raise = mx > m + KP_RAISE;
         if (__any_sync(0xffffffffu, raise)) {
-          // to a whole number: O, l and what is held of P are scaled by a power of two, which rounds nothing
-          const float up = raise ? ceilf(mx) : m, d = m - up, by = up == m ? 1.f : d < -126.f ? 0.f : kv8_pow2((int)d);
+          // by a whole number: O, l and what is held of P are scaled by a power of two, which rounds nothing.  From nothing to the
+          // maximum itself: the largest P of a row's first keys, often its largest of all, is a power of two then.
+          const float d = raise ? ceilf(mx - m) : 0.f, up = m == -CUDART_INF_F ? mx : m + d, by = d > 126.f ? 0.f : kv8_pow2(-(int)d);
           m = up;
           l *= by;
           ap_wait_st();
