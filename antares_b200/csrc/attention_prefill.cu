@@ -9,8 +9,8 @@
 // P is stored as an fp16 pair hi + lo, 22 bits of an fp32 probability's 24, and both halves are multiplied with V into
 // the same fp32 accumulator, so only q, K, V and the result are 16 bits wide.  P is scaled by 2^6 (the row sum with it),
 // which keeps lo out of the subnormals where it matters.  The running maximum is only raised when a tile exceeds it by
-// more than 2^8 (then O is rescaled in tensor memory): what the row is finally divided by
-// contains the same factor.  Error of the fp16 result against 64 bits, 2000 rows: 1.95138e-4, the fp32 single-query
+// more than 2^8 (a published way to spare rescaling, not an idea of this file; then O is rescaled in tensor memory): what the row is
+// finally divided by contains the same factor.  Error of the fp16 result against 64 bits, 2000 rows: 1.95138e-4, the fp32 single-query
 // kernel 1.95134e-4, the exact result rounded to fp16 1.95134e-4; the difference, 1e-6 of the result, is the tensor
 // cores' accumulation (it grows with the number of MMAs a row has gone through).  The pair's own share is 5e-8 of the
 // result, an fp32 probability's 2.4e-8, fp16 alone would be 2e-4.

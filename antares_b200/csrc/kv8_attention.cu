@@ -17,7 +17,8 @@
 // us (TB/s): 64 sequences, all of 16000 positions, 8 kv heads of 4 query heads 323 (6.5, 99 % of a copy's rate); one of 131072 and
 // 32 kv heads 170 (6.3); one of 131072 and 8 kv heads 54 (5.0); 64 ragged ones of up to 8000, 8 heads of 8 107 (5.2).  Where a share is
 // small, starting an item (7800 cycles) and the second launch weigh: 48 ragged ones of up to 4000 45 us (4.4), of one request of
-// 384 positions 7.0 us only a tenth is the stream.  16 rows a tile: products and exponentials bound it, twice a block's instructions.
+// 384 positions 6.7 us only a tenth is the stream.  16 rows a tile: products and exponentials bound it, twice a block's instructions.
+// Registers and bytes spilled, equal shares: 8 rows 168 and 64 (fp32 76), three CTAs an SM; 16 rows 255 and 24 (fp32 36), two.
 #include <math_constants.h>
 
 #include <cooperative_groups.h>
@@ -811,6 +812,10 @@ static int decode_launch(DecodeParams p, const DecodePlan &d, cudaStream_t strea
   return AB200_OK;
 }
 
+// Which kernels serve a call goes by the width of its page table, the most positions that its sequences can have: their lengths are
+// on the device.  A table much wider than its sequences are long costs the cluster form: one request of 384 positions and 32 heads, step /
+// attention 8.5 / 6.7 us with 64 pages of 64 rows in its row, 11.0 / 9.6 with 512 or 2000.
+//
 // Sequences of up to KD_FEW packed rows go through the kernel above, longer ones through the prompt kernel where rows of heads
 // times the positions that the pages hold are more than KD_PROMPT_WORK.  us, above / prompt kernel, rows of heads x positions:
 //   500 x 2600 (one kv head) 13.5 / 24.6     2240 x 570 14.1 / 18.3     4096 x 128 7.2 / 11.5     2048 x 64 12.2 / 10.3
@@ -935,7 +940,8 @@ extern "C" int ab200_kv8_step(const void *q, const void *k, const void *v, long 
   if (rc) return rc;
   AB200_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= a.bytes, "kv8_step: needs a 16-byte aligned workspace of %zu bytes, got %zu", a.bytes, workspace_bytes);
   // fp16 rows that fit into one tile are written by the attention kernel itself where an item is a cluster's (us, together /
-  // apart: one request of 384 positions and 32 heads 9.7 / 9.7 step behind step, 13.5 / 15.2 with a read of the rows behind each; 48
+  // apart: one request of 384 positions and 32 heads 9.7 / 9.7 step behind step, 13.5 / 15.2 with a read of the rows behind each; in a
+  // decoder of 8 layers, 360 positions, 434.7 / 434.0 a token: it saves a launch where something waits for the step, else nothing; 48
   // ragged ones in equal shares 69 / 55: each new block's 4 us then is one CTA's, and the others wait for it at the end).  Else by
   // a launch that the attention kernel starts beside, and only waits for where it reads those rows: 51.3 for the 48, against 54.5 one
   // after the other.

@@ -1,16 +1,20 @@
 // Attention of many query rows over the 8-bit paged KV cache on the 5th-generation tensor cores (layout: kv8.cuh; the
 // mathematics: kv8_attention.cu): x = (q . k_code) scale log2(e) ks + log2(vs), P = 2^(x - m), O += P v_code, l += sum P / vs.
-// Codes are fp16 numbers without rounding.  fp16 rows: q as it is, P rounded to one fp16 (a weight is off by up to
-// 2^-11 of itself, as the result is by its own rounding); fp32 rows: q and P as pairs of fp16, four products.
+// Codes are fp16 numbers without rounding.  fp32 rows: q and P as pairs of fp16, four products.  fp16 rows: q as it is, P rounded to
+// one fp16, once: a weight is off by up to 2^-11 of itself, as the result is by its own rounding.  The kernel over the fp16 cache
+// (attention_prefill.cu) holds a pair; here that would be a third product and half as many instructions again for the softmax warps,
+// which bound it, over a cache whose codes are 2^-8 apart.  Error of 2000 rows 2.65e-4 of the result, 2.1e-4 if P were exact.
 //
 // A CTA has 256 packed rows of a kv head (fp32: 128) and walks over 128 keys at a time: four warps bring codes to a ring of
 // raw bytes and widen them into swizzled operands, K and V in turn; a warp for each 128 rows issues its products; four warps
 // for each 128 rows have a row a thread.  Scores and O lie in tensor memory, P goes back over the scores: the second operand
-// of P V is V alone.  Two tiles of rows share the widened keys, and one's exponentials go on under the other's products.
+// of P V is V alone.  Two tiles of rows share the widened keys, and one's exponentials go on under the other's products.  (Two tiles of
+// rows in turn, a maximum that is only raised past a threshold and part of the exponentials off their unit are published ideas; the
+// kernel, its polynomial and its figures are this project's.)
 // Where few tiles of rows would leave SMs idle their keys are cut into up to 8 shares, joined by a second launch.
 //
 // Bound by the softmax warps: 12 instructions an element, widening included; a fourth of the exponentials are polynomials, since
-// the unit makes 16 a cycle.  2000 rows of 32 heads 58.5 us (561 TFLOP/s, a third of a library product's rate; 12000 cycles of a
+// the unit makes 16 a cycle.  128 registers, 8 bytes of them spilled.  2000 rows of 32 heads 58.7 us (559 TFLOP/s, a third of a library product's rate; 12000 cycles of a
 // CTA are its start and end); 1530 rows of seven sequences, 32 heads over 8 kv heads, behind 8963
 // positions 93 us.  Scores taken 32 at a time, in half the code and registers: 60.3 and 98.8; 152 registers for the softmax warps, 80 for
 // the loading ones: 58.0 and 93.6.

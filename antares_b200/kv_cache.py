@@ -45,7 +45,8 @@ class PagePool:
         return seq
 
     def fork(self, seq):
-        """A sequence with the same rows.  Nothing is copied: whichever writes into a shared page first gets its own (reserve)."""
+        """A sequence with the same rows.  Nothing is copied: whichever writes into a shared page first gets its own (reserve).  Rows
+        that were reserved and not written are shared as well: reserve again before they are."""
         self._known(seq)
         new = self.add()
         self.held[new], self.rows[new] = list(self.held[seq]), self.rows[seq]
@@ -138,7 +139,9 @@ class PagePool:
 class PagedKV8Cache:
     """The 8-bit cache of a model's layers.  layer(l) is what the ops.kv8_* calls take, batch(seqs) their page table and
     positions (columns without a page hold -1: rows that were not reserved are not written, and kernel_status says so).  A
-    serving step: reserve({seq: rows}), then per layer kv8_step or kv8_append + kv8_attention, then advance()."""
+    serving step: reserve({seq: rows}), then per layer kv8_step or kv8_append + kv8_attention, then advance().  max_seq: the rows a
+    sequence may get to (None: all pages' rows).  It is what a batch's table has room for, and kernels are chosen by that: a
+    server that knows its longest request says so."""
 
     def __init__(self, layers, pages, kv_heads, page_rows=64, max_seqs=64, max_seq=None, device="cuda"):
         if page_rows < 16 or page_rows & (page_rows - 1):
