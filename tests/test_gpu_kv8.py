@@ -760,17 +760,10 @@ def test_a_serving_step_does_not_wait_for_the_gpu(cuda):
     """reserve, batch, append, attention, step, fork, compact and advance queue their work and return; what batch() uploads is what
     it was called for, however late the copy runs."""
     from antares_b200.kv_cache import PagedKV8Cache
-    c = PagedKV8Cache(1, 40, 2, page_rows=16, max_seqs=8, max_seq=256)
     k, q = _randn(1, 40, 2, 128), _randn(2, 40, 4, 128)
-    cu = _ints([0, 20, 40])
-    for f in (ops.kv8_append, lambda *a, **kw: ops.kv8_attention(q, c.layer(0), *a[3:], **kw)):   # first calls load kernels
-        f(c.layer(0), k, k, *(t.cuda() for t in (torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))), cu_rows=cu)
-    torch.cuda.synchronize()
-    torch.cuda.set_sync_debug_mode("error")
-    busy, idle = torch.cuda.Event(), []
-    try:
-        torch.cuda._sleep(800_000_000)   # some 400 ms
-        busy.record()
+    cu, busy = _ints([0, 20, 40]), torch.cuda.Event()
+
+    def serve(c):
         a, b = c.add(), c.add()
         c.reserve({a: 20, b: 20})
         table, pos0 = c.batch([a, b])
@@ -789,9 +782,21 @@ def test_a_serving_step_does_not_wait_for_the_gpu(cuda):
                 c.advance(s, 1)
         c.free(b)
         c.compact()
-        idle.append(busy.query())
+        return seen
+
+    make = lambda: PagedKV8Cache(1, 40, 2, page_rows=16, max_seqs=8, max_seq=256)  # noqa: E731
+    keep = serve(make())   # the first call of each kind loads its kernel and gets memory from the driver, which both wait
+    c = make()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        torch.cuda._sleep(3_000_000_000)   # over a second
+        busy.record()
+        seen = serve(c)
+        idle = [busy.query()]
     finally:
         torch.cuda.set_sync_debug_mode("default")
+    del keep
     assert idle == [False]
     torch.cuda.synchronize()
     for table, pos0, held, rows in seen:
@@ -891,3 +896,24 @@ def test_fp16_rows_of_the_few_row_kernel_hold_p_in_22_bits(cuda, past, rows, hq,
     tight, loose = (kv8_ref.bound(want, spread, score, tiny, keys, F16, one) for one in (False, True))
     off = np.abs(got - want) / np.where(single, loose, tight)
     assert off.max() <= 1, (off.max(), np.unravel_index(off.argmax(), off.shape))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("past,rows,hq,hkv,page", [CASES[i] for i in (2, 3, 6, 8, 14, 18, 19, 20, 22)])
+def test_results_over_the_queries_and_scratch_of_the_caller(cuda, past, rows, hq, hkv, page, wide, dtype):
+    """out=q and a workspace of just the size that is asked for, filled with NaN: the bits of a new result."""
+    cache, table = _setup(len(past) + sum(rows), past, rows, hkv, page)
+    table = _wide(table, page) if wide else table
+    S, T, cu = len(past), sum(rows), None if len(set(rows)) == 1 else _cu(rows)
+    q, pos0 = _randn(1, T, hq, 128, dtype=dtype), _ints(past)
+    want = ops.kv8_attention(q, cache, table, pos0, cu_rows=cu, max_rows=max(rows))
+    n = ops.kv8_attention_workspace_bytes(S, T, max(rows), hq, hkv)
+    room = torch.full((n + 4096,), 255, dtype=torch.uint8, device="cuda")
+    keep = q.clone()
+    assert torch.equal(ops.kv8_attention(q, cache, table, pos0, cu_rows=cu, max_rows=max(rows), workspace=room[:n]), want) and torch.equal(q, keep)
+    assert ops.kv8_attention(q, cache, table, pos0, cu_rows=cu, max_rows=max(rows), out=q, workspace=room[:n]) is q
+    assert torch.equal(q, want) and (room[n:] == 255).all()
+    with pytest.raises(_lib.Ab200Error, match="workspace"):
+        ops.kv8_attention(q, cache, table, pos0, cu_rows=cu, max_rows=max(rows), workspace=room[:64])
+    assert ops.kernel_status() == 0
