@@ -191,6 +191,8 @@ class PagedKV8Cache:
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence is in a batch once, got %r" % (list(seqs),))
         n, width, device = len(seqs), self.pool.max_pages, self.k.device
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("batch() is not captured: it uploads what the host knows now (call it before, and copy its result where the captured calls read)")
         # one upload, from pinned memory that torch keeps until the copy has run: nothing waits for the GPU
         host = torch.full((n * (width + 1),), -1, dtype=torch.int32, pin_memory=device.type == "cuda")
         table = host[:n * width].view(n, width)

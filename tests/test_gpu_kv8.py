@@ -917,3 +917,21 @@ def test_results_over_the_queries_and_scratch_of_the_caller(cuda, past, rows, hq
     with pytest.raises(_lib.Ab200Error, match="workspace"):
         ops.kv8_attention(q, cache, table, pos0, cu_rows=cu, max_rows=max(rows), workspace=room[:64])
     assert ops.kernel_status() == 0
+
+
+def test_a_batch_is_not_captured(cuda):
+    """batch() uploads what the host knows now; a graph would keep the upload and replay it from memory that is another call's."""
+    from antares_b200.kv_cache import PagedKV8Cache
+    c = PagedKV8Cache(1, 8, 2, page_rows=16)
+    a = c.add()
+    c.reserve({a: 3})
+    want = c.batch([a])
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device="cuda")
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="captured"):
+            c.batch([a])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (x == 1).all() and all(torch.equal(t, w) for t, w in zip(c.batch([a]), want))
