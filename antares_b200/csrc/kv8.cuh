@@ -34,6 +34,10 @@ struct Kv8Rows {
   __device__ __forceinline__ int end(int s) const { return cu ? min(max(cu[s + 1], 0), T) : s * n + n; }
 };
 
+// A row's sum of P / vs is held times this: beside values of scale 0, which counts as 2^-100, P is up to 2^15, so a key adds up to 2^115 and
+// some thousands of them would be infinite; with it 2^22 keys are not, and a scale of 2^118 still leaves 2^-122.
+constexpr float KV8_SUM = 0x1p-10f;
+
 // 2^e, exact: -149 <= e <= 127.  A query's largest value can lie at either end of fp32, and 2^e that brings it to a fixed size beyond
 // both: that one goes in two steps.
 __device__ __forceinline__ float kv8_pow2(int e) { return __int_as_float(e >= -126 ? (127 + e) << 23 : 1 << (149 + e)); }

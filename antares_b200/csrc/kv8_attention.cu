@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       for (int u = 0; u < 2; ++u) {
         const float ks = (u ? scales.z : scales.x) * p.scale, vs = fmaxf(u ? scales.w : scales.y, KD_LEAST_SCALE);
         const float lvs = kd_lg2(vs);
-        inv_vs[u] = kd_rcp(vs);
+        inv_vs[u] = kd_rcp(vs) * KV8_SUM;
         // q . k: bytes times bytes, exact
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb) {
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
       T *out = (T *)p.out + ((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + col;
       // a part to be joined: FIXED into the ring's other half, else to memory
       float *part = FIXED ? reinterpret_cast<float *>(smem) + row * KV8_D + col : p.partial + (((size_t)blockIdx.x * 2 + slot) * ROWS + row) * KV8_D + col;
-      const float over = row < empty ? 0.f : 1.f / sum;
+      const float over = row < empty ? 0.f : KV8_SUM / sum;
 #pragma unroll
       for (int c = 0; c < PIECES; ++c) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
             acc = fmaf(*cluster.map_shared_rank(reinterpret_cast<float *>(smem) + row * KV8_D + tid, i), f, acc);
           }
           const int packed = done.first + row, token = packed / p.group, head = done.hk * p.group + packed - token * p.group;
-          ((T *)p.out)[((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + tid] = (T)(row < empty ? 0.f : acc / sum);
+          ((T *)p.out)[((size_t)(done.row0 + token) * p.Hq + head) * KV8_D + tid] = (T)(row < empty ? 0.f : acc * (KV8_SUM / sum));
         }
         cluster.sync();  // nobody leaves while its memory is read
       }
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(KJ_THREADS) kv8_join_kernel(const __grid_const
     const int packed = sp.w + row, token = packed / p.group, head = (sp.z & 0xFFFF) * p.group + packed - token * p.group;
     T *out = (T *)p.out + ((size_t)(sp.y + token) * p.Hq + head) * KV8_D + 4 * lane;
     const bool none = row < sp.z >> 20;
-    kd_store4(out, a.acc, none ? 0.f : 1.f / a.l);
+    kd_store4(out, a.acc, none ? 0.f : KV8_SUM / a.l);
   };
   // the parts of an item that two CTAs share, before it is known whether there is one
   float2 s0[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};

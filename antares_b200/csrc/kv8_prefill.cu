@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
   __shared__ uint32_t tmem_s;
   __shared__ int fail_s, seq_s;
   __shared__ float2 scales_s[4 * TILES][2][KP_BLOCKS];  // a softmax warp's own, of two tiles: factor of the scores, log2(vs)
-  __shared__ float over_s[4 * TILES][2][KP_BLOCKS];     // 1 / vs
+  __shared__ float over_s[4 * TILES][2][KP_BLOCKS];     // 1 / vs, times KV8_SUM
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Kv8Rows &r = p.r;
   pdl_wait();
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
     auto scales = [&](int j) {  // of tile j, whose values have come, to shared memory; asks for the next tile's
       if (lane < KP_BLOCKS) {
         const float vs = fmaxf(vs_next, KP_LEAST_SCALE);
-        scales_s[warp][j & 1][lane] = make_float2(ks_next * scale, __log2f(vs)), over_s[warp][j & 1][lane] = __fdividef(1.f, vs);
+        scales_s[warp][j & 1][lane] = make_float2(ks_next * scale, __log2f(vs)), over_s[warp][j & 1][lane] = __fdividef(KV8_SUM, vs);
       }
       ask(j + 1);
     };
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(KpShape<TILES, PARTS>::THREADS, 1) kv8_prefill
         }
         p.partial_ml[at] = make_float2(my_n > 0 ? m : -CUDART_INF_F, my_n > 0 ? l : 0.f);
       } else {
-        const float over = limit > 0 ? 1.f / l : 0.f;
+        const float over = limit > 0 ? KV8_SUM / l : 0.f;
         constexpr int CHUNKS = KV8_D * sizeof(T) / 16, EACH = 16 / sizeof(T);
         unsigned char *park = q_s + mine * (KV8_D * sizeof(T));
 #pragma unroll 1
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(KP_JOIN_WARPS * 32) kv8_prefill_join_kernel(co
   const float x[4] = {acc.x, acc.y, acc.z, acc.w};
   const bool none = p.r.pos0[place.seq] + (long)(packed / p.group) < 0;  // nothing to attend to; keys whose scores are all -inf have no softmax: 0 / 0
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(none ? 0.f : x[e] / l);
+  for (int e = 0; e < 4; ++e) out[e] = (T)(none ? 0.f : x[e] * (KV8_SUM / l));
 }
 
 template <typename T, int TILES, int PARTS>

@@ -935,3 +935,31 @@ def test_a_batch_is_not_captured(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert (x == 1).all() and all(torch.equal(t, w) for t, w in zip(c.batch([a]), want))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("seqs,rows,group", [(76, 66, 1), (1, 66, 1), (150, 130, 1), (76, 1, 1), (500, 1, 1), (700, 1, 16), (1, 1, 8), (20, 9, 8)])
+def test_many_keys_of_scale_zero_before_one_that_counts(cuda, seqs, rows, group, dtype):
+    """20000 keys without values, nearly 2^8 times the weight of the first ones, then one key beside which they all are nothing: its
+    values are the result, to 2^-30."""
+    past = 20000
+    cache, table = _setup(73, [past], [rows], 1, 64)
+    for t, fill in zip(cache, (79, 0, 0.02, 0.0)):
+        t.fill_(fill)
+    at = lambda p: (int(table[0, p // 64]), 0, p % 64)  # noqa: E731
+    for p in range(128):
+        cache[0][at(p)] = 0
+    cache[2][int(table[0, past // 64]), 0, past % 64 // 16] = 0.2      # the block of position 20000, a first one: its keys alone ...
+    cache[3][int(table[0, past // 64]), 0, past % 64 // 16] = 0.25
+    for p in range(past + 1, past - past % 16 + 16):                   # ... the first of which counts
+        cache[0][at(p)] = 0
+    values = torch.randint(-127, 128, (128,), generator=torch.Generator().manual_seed(1)).to(torch.int8).cuda()
+    cache[1][at(past)] = values
+    # 7.9 octaves for 79 * 0.02, 79 for 79 * 0.2
+    q = torch.full((seqs * rows, group, 128), 7.9 / (79 * 0.02 * 128 ** 0.5 * 1.4426950408889634), dtype=dtype, device="cuda")
+    got = ops.kv8_attention(q, cache, table.expand(seqs, -1), _ints([past] * seqs))
+    want = (values.double() * 0.25).expand_as(got)
+    # half a step of the result, half a step of one fp16 P (fp16 rows of the prompt kernel), the pair's and the exponential's 2^-20
+    off = (got.double() - want).abs() / (want.abs() * (torch.finfo(dtype).eps / 2 * 1.01 + (2.0 ** -11 if dtype == F16 else 0) + 2.0 ** -20) + 1e-30)
+    assert past % 16 == 0 and off.max() <= 1, (off.max(), got.isnan().sum())
+    assert ops.kernel_status() == 0
