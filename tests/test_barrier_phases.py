@@ -22,7 +22,7 @@ class Stuck(Exception):
 
 def explore(mma, warps, counts):
     """Runs every order.  mma: ("wait", barrier, parity), ("issue", product) and ("commit", barrier); warps: also ("arrive", barrier) and
-    ("needs", product), which must be complete then.  counts: arrivals that end a phase of each barrier."""
+    ("needs", product), which must be complete then, and ("first", product), which must not have been issued yet.  counts: arrivals that end a phase of each barrier."""
     names = sorted(counts)
     at = {b: i for i, b in enumerate(names)}
     programs = [mma] + warps
@@ -51,6 +51,9 @@ def explore(mma, warps, counts):
                     continue
             elif op[0] == "arrive":
                 b = arrive(bars, op[1])
+            elif op[0] == "first":
+                if op[1] in done or ("issue", op[1]) in queue:
+                    raise Stuck("%s is issued too early" % (op[1],))
             elif op[0] == "needs":
                 if op[1] not in done:
                     raise Stuck("%s is used before it is complete" % (op[1],))
@@ -84,6 +87,8 @@ def _kv8(n, parts, raises):
             mma += [("issue", ("s", j + 1, 1)), ("commit", "s1")]
     warp = []
     for j in range(n):
+        if parts == 2 and j > 0:  # fp32 rows: the product of the tile before is added to the others before the next may take its place
+            warp += [("wait", "o", (j - 1) & 1), ("needs", ("o", j - 1)), ("first", ("o", j))]
         warp += [("wait", "s0", j & 1), ("needs", ("s", j, 0))]
         if raises and j > 0:  # the first half waits itself, the other's scores were only issued after the product of the tile before
             warp += ([("wait", "o", (j - 1) & 1)] if parts == 1 else []) + [("needs", ("o", j - 1))]

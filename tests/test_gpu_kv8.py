@@ -963,3 +963,43 @@ def test_many_keys_of_scale_zero_before_one_that_counts(cuda, seqs, rows, group,
     off = (got.double() - want).abs() / (want.abs() * (torch.finfo(dtype).eps / 2 * 1.01 + (2.0 ** -11 if dtype == F16 else 0) + 2.0 ** -20) + 1e-30)
     assert past % 16 == 0 and off.max() <= 1, (off.max(), got.isnan().sum())
     assert ops.kernel_status() == 0
+
+
+def _exact_on_gpu(q, cache, table, past, rows):
+    """Rows of sequences as long as one another, float64 [S rows, Hq, 128]."""
+    S, hkv, hq = len(table), cache[0].shape[1], q.shape[1]
+    out = torch.empty(q.shape, dtype=torch.float64, device="cuda")
+    for s in range(S):
+        k, v = ((c[table[s].long()].double() * sc[table[s].long()].double().repeat_interleave(16, -1)[..., None]).permute(1, 0, 2, 3).reshape(hkv, -1, 128)
+                for c, sc in ((cache[0], cache[2]), (cache[1], cache[3])))
+        limit = past + 1 + torch.arange(rows, device="cuda")
+        for h in range(hq):
+            x = q[s * rows:(s + 1) * rows, h].double() @ k[h // (hq // hkv), :past + rows].T * 128 ** -0.5
+            x.masked_fill_(torch.arange(past + rows, device="cuda") >= limit[:, None], float("-inf"))
+            out[s * rows:(s + 1) * rows, h] = torch.softmax(x, -1) @ v[h // (hq // hkv), :past + rows]
+    return out
+
+
+def _check_sums(seqs, past, rows, hq, hkv, hint, wide):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    page, need = 64, -(-(past + rows) // 64)
+    codes = [(40 * torch.randn(seqs * need, hkv, page, 128, device="cuda", generator=g)).round().clamp(-127, 127).to(torch.int8) for _ in range(2)]
+    cache = codes + [0.02 + 0.01 * torch.rand(seqs * need, hkv, page // 16, device="cuda", generator=g) for _ in range(2)]
+    table = torch.arange(seqs * need, device="cuda").int().view(seqs, need)
+    q = torch.randn(seqs * rows, hq, 128, device="cuda", generator=g)
+    cu = _ints([i * rows for i in range(seqs + 1)]) if hint else None
+    got = ops.kv8_attention(q, cache, _wide(table, page) if wide else table, _ints([past] * seqs), cu_rows=cu, max_rows=hint).double()
+    some = min(seqs, 3)
+    want, got = _exact_on_gpu(q[:some * rows], cache, table[:some], past, rows), got[:some * rows]
+    bias = float(((got - want) * want).sum() / (want * want).sum())
+    off = float((got - want).norm() / want.norm())
+    # Added up in fp32 that rounds, errors have no sign.  A product's own sum takes 8 steps (with two blocks of keys: 4), cut towards zero by
+    # at most 2^-23 of what it holds, on average half of a whole sum: 2^-21.  In all: that, scores of 2^-19 of their size (a few, and
+    # half of them of either sign) and 2^-20 for weights and their exponentials: 2^-19 of the result's norm.
+    assert abs(bias) <= 2.0 ** -21 and off <= 2.0 ** -19, (bias, off)
+    assert ops.kernel_status() == 0
+
+
+@pytest.mark.parametrize("seqs,past,rows,hq,hkv", [(1, 16000, 300, 8, 2), (1, 2000, 300, 160, 160), (76, 20000, 70, 1, 1)])
+def test_sums_of_fp32_prompts_over_many_keys(cuda, seqs, past, rows, hq, hkv):
+    _check_sums(seqs, past, rows, hq, hkv, None, True)
