@@ -18,7 +18,7 @@
 // 32 kv heads 170 (6.3); one of 131072 and 8 kv heads 54 (5.0); 64 ragged ones of up to 8000, 8 heads of 8 107 (5.2).  Where a share is
 // small, starting an item (7800 cycles) and the second launch weigh: 48 ragged ones of up to 4000 45 us (4.4), of one request of
 // 384 positions 6.7 us only a tenth is the stream.  16 rows a tile: products and exponentials bound it, twice a block's instructions.
-// Registers and bytes spilled, equal shares: 8 rows 168 and 64 (fp32 76), three CTAs an SM; 16 rows 255 and 24 (fp32 36), two.
+// Registers and bytes spilled, equal shares: 8 rows 168 and 64 (fp32 80), three CTAs an SM; 16 rows 255 and 32 (fp32 12), two.
 #include <math_constants.h>
 
 #include <cooperative_groups.h>
@@ -35,6 +35,7 @@ constexpr int KD_WARPS = 4, KD_THREADS = KD_WARPS * 32, KD_STAGES = 4;
 constexpr int KD_STAGE_BYTES = 2 * KV8_BLOCK * KV8_D;  // a block of K, a block of V
 constexpr int KD_LEAST = 8;                            // blocks a CTA takes at least, two a warp
 constexpr int KD_ITEM = 16;                            // what an item costs besides its blocks, in blocks: 7800 cycles against 470 a block
+constexpr int KD_CUT = 64;                             // blocks that a CTA adds up in the tensor cores alone, fp32 rows
 constexpr float KD_RAISE = 8.f, KD_P_EXP = 6.f;        // P is scaled by 2^6: its second half stays out of fp16's subnormals
 constexpr float KD_LEAST_SCALE = 0x1p-100f;            // a V scale below it (a block of zeros) counts as this
 
@@ -65,6 +66,11 @@ __device__ __forceinline__ void kd_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void kd_mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {  // of a sum: adds to nothing
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 // The first product of a chain starts from KD_ZERO: an integer below 2^22 added to these bits is that integer plus 1.5 * 2^23
 // as a float, so a subtraction reads the sum and nothing is converted.
@@ -578,22 +584,44 @@ __global__ void __launch_bounds__(KD_THREADS, ROWS == 8 ? 3 : 2) kv8_decode_kern
           l[n] = fmaf(sum, inv_vs[u], l[n]);
         }
       }
+      // keys 0-7 and 8-15 of piece c, then of piece c + 1; transposed: two keys, two dims a word
+      auto values = [&](int u, int c, uint32_t(&v)[4]) { kd_ldsm_t(v, st + u * KD_STAGE_BYTES + v_row + (((c + v_chunk) ^ v_sw) << 4)); };
+      auto product = [&](float(&even)[4], float(&odd)[4], const uint32_t(&p_)[4], uint32_t v0, uint32_t v1, bool first) {
+        const uint32_t u0 = v0 ^ 0x80808080u, u1 = v1 ^ 0x80808080u;
+        const uint32_t e0 = kd_half2<0x4240>(u0), e1 = kd_half2<0x4240>(u1), d0 = kd_half2<0x4341>(u0), d1 = kd_half2<0x4341>(u1);
+        if (first) kd_mma_first(even, p_[0], p_[1], p_[2], p_[3], e0, e1), kd_mma_first(odd, p_[0], p_[1], p_[2], p_[3], d0, d1);
+        else kd_mma(even, p_[0], p_[1], p_[2], p_[3], e0, e1), kd_mma(odd, p_[0], p_[1], p_[2], p_[3], d0, d1);
+      };
+      if constexpr (sizeof(T) == 2 || FIXED) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < 8; c += 2) {
+            uint32_t v[4];
+            values(u, c, v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int n = 0; n < NR; ++n) product(o[2 * (c + h)], o[2 * (c + h) + 1], pa[u][n], v[2 * h], v[2 * h + 1], false);
+          }
+      } else {
+        // fp32 rows: the tensor cores cut what they add to 24 bits, always towards zero, 3e-6 of a sum over 16000 keys.  So two blocks'
+        // product is a sum of its own, the low halves of P first, and joins the others by an addition that rounds.  A cluster's CTA has
+        // KD_CUT blocks at most, in which 2e-7 are cut, and keeps its shorter code.  us, one sum / sums of two blocks: 5 sequences of up to 1000
+        // positions 13.2 / 13.7, 64 of 16000 332 / 331, 16 times four rows 59 / 64.
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
-          uint32_t v[4];
-          // keys 0-7 and 8-15 of piece c, then of piece c + 1; transposed: two keys, two dims a word
-          kd_ldsm_t(v, st + u * KD_STAGE_BYTES + v_row + (((c + v_chunk) ^ v_sw) << 4));
+          uint32_t v[2][4];
+          values(0, c, v[0]), values(1, c, v[1]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t u0 = v[2 * h] ^ 0x80808080u, u1 = v[2 * h + 1] ^ 0x80808080u;
-            const uint32_t e0 = kd_half2<0x4240>(u0), e1 = kd_half2<0x4240>(u1), d0 = kd_half2<0x4341>(u0), d1 = kd_half2<0x4341>(u1);
+            float even[4], odd[4];
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-              kd_mma(o[2 * (c + h)], pa[u][n][0], pa[u][n][1], pa[u][n][2], pa[u][n][3], e0, e1);
-              kd_mma(o[2 * (c + h) + 1], pa[u][n][0], pa[u][n][1], pa[u][n][2], pa[u][n][3], d0, d1);
-            }
+            for (int n = NR - 1; n >= 0; --n)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) product(even, odd, pa[u][n], v[u][2 * h], v[u][2 * h + 1], n == NR - 1 && u == 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[2 * (c + h)][e] += even[e], o[2 * (c + h) + 1][e] += odd[e];
           }
         }
       }
@@ -762,7 +790,7 @@ struct DecodePlan {
   int tiles;
   size_t partial_bytes, bytes;
 };
-static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool uniform, long capacity) {
+static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool uniform, long capacity, int dtype) {
   DecodePlan d;
   const long group = Hq / Hkv;
   d.rows = (long)max_rows * group <= 8 ? 8 : 16;
@@ -779,7 +807,8 @@ static DecodePlan decode_plan(int S, int T, int max_rows, int Hq, int Hkv, bool 
   if (uniform && items <= d.ctas) {
     int c = 1;
     while (c < 8 && items * c * 2 <= d.ctas) c *= 2;
-    if ((blocks + c - 1) / c <= items * blocks / (S == 1 ? 1 : 2) / d.ctas + 24) d.splits = c;
+    const long each = (blocks + c - 1) / c;
+    if (each <= items * blocks / (S == 1 ? 1 : 2) / d.ctas + 24 && (dtype == AB200_F16 || each <= KD_CUT)) d.splits = c;
   }
   return d;
 }
@@ -837,7 +866,7 @@ static int attend_plan(const Kv8Cache &c, const Kv8Rows &r, int max_rows, int Hq
   const long capacity = (long)r.max_pages << c.shift, most = r.cu ? max_rows : r.n;
   a->prompts = most * group > KD_FEW && (long)r.T * Hq * capacity > KD_PROMPT_WORK && !rotate;
   a->few = !a->prompts || r.cu != nullptr;
-  a->d = decode_plan(r.S, r.T, a->few && a->prompts ? std::max(KD_FEW / group, 1) : (int)most, Hq, c.H, r.cu == nullptr, capacity);
+  a->d = decode_plan(r.S, r.T, a->few && a->prompts ? std::max(KD_FEW / group, 1) : (int)most, Hq, c.H, r.cu == nullptr, capacity, dtype);
   a->p = Kv8PrefillParams{};
   a->p.c = c, a->p.r = r, a->p.group = group;
   size_t prompt_bytes = 0;

@@ -1003,3 +1003,9 @@ def _check_sums(seqs, past, rows, hq, hkv, hint, wide):
 @pytest.mark.parametrize("seqs,past,rows,hq,hkv", [(1, 16000, 300, 8, 2), (1, 2000, 300, 160, 160), (76, 20000, 70, 1, 1)])
 def test_sums_of_fp32_prompts_over_many_keys(cuda, seqs, past, rows, hq, hkv):
     _check_sums(seqs, past, rows, hq, hkv, None, True)
+
+
+@pytest.mark.parametrize("seqs,past,rows,hq,hkv,hint", [(64, 16000, 1, 32, 8, None), (400, 8000, 1, 8, 1, None), (40, 16000, 4, 32, 8, None), (1, 16000, 300, 8, 2, 1), (3, 16000, 9, 8, 8, 9),
+                                                            (1, 8000, 1, 222, 222, None), (1, 7000, 1, 32, 32, None)])
+def test_sums_of_few_fp32_rows_over_many_keys(cuda, seqs, past, rows, hq, hkv, hint):
+    _check_sums(seqs, past, rows, hq, hkv, hint, False)
